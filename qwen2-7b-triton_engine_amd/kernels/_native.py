@@ -107,6 +107,23 @@ SIGNATURES = {
     "awq_w4a16_gemm_noalloc": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I32, _VP]),
 }
 
+# The same for include/awq_serving.h.
+_SZ = ctypes.c_size_t
+SERVING_SIGNATURES = {
+    "awq_serve_page_step": (ctypes.c_int, [_VP] * 9 + [_I64] * 5 + [_VP]),
+    "awq_serve_page_release": (ctypes.c_int, [_VP] * 5 + [_I64] * 4 + [_VP]),
+    "awq_serve_kv4_append": (ctypes.c_int, [_VP, _I64] + [_VP] * 6 + [_I64] * 8 + [_I32, _VP]),
+    "awq_serve_kv4_gather": (ctypes.c_int, [_VP] * 4 + [_I64] * 6 + [_I32, _VP]),
+    "awq_serve_kv4_attention_workspace": (_SZ, [_I64] * 8),
+    "awq_serve_kv4_attention": (ctypes.c_int, [_VP, _I64] + [_VP] * 5 + [_I64] * 10 + [ctypes.c_float, _I32, _VP, _SZ, _VP]),
+    "awq_serve_logits_workspace": (_SZ, [_I64] * 2),
+    "awq_serve_logits": (ctypes.c_int, [_VP, _I64, _VP, _VP, _I64, _I64, _I32, _VP, _I32, _I64] + [_VP] * 8 +
+                         [_I64, _VP, _VP, _SZ, _VP]),
+}
+SERVE_FP16, SERVE_BF16, SERVE_FP32 = 0, 1, 2
+SERVE_MAX_REQUESTS = 4096
+SERVE_MAX_GROUP = 64
+
 _lib = None
 _binding = None
 
@@ -155,7 +172,7 @@ def lib() -> ctypes.CDLL:
                 f"W4A16 AWQ HIP library not found at {LIB_PATH}; build it with "
                 "`python qwen2-7b-triton_engine_amd/build.py` (there is no fallback path)")
         L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in (*SIGNATURES.items(), *SERVING_SIGNATURES.items()):
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

@@ -1,0 +1,172 @@
+"""Block tables, slots and positions of a serving step, built on the GPU from
+the requests' lengths (``awq_serve_page_step``, ``awq_serve_page_release``).
+
+A cache of pages is shared by up to ``MAX_REQUESTS`` requests (``PagedTables``):
+which pages a request has, how many tokens it holds, and which pages are free.
+``paged_step`` adds a step's new tokens -- one each while decoding, a prompt or a
+chunk of one before -- and returns a ``PagedStep``: where each row of the batch is
+stored and which position it stands at, and the state after the step.  It
+changes neither lengths nor free pages until ``PagedTables.commit``, so a step in
+which a request was refused (``PagedStep.failed``) can be given up or made smaller.
+The reference has one static cache and one sequence
+(``inference/kv_cache.py:31-67``); these have no counterpart there.
+"""
+from __future__ import annotations
+
+import dataclasses
+
+import torch
+
+from . import _native
+from .awq_gemm import _OnDevice, _stream_handle
+
+__all__ = ["PagedTables", "PagedStep", "paged_step", "paged_release", "MAX_REQUESTS", "PAGE_SIZES"]
+
+MAX_REQUESTS = _native.SERVE_MAX_REQUESTS
+PAGE_SIZES = (16, 32, 64, 128, 256)
+_INT_MAX = 2**31 - 1
+
+
+def _check_i32(t: torch.Tensor, what: str, shape: tuple, dev: torch.device) -> None:
+    if t.dtype is not torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{what} must be a contiguous int32 tensor {shape} on {dev}, got {t.dtype} {tuple(t.shape)} "
+                         f"on {t.device}")
+
+
+@dataclasses.dataclass
+class PagedTables:
+    """``block_tables`` int32 ``[requests, width]``: the pages of each request in
+    order; ``state`` int32 ``[requests + 1]``: the requests' lengths, then the
+    number of free pages; ``free_pages`` int32 ``[num_pages]``, the first
+    ``state[-1]`` of them free, taken from the end."""
+
+    block_tables: torch.Tensor
+    state: torch.Tensor
+    free_pages: torch.Tensor
+    page_size: int
+
+    def __init__(self, requests: int, width: int, num_pages: int, page_size: int = 64,
+                 device: torch.device | str = "cuda:0"):
+        dev = torch.device(device)
+        self._set(torch.full((requests, width), -1, dtype=torch.int32, device=dev),
+                  torch.zeros(requests + 1, dtype=torch.int32, device=dev),
+                  # from the end: page 0 is taken first
+                  torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=dev), page_size)
+        self.state[-1] = num_pages
+
+    @classmethod
+    def of(cls, block_tables: torch.Tensor, state: torch.Tensor, free_pages: torch.Tensor,
+           page_size: int = 64) -> "PagedTables":
+        """Tables over tensors that exist; they are used in place."""
+        t = cls.__new__(cls)
+        t._set(block_tables, state, free_pages, page_size)
+        return t
+
+    def _set(self, block_tables, state, free_pages, page_size):
+        if block_tables.dim() != 2 or free_pages.dim() != 1:
+            raise ValueError("block_tables must be 2-D and free_pages 1-D")
+        requests, width = block_tables.shape
+        dev = block_tables.device
+        _check_i32(block_tables, "block_tables", (requests, width), dev)
+        _check_i32(state, "state", (requests + 1,), dev)
+        _check_i32(free_pages, "free_pages", (free_pages.shape[0],), dev)
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size {page_size} must be one of {PAGE_SIZES}")
+        if not 0 < requests <= MAX_REQUESTS or width < 1 or free_pages.shape[0] < 1:
+            raise ValueError(f"{requests} requests of {width} pages, {free_pages.shape[0]} pages in all: need 1 to "
+                             f"{MAX_REQUESTS} requests and at least one page")
+        if width > _INT_MAX // page_size - 1 or free_pages.shape[0] > _INT_MAX // page_size:
+            raise ValueError("token numbers pass 32 bits")
+        self.block_tables, self.state, self.free_pages, self.page_size = block_tables, state, free_pages, page_size
+
+    @property
+    def lengths(self) -> torch.Tensor:
+        return self.state[:-1]
+
+    @property
+    def free_count(self) -> torch.Tensor:
+        return self.state[-1:]
+
+    def commit(self, step: "PagedStep") -> None:
+        """The step's lengths and free pages become the tables' (the tensor itself: no copy)."""
+        if step.state.shape != self.state.shape or step.state.device != self.state.device:
+            raise ValueError("the step belongs to other tables")
+        self.state = step.state
+
+
+@dataclasses.dataclass
+class PagedStep:
+    """``slots`` and ``positions`` int32 ``[total]`` of the batch's rows (-1: no token),
+    ``query_start`` int32 ``[requests + 1]`` the requests' first rows, ``state`` as the
+    tables' after the step (``lengths`` of it: with the new tokens), ``failed`` int32
+    ``[requests]``, 1 where a request was refused."""
+
+    state: torch.Tensor
+    query_start: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    failed: torch.Tensor
+
+    @property
+    def lengths(self) -> torch.Tensor:
+        return self.state[:-1]
+
+    @classmethod
+    def empty(cls, requests: int, total: int, device: torch.device) -> "PagedStep":
+        # one allocation: an allocator call costs about as much as the launch
+        sizes = (requests + 1, requests + 1, total, total, requests)
+        flat = torch.empty(sum(sizes), dtype=torch.int32, device=device)
+        return cls(*flat.split(sizes))
+
+
+def paged_step(tables: PagedTables, new_tokens: torch.Tensor, total: int, out: PagedStep | None = None) -> PagedStep:
+    """The rows of ``new_tokens`` (int32 ``[requests]``) more tokens of each request in a
+    batch of ``total`` rows, the first request's first.  New pages are entered into
+    ``tables.block_tables``; lengths and free pages change with ``tables.commit``.
+
+    A request is refused -- ``failed`` 1, slots and positions -1, nothing taken -- whose
+    rows pass ``total``, whose tokens pass its table's width, or for which and all
+    before it the free pages do not suffice.  ``out``: a step of the same sizes
+    whose tensors are reused (not the one whose ``state`` the tables hold)."""
+    requests, width = tables.block_tables.shape
+    dev = tables.state.device
+    if dev.type != "cuda":
+        raise ValueError(f"the tables must be on a ROCm device, got {dev}")
+    if new_tokens.dtype is not torch.int32 or new_tokens.shape != (requests,) or new_tokens.device != dev \
+            or not new_tokens.is_contiguous():
+        raise ValueError(f"new_tokens must be a contiguous int32 tensor {(requests,)} on {dev}")
+    if total < 0 or total > _INT_MAX // 2:
+        raise ValueError(f"total {total} must be in [0, {_INT_MAX // 2}]")
+    if out is None:
+        out = PagedStep.empty(requests, total, dev)
+    else:
+        for name, n in (("state", requests + 1), ("query_start", requests + 1), ("slots", total), ("positions", total),
+                        ("failed", requests)):
+            _check_i32(getattr(out, name), f"out.{name}", (n,), dev)
+        if out.state.data_ptr() == tables.state.data_ptr():
+            raise ValueError("out.state is the tables' own state: the step reads it while it writes")
+    with _OnDevice(dev):
+        st = _native.lib().awq_serve_page_step(
+            tables.state.data_ptr(), new_tokens.data_ptr(), tables.block_tables.data_ptr(),
+            tables.free_pages.data_ptr(), out.state.data_ptr(), out.query_start.data_ptr(), out.slots.data_ptr(),
+            out.positions.data_ptr(), out.failed.data_ptr(), requests, total, width, tables.free_pages.shape[0],
+            tables.page_size, _stream_handle(dev))
+    _native.check(st, "awq_serve_page_step")
+    return out
+
+
+def paged_release(tables: PagedTables, keep: torch.Tensor) -> None:
+    """Request b keeps its first ``keep[b]`` tokens (int32 ``[requests]``; 0: the request
+    ended) and returns the pages past them."""
+    requests, width = tables.block_tables.shape
+    dev = tables.state.device
+    if dev.type != "cuda":
+        raise ValueError(f"the tables must be on a ROCm device, got {dev}")
+    _check_i32(keep, "keep", (requests,), dev)
+    state = torch.empty_like(tables.state)
+    with _OnDevice(dev):
+        st = _native.lib().awq_serve_page_release(
+            tables.state.data_ptr(), keep.data_ptr(), tables.block_tables.data_ptr(), tables.free_pages.data_ptr(),
+            state.data_ptr(), requests, width, tables.free_pages.shape[0], tables.page_size, _stream_handle(dev))
+    _native.check(st, "awq_serve_page_release")
+    tables.state = state
