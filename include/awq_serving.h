@@ -71,8 +71,8 @@ extern "C" {
 /* A step's new tokens: request b holds state[b] tokens and adds new_tokens[b],
  * its rows following those of request b - 1 in a batch of `total` rows.
  * state int32 [requests + 1]: the lengths, then the number of free pages; a
- * free page is taken from the end of free_pages (int32 [num_pages], the first
- * state[requests] of them free).  block_tables int32 [requests, table_width]:
+ * free page is taken from the end of free_pages (int32 [capacity], as many as can be
+ * free at once, the first state[requests] of them free).  block_tables int32 [requests, table_width]:
  * entries of pages that the step takes are written.
  *
  * A request is refused if new_tokens < 0 or length < 0, its rows pass `total`,
@@ -90,14 +90,14 @@ extern "C" {
 int awq_serve_page_step(const int32_t* state, const int32_t* new_tokens, int32_t* block_tables,
                         const int32_t* free_pages, int32_t* new_state, int32_t* query_start, int32_t* slots,
                         int32_t* positions, int32_t* failed, int64_t requests, int64_t total, int64_t table_width,
-                        int64_t num_pages, int64_t page_size, void* stream);
+                        int64_t capacity, int64_t page_size, void* stream);
 
 /* Request b keeps its first min(max(keep[b], 0), length) tokens; the pages past them
  * go onto the end of free_pages in request and page order.  new_state as above.
  * The table's entries stay as they are (those past a length mean nothing). */
 int awq_serve_page_release(const int32_t* state, const int32_t* keep, const int32_t* block_tables,
                            int32_t* free_pages, int32_t* new_state, int64_t requests, int64_t table_width,
-                           int64_t num_pages, int64_t page_size, void* stream);
+                           int64_t capacity, int64_t page_size, void* stream);
 
 /* q, k and v of `tokens` rows of a fused projection, qkv [tokens, (num_heads + 2
  * num_kv_heads) * head_dim] with qkv_stride elements from row to row: rotate-half

@@ -21,11 +21,12 @@ int log2_page(int64_t page_size) {
 
 int done(hipError_t e) { return e == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH; }
 
-// Tables of `requests` rows: slots and lengths stay 32-bit integers.
+// Tables of `requests` rows: slots stay 32-bit integers, lengths below 2^30 (sums of
+// a length and a stretch of tokens do not overflow).
 int check_pages(int64_t requests, int64_t width, int64_t num_pages, int64_t page_size) {
     if (requests <= 0 || width <= 0 || num_pages <= 0) return AWQ_ERR_BAD_DIMS;
     if (log2_page(page_size) < 0) return AWQ_ERR_PATH;
-    if (requests > AWQ_SERVE_MAX_REQUESTS || width > kIndexLimit / page_size - 1 || num_pages > kIndexLimit / page_size)
+    if (requests > AWQ_SERVE_MAX_REQUESTS || width > (1 << 30) / page_size || num_pages > kIndexLimit / page_size)
         return AWQ_ERR_TOO_LARGE;
     return AWQ_OK;
 }
@@ -41,8 +42,8 @@ int check_cache(int64_t kvh, int64_t hd, int64_t num_pages, int64_t page_size, i
     return AWQ_OK;
 }
 
-int check_step(const PageStepArgs& a, int64_t requests, int64_t width, int64_t num_pages, int64_t page_size) {
-    const int st = check_pages(requests, width, num_pages, page_size);
+int check_step(const PageStepArgs& a, int64_t requests, int64_t width, int64_t capacity, int64_t page_size) {
+    const int st = check_pages(requests, width, capacity, page_size);
     if (st != AWQ_OK) return st;
     if (!a.state || !a.tokens || !a.tables || !a.free_pages || !a.new_state) return AWQ_ERR_NULL_POINTER;
     if (!aligned(a.state, 4) || !aligned(a.tokens, 4) || !aligned(a.tables, 4) || !aligned(a.free_pages, 4) ||
@@ -58,7 +59,7 @@ extern "C" {
 int awq_serve_page_step(const int32_t* state, const int32_t* new_tokens, int32_t* block_tables,
                         const int32_t* free_pages, int32_t* new_state, int32_t* query_start, int32_t* slots,
                         int32_t* positions, int32_t* failed, int64_t requests, int64_t total, int64_t table_width,
-                        int64_t num_pages, int64_t page_size, void* stream) {
+                        int64_t capacity, int64_t page_size, void* stream) {
     PageStepArgs a = {};
     a.state = state;
     a.tokens = new_tokens;
@@ -69,7 +70,7 @@ int awq_serve_page_step(const int32_t* state, const int32_t* new_tokens, int32_t
     a.slots = slots;
     a.positions = positions;
     a.failed = failed;
-    const int st = check_step(a, requests, table_width, num_pages, page_size);
+    const int st = check_step(a, requests, table_width, capacity, page_size);
     if (st != AWQ_OK) return st;
     if (total < 0) return AWQ_ERR_BAD_DIMS;
     if (total > kIndexLimit / 2) return AWQ_ERR_TOO_LARGE;
@@ -79,25 +80,25 @@ int awq_serve_page_step(const int32_t* state, const int32_t* new_tokens, int32_t
     a.requests = (int)requests;
     a.total = (int)total;
     a.width = (int)table_width;
-    a.num_pages = (int)num_pages;
+    a.capacity = (int)capacity;
     a.page_log2 = log2_page(page_size);
     return done(launch_page_step(a, static_cast<hipStream_t>(stream)));
 }
 
 int awq_serve_page_release(const int32_t* state, const int32_t* keep, const int32_t* block_tables,
                            int32_t* free_pages, int32_t* new_state, int64_t requests, int64_t table_width,
-                           int64_t num_pages, int64_t page_size, void* stream) {
+                           int64_t capacity, int64_t page_size, void* stream) {
     PageStepArgs a = {};
     a.state = state;
     a.tokens = keep;
     a.tables = const_cast<int32_t*>(block_tables);
     a.free_pages = free_pages;
     a.new_state = new_state;
-    const int st = check_step(a, requests, table_width, num_pages, page_size);
+    const int st = check_step(a, requests, table_width, capacity, page_size);
     if (st != AWQ_OK) return st;
     a.requests = (int)requests;
     a.width = (int)table_width;
-    a.num_pages = (int)num_pages;
+    a.capacity = (int)capacity;
     a.page_log2 = log2_page(page_size);
     return done(launch_page_release(a, static_cast<hipStream_t>(stream)));
 }

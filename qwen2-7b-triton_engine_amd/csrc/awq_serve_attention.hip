@@ -19,29 +19,29 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kCols = 16;              // (row, query head) pairs of one workgroup: the columns of an MFMA
-constexpr int kWaveKeys = 32;          // tokens of one inner pass of a wave
+constexpr int kCols = 16;              // (row, query head) pairs of a decode workgroup: the columns of an MFMA
+constexpr int kWaveKeys = 32;          // tokens of one inner pass of a decode wave
 constexpr int kKeys = kWaveKeys * kWaves;
+constexpr int kTileKeys = 64;          // tokens of a tile kernel's step
 constexpr int kPExp = 14;              // the probabilities' scale before they are split: 2^14
 constexpr int kQExp = 8;               // q's largest value lies in 2^7 .. 2^8: a group's sum stays below 2^15
 
-// What a workgroup works on.
-struct Item {
-    int b, row0, rows, len, base;      // request, its first row, rows, tokens; its first item
-    int chunk, splits, blocks, rel;    // tokens an item, items along them, blocks of columns; this item's number
-};
+// ---- which item a workgroup has --------------------------------------------------
 
+// Requests of few columns (rows times the heads that share a kv head) go to the
+// decode kernel in blocks of 16 columns, the others to the tile kernel in
+// blocks of 64 or 128.  An item is a block and a stretch of tokens.
 struct Request {
-    int row0, rows, len;
+    int row0, rows, len;               // first row, rows, tokens
 };
 __device__ __forceinline__ Request request(const Kv4AttnArgs& a, int b) {
     Request r = {0, 0, 0};
     if (b < a.requests) {
-        const int lo = a.query_start[b], hi = a.query_start[b + 1];
+        const int lo = a.query_start[b], hi = a.query_start[b + 1], len = a.seq_lens[b];
         r.row0 = lo < 0 ? 0 : lo < a.total ? lo : a.total;
         const int end = hi < r.row0 ? r.row0 : hi < a.total ? hi : a.total;
         r.rows = end - r.row0;
-        r.len = a.seq_lens[b] < 0 ? 0 : a.seq_lens[b];
+        r.len = len < 0 ? 0 : len;
     }
     return r;
 }
@@ -51,122 +51,224 @@ __device__ __forceinline__ int walked(const Kv4AttnArgs& a, int len) {
     const int64_t room = (int64_t)a.width << a.s.page_log2;
     return len <= room ? len : (int)room + 1;
 }
-__device__ __forceinline__ int column_blocks(const Kv4AttnArgs& a, int rows) {
-    const int most = rows < a.max_query ? rows : a.max_query;
-    return (int)(((int64_t)most * (a.nh / a.s.kvh) + kCols - 1) / kCols);
+__device__ __forceinline__ int columns(const Kv4AttnArgs& a, int rows) {
+    return (rows < a.max_query ? rows : a.max_query) * (a.nh / a.s.kvh);
+}
+// Blocks of COLS columns that a request has in this kernel, and its tokens in steps of KEYS.
+template <int COLS, int KEYS>
+__device__ __forceinline__ void sizes(const Kv4AttnArgs& a, const Request& r, int& blocks, int& steps) {
+    const int c = columns(a, r.rows);
+    const bool mine = (c <= a.limit) == (COLS == kCols);
+    blocks = mine ? (c + COLS - 1) / COLS : 0;
+    steps = (int)(((int64_t)walked(a, r.len) + KEYS - 1) / KEYS);
 }
 
-constexpr int kTarget = 1024;          // items that a launch aims at, all kv heads together
-__host__ __device__ inline int items_per_head(int kvh) { return kvh < kTarget ? kTarget / kvh : 1; }
+struct Item {
+    Request r;
+    int b;                             // the request's number
+    int chunk, splits, blocks;         // tokens of an item, items along the tokens, blocks of columns
+    int base, rel;                     // number of the request's first item; this item's after it
+};
 
-// Finds an item (by number) or a row's items (by row): every workgroup walks over
-// the requests' lengths by itself, so that no launch has to prepare a list.
-// The tokens of an item are a multiple of kKeys, as few as the target allows.
-template <bool BY_ROW>
-__device__ bool find_item(const Kv4AttnArgs& a, int want, Item* found, int64_t* sums) {
-    const int tid = threadIdx.x;
-    if (tid == 0) found->b = -1;
-    int64_t work = 0;
-    for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
-        const Request r = request(a, b0 + tid);
+// Sums over the lanes up to this one.
+__device__ __forceinline__ int wave_scan32(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);    // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
+// Finds an item by its number.  Every wave walks over the requests' lengths by
+// itself, 64 at a time and without a barrier: no launch has to prepare a list,
+// and the host need not know the lengths.  The tokens of an item are a multiple of
+// KEYS, as few as `target` items in all allow (at most target + the blocks of all
+// requests come out); without a target an item has all of its request's.
+template <int COLS, int KEYS>
+__device__ __forceinline__ bool find_item(const Kv4AttnArgs& a, int want, int target, Item& it) {
+    constexpr int kMost = (1 << 29) / KEYS;
+    const int lane = threadIdx.x & 63;
+    Request r = request(a, lane);
+    int blocks, steps, m = kMost;
+    sizes<COLS, KEYS>(a, r, blocks, steps);
+    if (target) {
+        int64_t work = (int64_t)blocks * steps;
+        for (int b0 = 64; b0 < a.requests; b0 += 64) {
+            sizes<COLS, KEYS>(a, request(a, b0 + lane), blocks, steps);
+            work += (int64_t)blocks * steps;
+        }
+        // Sums below 2^24 a lane, as good as always, are added in 32 bits.
         int64_t all;
-        block_scan<kWaves>((int64_t)walked(a, r.len) * column_blocks(a, r.rows), sums, all);
-        work += all;
+        if (a.requests == 1) {
+            all = (int64_t)__builtin_amdgcn_readfirstlane((int)(work >> 32)) << 32 |
+                  (uint32_t)__builtin_amdgcn_readfirstlane((int)work);
+        } else if (__all(work < (1 << 24))) {
+            all = __builtin_amdgcn_readlane(wave_scan32((int)work), 63);
+        } else {
+            all = __shfl(wave_scan(work), 63);
+        }
+        const int64_t most = (int64_t)target * kMost;
+        const uint32_t few = all < 0x7FFFFFFF - target ? (uint32_t)(all + target - 1) / (uint32_t)target : 0;
+        m = few ? (few < (uint32_t)kMost ? (int)few : kMost)
+                : all == 0 ? 1 : all < most ? (int)((all + target - 1) / target) : kMost;
+        m = __builtin_amdgcn_readfirstlane(m);
     }
-    const int64_t per = (int64_t)kKeys * items_per_head(a.s.kvh);
-    const int64_t chunk64 = kKeys * ((work + per - 1) / per);
-    const int chunk = (int)(chunk64 < kKeys ? kKeys : chunk64 < (1 << 30) ? chunk64 : (1 << 30));
-    int64_t before = 0;
-    for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
-        const Request r = request(a, b0 + tid);
-        const int n = walked(a, r.len), blocks = column_blocks(a, r.rows), splits = (int)(((int64_t)n + chunk - 1) / chunk);
-        int64_t all;
-        const int64_t mine = (int64_t)blocks * splits, upto = before + block_scan<kWaves>(mine, sums, all);
-        before += all;
-        const bool hit = BY_ROW ? want >= r.row0 && want < r.row0 + r.rows : want >= upto - mine && want < upto;
-        if (hit) *found = Item{b0 + tid, r.row0, r.rows, r.len, (int)(upto - mine), chunk, splits, blocks,
-                               (int)(want - (upto - mine))};
+    int before = 0;
+    for (int b0 = 0; b0 < a.requests; b0 += 64) {
+        if (a.requests > 64) r = request(a, b0 + lane);
+        sizes<COLS, KEYS>(a, r, blocks, steps);
+        const int splits = (int)((uint32_t)(steps + m - 1) / (uint32_t)m), mine = blocks * splits;
+        const int upto = before + wave_scan32(mine);
+        const uint64_t hit = __ballot(want >= upto - mine && want < upto);
+        if (hit) {
+            const int at = __builtin_ctzll(hit);
+            auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+            it.b = b0 + at;
+            it.r = Request{pick(r.row0), pick(r.rows), pick(r.len)};
+            it.b = b0 + at;
+            it.chunk = m * KEYS;
+            it.splits = pick(splits);
+            it.blocks = pick(blocks);
+            it.base = pick(upto - mine);
+            it.rel = want - it.base;
+            return true;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
     }
-    __syncthreads();
-    return found->b >= 0;
-}
-// The item in scalar registers: the same for every lane.
-__device__ __forceinline__ Item uniform(const Item* lds) {
-    Item it;
-    const int* from = reinterpret_cast<const int*>(lds);
-    int* to = reinterpret_cast<int*>(&it);
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(Item) / sizeof(int)); ++i) to[i] = __builtin_amdgcn_readfirstlane(from[i]);
-    return it;
+    return false;
 }
 
+// What the combining launch has to know of a row.
+struct RowRecord {
+    int row, base;                     // the row's place in its request; its first item, ~ of it for the tile kernel's
+    int blocks, splits;                // 0 items: zeros are to be written; 1: the row is done
+};
+// Written by the first item of a request.
+__device__ __forceinline__ void write_records(const Kv4AttnArgs& a, const Item& it, bool tile) {
+    if (it.rel != 0 || blockIdx.y != 0) return;
+    for (int i = threadIdx.x; i < it.r.rows; i += kThreads) {
+        const bool blind = (int64_t)it.r.len - it.r.rows + i < 0;
+        a.records[it.r.row0 + i] = i32x4{i, tile ? ~it.base : it.base, it.blocks,
+                                         i >= a.max_query || it.splits == 1 ? 1 : blind ? 0 : it.splits};
+    }
+}
+// Rows that no item has -- of no request, or of one without tokens -- are zeros.
+// Done by the first workgroup past the items; a grid has at least one.
+__device__ __forceinline__ void zero_rows(const Kv4AttnArgs& a) {
+    const int pieces = a.nh * a.s.hd / 8;                // of 16 bytes
+    auto clear = [&](int lo, int hi) {
+        u32x4* out = reinterpret_cast<u32x4*>(a.out);
+        for (int64_t i = (int64_t)lo * pieces + threadIdx.x; i < (int64_t)hi * pieces; i += kThreads) out[i] = u32x4{0, 0, 0, 0};
+        for (int i = lo + (int)threadIdx.x; i < hi; i += kThreads) a.records[i] = i32x4{0, 0, 0, 1};
+    };
+    const int lane = threadIdx.x & 63;
+    for (int b0 = 0; b0 < a.requests; b0 += 64) {
+        const Request r = request(a, b0 + lane);
+        uint64_t none = __ballot(r.len == 0 && r.rows > 0);
+        for (; none; none &= none - 1) {
+            const int at = __builtin_ctzll(none), row0 = __builtin_amdgcn_readlane(r.row0, at);
+            clear(row0, row0 + __builtin_amdgcn_readlane(r.rows, at));
+        }
+    }
+    const Request first = request(a, 0), last = request(a, a.requests - 1);
+    clear(0, first.row0);
+    clear(last.row0 + last.rows, a.total);
+}
+
+// ---- pieces of both kernels ---------------------------------------------------------
+
+// Maximum over the four lanes that share a column (lane, lane + 16, + 32, + 48).
+__device__ __forceinline__ float column_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+// The running maximum is raised only where a score passes it by more than this
+// (in powers of two): probabilities of up to 2^1.5, scaled by 2^14, still fit fp16,
+// and most passes do without the cross-lane maximum and the rescaling.
+constexpr float kSlack = 1.5f;
+
+// 0x4C004C00 in a VGPR, opaque to the optimiser (awq_device.h magic_vgpr): the
+// and-or below stays one instruction.
+constexpr uint32_t kBase16 = 0x4C004C00u;
+__device__ __forceinline__ uint32_t base16_vgpr() {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)kBase16, (int)kBase16, 0x111, 0xF, 0xF, false);
+}
 // Eight codes of a word times a scale, exact: nibble u and nibble u + 4 make
 // pair u.  A nibble in bits 6 .. 9 of 0x4C00 is fp16 16 + code; (16 + code) s - 16 s
 // is rounded once, to a value that needs no rounding.
-__device__ __forceinline__ void scaled_codes(uint32_t w, half2_t s, half2_t minus16s, half2_t (&o)[4]) {
-    constexpr uint32_t kMask = 0x03C003C0u, kBase = 0x4C004C00u;
-    o[0] = __builtin_elementwise_fma(as_h2(and_or(w << 6, kMask, kBase)), s, minus16s);
-    o[1] = __builtin_elementwise_fma(as_h2(and_or(w << 2, kMask, kBase)), s, minus16s);
-    o[2] = __builtin_elementwise_fma(as_h2(and_or(w >> 2, kMask, kBase)), s, minus16s);
-    o[3] = __builtin_elementwise_fma(as_h2(and_or(w >> 6, kMask, kBase)), s, minus16s);
+__device__ __forceinline__ void scaled_codes(uint32_t w, uint32_t base, half2_t s, half2_t minus16s, half2_t (&o)[4]) {
+    constexpr uint32_t kMask = 0x03C003C0u;
+    o[0] = __builtin_elementwise_fma(as_h2(and_or(w << 6, kMask, base)), s, minus16s);
+    o[1] = __builtin_elementwise_fma(as_h2(and_or(w << 2, kMask, base)), s, minus16s);
+    o[2] = __builtin_elementwise_fma(as_h2(and_or(w >> 2, kMask, base)), s, minus16s);
+    o[3] = __builtin_elementwise_fma(as_h2(and_or(w >> 6, kMask, base)), s, minus16s);
 }
 __device__ __forceinline__ half2_t times_minus16(half2_t s) { return s * half2_t{(half_t)-16.0f, (half_t)-16.0f}; }
 
-// What one lane holds of 16 tokens: lane (i, t) = (lane & 15, lane >> 4).
-template <int HD, int GN>
-struct Tile {
-    uint32_t kw[HD / 32];              // token i, columns 32 s + 8 t .. of K
-    half2_t ks[GN];                    // its (scale, zero)
-    u32x4 vw;                          // tokens 4 t .. 4 t + 3, eight columns of V around HD / 16 * i
-    half4_t vs, vz;                    // their scales in these columns' group; zeros of group min(i, GN - 1)
+// A barrier for LDS alone: loads from memory stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <int GN>
+struct PairsOf {
+    typedef half_t type __attribute__((ext_vector_type(2 * GN)));
 };
 
-template <int HD, int GN>
-__device__ __forceinline__ void load_tile(Tile<HD, GN>& x, const Kv4AttnArgs& a, const int32_t* table, int g, int key0,
-                                          int n, int i, int t) {
-    constexpr int kSteps = HD / 32;
-    const int index = key0 >> a.s.page_log2;
-    const bool inside = key0 < n;
-    int page = inside && index < a.width ? table[index] : -1;
-    const bool there = page >= 0 && page < a.s.num_pages;
-    page = there ? page : 0;
-    const int tok = key0 & (a.s.page() - 1);
-    const uint8_t* block = a.cache + ((int64_t)page * a.s.kvh + g) * a.s.block();
-    const uint8_t* kc = block + (tok + i) * (HD / 2) + t * (HD / 8);
-    if constexpr (kSteps == 4) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(kc);
+// A column's query as the B operand of the k-steps: lane (column, t) holds
+// columns 32 s + 8 t + e of the head; the sums of the groups in three parts, lane
+// t those of group t.  Returns the exponent of the row's power of two.
+template <int HD, int GN, bool BF16>
+__device__ __forceinline__ int load_query(const uint16_t* src, int t, half8_t (&q)[HD / 32], half8_t& qz) {
+    constexpr int kSteps = HD / 32, G = HD / GN;
+    float x[kSteps][8], mx = 0.0f;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) x.kw[s] = w[s];
-    } else {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(kc);
-        x.kw[0] = w.x;
-        x.kw[1] = w.y;
+    for (int s = 0; s < kSteps; ++s) {
+        load8<BF16>(src + 32 * s + 8 * t, x[s]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[s][e]));
     }
-    const uint8_t* ks = block + 2 * a.s.k_bytes() + (tok + i) * (4 * GN);
-    typedef half_t pairs_t __attribute__((ext_vector_type(2 * GN)));
-    const pairs_t kz = *reinterpret_cast<const pairs_t*>(ks);
+    mx = column_max(mx);
+    int exp = kQExp - __builtin_amdgcn_frexp_expf(mx);
+    exp = exp < 100 ? exp : 100;
+    const float up = __builtin_ldexpf(1.0f, exp);
+    float sum[GN];
 #pragma unroll
-    for (int q = 0; q < GN; ++q) x.ks[q] = half2_t{kz[2 * q], kz[2 * q + 1]};
-    const int tb = (tok >> 2) + t;
-    const int j8 = HD == 128 ? i : i >> 1;
-    x.vw = *reinterpret_cast<const u32x4*>(block + a.s.k_bytes() + (tb * (HD / 8) + j8) * 16);
-    const uint8_t* vs = block + 2 * a.s.k_bytes() + a.s.scale_bytes() + tb * (16 * GN);
-    x.vs = *reinterpret_cast<const half4_t*>(vs + 16 * (8 * j8 / (HD / GN)));
-    x.vz = *reinterpret_cast<const half4_t*>(vs + 16 * (i < GN ? i : GN - 1) + 8);
-    if (inside && !there) {            // a page outside the cache: NaN for the queries that see it
+    for (int i = 0; i < GN; ++i) sum[i] = 0.0f;
 #pragma unroll
-        for (int q = 0; q < GN; ++q) x.ks[q] = half2_t{(half_t)NAN, (half_t)NAN};
-    }
-    if (!there || key0 + 16 > n) {     // tokens past the length may hold anything
+    for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (!there || key0 + 4 * t + r >= n) {
-                x.vs[r] = (half_t)0.0f;
-                x.vz[r] = (half_t)0.0f;
-            }
+        for (int e = 0; e < 8; ++e) {
+            q[s][e] = (half_t)(x[s][e] * up);
+            sum[32 * s / G] += (float)q[s][e];
         }
+    float mine = 0.0f;
+#pragma unroll
+    for (int i = 0; i < GN; ++i) {
+        sum[i] += __shfl_xor(sum[i], 16);
+        sum[i] += __shfl_xor(sum[i], 32);
+        if (t == i) mine = sum[i];
     }
+    qz = half8_t{};
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {          // 33 bits
+        qz[e] = (half_t)mine;
+        mine -= (float)qz[e];
+    }
+    return exp;
 }
+
+// A page's number in a request's table: -1 past the length or the table.
+__device__ __forceinline__ int page_at(const Kv4AttnArgs& a, const int32_t* table, int key, int n) {
+    const int index = key >> a.s.page_log2;
+    return key < n && index < a.width ? table[index] : -1;
+}
+
+// ---- few columns: decode ---------------------------------------------------------------
 
 // One workgroup: an item's tokens of one kv head for up to 16 columns, 32
 // tokens per wave and pass.  S^T = K Q^T puts a column in each MFMA column, so one
@@ -174,101 +276,133 @@ __device__ __forceinline__ void load_tile(Tile<HD, GN>& x, const Kv4AttnArgs& a,
 // the B operand of O^T = V^T P^T (its k order, tokens 4 t + r of two tiles, is V's
 // as loaded).  V's row order in that product is free: lane i takes the columns
 // i VC .. i VC + VC - 1 of its tokens and supplies one of them to each of VC
-// products.  The waves' results meet once, at the end.
+// products.  K's registers are loaded again as soon as its product is made, V's
+// likewise: each is in flight under the other half of the pass, without a second
+// set of registers.  The waves' results meet once, at the end.
 template <int HD, int GN, bool BF16>
-__global__ __launch_bounds__(kThreads) void awq_kv4_decode_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs a) {
     constexpr int kSteps = HD / 32;
     constexpr int VC = HD / 16;            // V columns per lane
     constexpr int G = HD / GN;
     constexpr int kStride = HD + 4;        // floats per column of the reduction buffer
-    __shared__ int64_t sums[kWaves];
-    __shared__ Item item_lds;
     __shared__ float m_lds[kWaves][kCols], l_lds[kWaves][kCols];
     __shared__ int lim_lds[kCols];
     __shared__ __align__(16) float o_lds[kWaves][kCols][kStride];
 
-    if (!find_item<false>(a, blockIdx.x, &item_lds, sums)) return;
-    const Item it = uniform(&item_lds);
+    Item it;
+    if (!find_item<kCols, kKeys>(a, blockIdx.x, a.decode_target, it)) {
+        if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) zero_rows(a);   // the grid's last column has no item
+        return;
+    }
+    write_records(a, it, false);
     const int g = blockIdx.y, group = a.nh / a.s.kvh;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, t = lane >> 4;
     const int block = it.rel % it.blocks, split = it.rel / it.blocks;
-    const int live_rows = it.rows < a.max_query ? it.rows : a.max_query;
-    const int c0 = block * kCols, cols = live_rows * group - c0 < kCols ? live_rows * group - c0 : kCols;
-    const int n = walked(a, it.len);
+    const int all_cols = columns(a, it.r.rows), c0 = block * kCols;
+    const int cols = all_cols - c0 < kCols ? all_cols - c0 : kCols;
+    const int n = walked(a, it.r.len);
+    // The block's last column sees the most tokens.
+    const int64_t last_pos = (int64_t)it.r.len - it.r.rows + (c0 + cols - 1) / group;
+    const int lim_max = last_pos < 0 ? 0 : last_pos + 1 < n ? (int)(last_pos + 1) : n;
+    const int start = split * it.chunk;
+    const int end = lim_max < start + it.chunk ? lim_max : start + it.chunk;
+
+    // What this lane reads of 16 tokens, from where they begin in the codes and in the scales.
+    const int j8 = HD == 128 ? col : col >> 1;
+    const uint32_t k_ofs = col * (HD / 2) + t * (HD / 8), v_ofs = a.s.k_bytes() + (t * (HD / 8) + j8) * 16;
+    const uint32_t ks_ofs = col * (4 * GN), vs_ofs = a.s.scale_bytes() + t * (16 * GN) + 16 * (8 * j8 / G);
+    const uint32_t vz_ofs = a.s.scale_bytes() + t * (16 * GN) + 16 * (col < GN ? col : GN - 1) + 8;
+    struct Place {                         // of 16 tokens
+        const uint8_t *codes, *scales;
+        bool there;
+    };
+    auto place = [&](int page, int key) {
+        Place p;
+        p.there = page >= 0 && page < a.s.num_pages;
+        const int tok = key & (a.s.page() - 1);
+        const uint8_t* block_at = a.cache + ((int64_t)(p.there ? page : 0) * a.s.kvh + g) * a.s.block();
+        p.codes = block_at + tok * (HD / 2);
+        p.scales = block_at + 2 * a.s.k_bytes() + tok * (4 * GN);
+        return p;
+    };
+    uint32_t kw[2][kSteps];                // token col, columns 32 s + 8 t .. of K
+    half2_t ks[2][GN];                     // its (scale, zero)
+    u32x4 vw[2];                           // tokens 4 t .. 4 t + 3, eight columns of V around VC col
+    half4_t vs[2], vz[2];                  // their scales in these columns' group; the zeros of group min(col, GN - 1)
+    auto load_k = [&](const Place (&p)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (kSteps == 4) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(p[h].codes + k_ofs);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) kw[h][s] = w[s];
+            } else {
+                const u32x2 w = *reinterpret_cast<const u32x2*>(p[h].codes + k_ofs);
+                kw[h][0] = w.x;
+                kw[h][1] = w.y;
+            }
+            const auto kz = *reinterpret_cast<const typename PairsOf<GN>::type*>(p[h].scales + ks_ofs);
+#pragma unroll
+            for (int i = 0; i < GN; ++i) ks[h][i] = half2_t{kz[2 * i], kz[2 * i + 1]};
+        }
+    };
+    auto load_v = [&](const Place (&p)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            vw[h] = *reinterpret_cast<const u32x4*>(p[h].codes + v_ofs);
+            vs[h] = *reinterpret_cast<const half4_t*>(p[h].scales + vs_ofs);
+            vz[h] = *reinterpret_cast<const half4_t*>(p[h].scales + vz_ofs);
+        }
+    };
+
+    const int32_t* table = a.tables + (int64_t)it.b * a.width;
+    int key0 = start + kWaveKeys * wave;
+    Place now[2];
+    now[0] = place(page_at(a, table, key0, n), key0);
+    now[1] = place(page_at(a, table, key0 + 16, n), key0 + 16);
+    if (key0 < end) {
+        load_k(now);
+        load_v(now);
+    }
+    int page0 = page_at(a, table, key0 + kKeys, n), page1 = page_at(a, table, key0 + kKeys + 16, n);
 
     // This lane's column: row c / group of the request, head c % group.
     const int c = c0 + (col < cols ? col : 0);
     const int row = c / group, head = g * group + c % group;
-    const int64_t pos = (int64_t)it.len - it.rows + row;
+    const int64_t pos = (int64_t)it.r.len - it.r.rows + row;
     const int lim = pos < 0 ? 0 : pos + 1 < n ? (int)(pos + 1) : n;   // tokens it sees
-    // Rows grow along the columns: the block's first sees the fewest tokens, its last the most.
-    const int lim_min = __builtin_amdgcn_readlane(lim, 0);
-    const int lim_max = __builtin_amdgcn_readlane(lim, cols - 1);
-    const int start = split * it.chunk;
-    const int end = lim_max < start + it.chunk ? lim_max : start + it.chunk;
-
-    half8_t q[kSteps], qz = {};
-    int exp;                               // of the row's power of two
-    {
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.row0 + row) * a.ld + (int64_t)head * HD;
-        float x[kSteps][8], mx = 0.0f;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            load8<BF16>(src + 32 * s + 8 * t, x[s]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[s][e]));
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        exp = kQExp - __builtin_amdgcn_frexp_expf(mx);
-        exp = exp < 100 ? exp : 100;
-        const float up = __builtin_ldexpf(1.0f, exp);
-        float sum[GN];
-#pragma unroll
-        for (int i = 0; i < GN; ++i) sum[i] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                q[s][e] = (half_t)(x[s][e] * up);
-                sum[32 * s / G] += (float)q[s][e];
-            }
-        float mine = 0.0f;
-#pragma unroll
-        for (int i = 0; i < GN; ++i) {
-            sum[i] += __shfl_xor(sum[i], 16);
-            sum[i] += __shfl_xor(sum[i], 32);
-            if (t == i) mine = sum[i];
-        }
-#pragma unroll
-        for (int e = 0; e < 3; ++e) {      // 33 bits
-            qz[e] = (half_t)mine;
-            mine -= (float)qz[e];
-        }
-    }
-
+    const int lim_min = __builtin_amdgcn_readlane(lim, 0);            // rows grow along the columns
+    half8_t q[kSteps], qz;
+    const int exp = load_query<HD, GN, BF16>(
+        reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + row) * a.ld + (int64_t)head * HD, t, q, qz);
     // exp(scale x) = exp2(x factor); the scores here are 2^exp times as large.
     // Every exponent is a difference of scores first: what they were rounded to
     // on the way must be the same wherever two meet.
     const float factor = a.scale * 1.4426950408889634f, unit = __builtin_ldexpf(factor, -exp);
+    const uint32_t base = base16_vgpr();
+    // Rows GN .. 15 of the zeros' block: a row of ones at 4, the rest zero.
+    const uint32_t z_mask = col < GN ? 0xFFFFFFFFu : 0u, z_fill = col == 4 ? 0x3C003C00u : 0u;
+
     float m = -INFINITY;                   // of column `col`
     floatx4 acc[VC], acc_z = {0.f, 0.f, 0.f, 0.f};   // acc_z: rows 0 .. GN - 1 the groups' zeros, row 4 the sum
 #pragma unroll
     for (int v = 0; v < VC; ++v) acc[v] = floatx4{0.f, 0.f, 0.f, 0.f};
-    const int32_t* table = a.tables + (int64_t)it.b * a.width;
-    Tile<HD, GN> x[2];
-    int key0 = start + kWaveKeys * wave;
-    if (key0 < end) {
-        load_tile(x[0], a, table, g, key0, n, col, t);
-        load_tile(x[1], a, table, g, key0 + 16, n, col, t);
-    }
-    for (; key0 < end; key0 += kKeys) {
-        Tile<HD, GN> y[2];
-        if (key0 + kKeys < end) {          // the next pass's, in flight under this one
-            load_tile(y[0], a, table, g, key0 + kKeys, n, col, t);
-            load_tile(y[1], a, table, g, key0 + kKeys + 16, n, col, t);
+    while (key0 < end) {
+        const bool more = key0 + kKeys < end;
+        Place next[2];
+        next[0] = place(page0, key0 + kKeys);
+        next[1] = place(page1, key0 + kKeys + 16);
+        page0 = page_at(a, table, key0 + 2 * kKeys, n);
+        page1 = page_at(a, table, key0 + 2 * kKeys + 16, n);
+
+        if (!now[0].there || !now[1].there) {   // a page outside the cache: NaN for the queries that see it
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (!now[h].there)
+#pragma unroll
+                    for (int i = 0; i < GN; ++i) ks[h][i] = half2_t{(half_t)NAN, (half_t)NAN};
         }
         floatx4 s[2];
 #pragma unroll
@@ -276,18 +410,19 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_decode_kernel(Kv4AttnArgs a)
             half8_t z = {};
 #pragma unroll
             for (int i = 0; i < GN; ++i)
-                if (t == i) z[0] = z[1] = z[2] = x[h].ks[i].y;
+                if (t == i) z[0] = z[1] = z[2] = ks[h][i].y;
             s[h] = mfma16x16x32(z, qz, floatx4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
             for (int st = 0; st < kSteps; ++st) {
-                const half_t sc = x[h].ks[32 * st / G].x;
+                const half_t sc = ks[h][32 * st / G].x;
                 const half2_t s2 = {sc, sc};
                 half2_t o[4];
-                scaled_codes(x[h].kw[st], s2, times_minus16(s2), o);
+                scaled_codes(kw[h][st], base, s2, times_minus16(s2), o);
                 const half8_t k = {o[0].x, o[0].y, o[1].x, o[1].y, o[2].x, o[2].y, o[3].x, o[3].y};
                 s[h] = mfma16x16x32(k, q[st], s[h]);
             }
         }
+        if (more) load_k(next);
         if (key0 + kWaveKeys > lim_min) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -295,22 +430,18 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_decode_kernel(Kv4AttnArgs a)
                 for (int r = 0; r < 4; ++r)
                     if (key0 + 16 * h + 4 * t + r >= lim) s[h][r] = -INFINITY;
         }
-        float mx = -INFINITY;
+        float mx = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[h][r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m, mx);
-        const float ref = mn == -INFINITY ? 0.0f : mn;   // nothing yet: every exponential is 0
-        if (__any(mn > m)) {
-            const float alpha = __builtin_amdgcn_exp2f((m - ref) * unit);
+        for (int r = 1; r < 4; ++r) mx = fmaxf(mx, fmaxf(s[0][r], s[1][r]));
+        if (__any((mx - m) * unit > kSlack)) {
+            const float mn = fmaxf(m, column_max(mx));
+            const float alpha = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : (m - mn) * unit);
             acc_z *= alpha;
 #pragma unroll
             for (int v = 0; v < VC; ++v) acc[v] *= alpha;
+            m = mn;
         }
-        m = mn;
+        const float ref = m == -INFINITY ? 0.0f : m;     // nothing yet: every exponential is 0
         float p[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -319,43 +450,51 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_decode_kernel(Kv4AttnArgs a)
         half8_t phi, plo;
         split16(p, kPExp, phi, plo);
 
-        // The zeros' rows and the row of ones.
-        half8_t z = {};
+        if (!now[0].there || !now[1].there || key0 + kWaveKeys > n) {   // tokens past the length may hold anything
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const half_t fill = (half_t)(col == 4 ? 1.0f : 0.0f);
-            z[r] = col < GN ? x[0].vz[r] : fill;
-            z[4 + r] = col < GN ? x[1].vz[r] : fill;
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!now[h].there || key0 + 16 * h + 4 * t + r >= n) vs[h][r] = vz[h][r] = (half_t)0.0f;
         }
-        acc_z = mfma16x16x32(z, plo, acc_z);
-        acc_z = mfma16x16x32(z, phi, acc_z);
-        half2_t pairs[4][VC];              // [tokens 2 k, 2 k + 1 of the two tiles][column]
+        union {
+            uint32_t w[4];
+            half8_t h;
+        } z;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const Tile<HD, GN>& y0 = x[k >> 1];
-            const uint32_t w0 = y0.vw[2 * (k & 1)], w1 = y0.vw[2 * (k & 1) + 1];
-            const half2_t s2 = {y0.vs[2 * (k & 1)], y0.vs[2 * (k & 1) + 1]}, m16 = times_minus16(s2);
-            if constexpr (VC == 8) {
-                half2_t o[4];
-                scaled_codes(__builtin_amdgcn_perm(w1, w0, 0x05040100u), s2, m16, o);   // columns 0 .. 3
+        for (int h = 0; h < 2; ++h) {
+            const u32x2 w = __builtin_bit_cast(u32x2, vz[h]);
+            z.w[2 * h] = (w.x & z_mask) | z_fill;
+            z.w[2 * h + 1] = (w.y & z_mask) | z_fill;
+        }
+        acc_z = mfma16x16x32(z.h, plo, acc_z);
+        acc_z = mfma16x16x32(z.h, phi, acc_z);
+        // Four columns at a time: the words' lower halves, then their upper ones
+        // (heads of 64: a lane has four columns, one half or the other).
 #pragma unroll
-                for (int u = 0; u < 4; ++u) pairs[k][u] = o[u];
-                scaled_codes(__builtin_amdgcn_perm(w1, w0, 0x07060302u), s2, m16, o);   // columns 4 .. 7
+        for (int part = 0; part < VC / 4; ++part) {
+            const uint32_t half = VC == 8 ? (part ? 0x07060302u : 0x05040100u) : (col & 1 ? 0x07060302u : 0x05040100u);
+            half2_t pairs[4][4];           // [tokens 2 k, 2 k + 1 of the two tiles][column]
 #pragma unroll
-                for (int u = 0; u < 4; ++u) pairs[k][4 + u] = o[u];
-            } else {                       // 4 columns a lane: the word's lower half or its upper one
-                scaled_codes(__builtin_amdgcn_perm(w1, w0, col & 1 ? 0x07060302u : 0x05040100u), s2, m16, pairs[k]);
+            for (int k = 0; k < 4; ++k) {
+                const half4_t sv = vs[k >> 1];
+                const half2_t s2 = {sv[2 * (k & 1)], sv[2 * (k & 1) + 1]};
+                scaled_codes(__builtin_amdgcn_perm(vw[k >> 1][2 * (k & 1) + 1], vw[k >> 1][2 * (k & 1)], half), base, s2,
+                             times_minus16(s2), pairs[k]);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const half8_t w = {pairs[0][u].x, pairs[0][u].y, pairs[1][u].x, pairs[1][u].y,
+                                   pairs[2][u].x, pairs[2][u].y, pairs[3][u].x, pairs[3][u].y};
+                floatx4& d = acc[4 * part + u];
+                d = mfma16x16x32(w, plo, d);
+                d = mfma16x16x32(w, phi, d);
             }
         }
-#pragma unroll
-        for (int v = 0; v < VC; ++v) {
-            const half8_t w = {pairs[0][v].x, pairs[0][v].y, pairs[1][v].x, pairs[1][v].y,
-                               pairs[2][v].x, pairs[2][v].y, pairs[3][v].x, pairs[3][v].y};
-            acc[v] = mfma16x16x32(w, plo, acc[v]);
-            acc[v] = mfma16x16x32(w, phi, acc[v]);
-        }
-        x[0] = y[0];
-        x[1] = y[1];
+        if (more) load_v(next);
+        now[0] = next[0];
+        now[1] = next[1];
+        key0 += kKeys;
     }
 
     // This lane: rows 4 t + r of each product, i.e. columns VC (4 t + r) + v of column `col`.
@@ -397,7 +536,7 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_decode_kernel(Kv4AttnArgs a)
         if (it.splits == 1) {
             const int cc = c0 + k, r = cc / group, h = g * group + cc % group;
             const float y = lim_lds[k] == 0 ? 0.0f : sum / ls;
-            reinterpret_cast<uint16_t*>(a.out)[((int64_t)(it.row0 + r) * a.nh + h) * HD + d] = to16<BF16>(y);
+            reinterpret_cast<uint16_t*>(a.out)[((int64_t)(it.r.row0 + r) * a.nh + h) * HD + d] = to16<BF16>(y);
         } else {
             float* dst = a.part + (((int64_t)blockIdx.x * a.s.kvh + g) * kCols + k) * (HD + 2);
             dst[d] = sum;
@@ -409,67 +548,500 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_decode_kernel(Kv4AttnArgs a)
     }
 }
 
-// out[row, head] = sum of its items' parts, each weighted by exp2(its maximum -
-// the overall maximum).  One workgroup per row and kv head.  Rows that see no
-// token, and rows of no request, are set to zero here.
-template <int HD, bool BF16>
-__global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a) {
-    __shared__ int64_t sums[kWaves];
-    __shared__ Item item_lds;
-    const int row = blockIdx.x, g = blockIdx.y, group = a.nh / a.s.kvh;
-    const bool found = find_item<true>(a, row, &item_lds, sums);
-    const Item it = uniform(&item_lds);
-    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + ((int64_t)row * a.nh + g * group) * HD;
-    if (!found || it.splits == 0) {
-        for (int i = threadIdx.x; i < group * HD; i += kThreads) out[i] = 0;
+// ---- many columns: tiles ---------------------------------------------------------------
+
+// Place of a token within its 64-token tile of the transposed V: the S^T product
+// leaves lane group t with tokens 4 t .. 4 t + 3 of each 16-token block, and the P V
+// product wants 8 consecutive k per lane: 8 consecutive places hold tokens
+// 4 t .. 4 t + 3 of two neighbouring blocks.  Four neighbouring tokens (block of
+// four tb) stay together, at place 32 (tb / 8) + 8 (tb % 4) + 4 (tb / 4 % 2).
+
+// Swizzle of a row's 16-byte chunks in LDS, K: 16 rows' same chunk is what one
+// operand read fetches, and the rows start on the same bank.
+template <int CHUNKS>
+__device__ __forceinline__ int k_chunk(int row, int chunk) {
+    return chunk ^ (row & (CHUNKS < 16 ? CHUNKS - 1 : 15));
+}
+// V: reads as K's; writes go to the same chunk of rows that are 8 apart.
+__device__ __forceinline__ int v_chunk(int row, int chunk) { return chunk ^ ((row ^ (row >> 3)) & 7); }
+
+// One workgroup: 64 NQ columns of one kv head, 16 NQ per wave, over an item's
+// tokens in tiles of 64.  The tile's codes are multiplied out once per workgroup,
+// exactly, into LDS -- K as it is, V transposed, its zeros and a row of ones as
+// rows of their own -- and every wave reads its operands there.  The codes of the
+// next tile are on their way in registers meanwhile (36 bytes a thread), so
+// that two LDS buffers and one barrier a tile suffice.
+template <int HD, int GN, int NQ, bool BF16>
+__global__ __launch_bounds__(kThreads, 2) void awq_kv4_tile_kernel(Kv4AttnArgs a) {
+    constexpr int kSteps = HD / 32, kDb = HD / 16, kChunks = HD / 8, G = HD / GN;
+    constexpr int COLS = 64 * NQ;
+    constexpr int kRows = HD + 16;                       // of the transposed V: columns, zeros, ones
+    constexpr int kK = kTileKeys * HD, kV = kRows * kTileKeys, kZ = kTileKeys * 4;   // halfs
+    __shared__ __align__(16) half_t lds[2][kK + kV + kZ];
+
+    Item it;
+    const int tid = threadIdx.x, lane = tid & 63;
+    if (!find_item<COLS, kTileKeys>(a, blockIdx.x, a.tile_target, it)) {
+        if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && a.limit == 0) zero_rows(a);
         return;
     }
-    const int r = row - it.row0;
-    if (it.splits == 1 || r >= a.max_query) return;
-    const float factor = a.scale * 1.4426950408889634f;
-    const bool blind = (int64_t)it.len - it.rows + r < 0;
-    for (int i = threadIdx.x; i < group * HD; i += kThreads) {
-        const int c = r * group + i / HD, d = i % HD;
-        const int64_t step = (int64_t)it.blocks * a.s.kvh * kCols * (HD + 2);
-        const float* base = a.part + (((int64_t)(it.base + c / kCols) * a.s.kvh + g) * kCols + c % kCols) * (HD + 2);
-        float mx = -INFINITY;
-        for (int s = 0; s < it.splits; ++s) mx = fmaxf(mx, base[s * step + HD]);
-        const float ref = mx == -INFINITY ? 0.0f : mx;
-        float sum = 0.0f, l = 0.0f;
-        for (int s = 0; s < it.splits; ++s) {
-            const float w = __builtin_amdgcn_exp2f((base[s * step + HD] - ref) * factor);
-            sum = fmaf(w, base[s * step + d], sum);
-            l = fmaf(w, base[s * step + HD + 1], l);
+    write_records(a, it, true);
+    const int g = blockIdx.y, group = a.nh / a.s.kvh;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, t = lane >> 4;
+    // The last blocks, which see the most tokens, start first.
+    const int block = it.blocks - 1 - it.rel % it.blocks, split = it.rel / it.blocks;
+    const int all_cols = columns(a, it.r.rows), c0 = block * COLS;
+    const int n = walked(a, it.r.len);
+    auto limit_of = [&](int c) {                         // tokens that a column sees
+        const int64_t pos = (int64_t)it.r.len - it.r.rows + c / group;
+        return pos < 0 ? 0 : pos + 1 < n ? (int)(pos + 1) : n;
+    };
+    const int c_last = c0 + COLS < all_cols ? c0 + COLS - 1 : all_cols - 1;
+    const int start = split * it.chunk, lim_wg = limit_of(c_last);
+    const int end = lim_wg < start + it.chunk ? lim_wg : start + it.chunk;
+    const int tiles = end > start ? (end - start + kTileKeys - 1) / kTileKeys : 0;
+    const int32_t* table = a.tables + (int64_t)it.b * a.width;
+
+    // Rows of the zeros' block that no tile writes: ones at 4, else zero; zeros of no group.
+    for (int i = tid; i < 2 * (16 * kTileKeys + kZ); i += kThreads) {
+        const int b = i / (16 * kTileKeys + kZ), j = i % (16 * kTileKeys + kZ);
+        if (j < 16 * kTileKeys) {
+            const int r = j / kTileKeys;
+            if (r >= GN) lds[b][kK + HD * kTileKeys + j] = (half_t)(r == 4 ? 1.0f : 0.0f);
+        } else if ((j - 16 * kTileKeys) % 4 >= GN) {
+            lds[b][kK + kV + j - 16 * kTileKeys] = (half_t)0.0f;
         }
-        out[i] = to16<BF16>(blind ? 0.0f : sum / l);
+    }
+
+    // What this thread brings of a tile: K, token tid / 4, columns 32 s + 8 (tid % 4) ..; V, four
+    // tokens, eight columns (heads of 64: half of the threads).
+    const int k_tok = tid >> 2, k_t = tid & 3;
+    const int v_tb = tid / kChunks, v_j = tid % kChunks, v_g = 8 * v_j / G;
+    const bool has_v = v_tb < kTileKeys / 4;
+    uint32_t kw[kSteps];
+    typename PairsOf<GN>::type ks;
+    u32x4 vw;
+    half4_t vs, vz;
+    auto load = [&](int key, int k_page, int v_page) {
+        const bool k_there = k_page >= 0 && k_page < a.s.num_pages, v_there = v_page >= 0 && v_page < a.s.num_pages;
+        const int k_in = (key + k_tok) & (a.s.page() - 1), v_in = ((key + 4 * v_tb) & (a.s.page() - 1)) >> 2;
+        const uint8_t* kb = a.cache + ((int64_t)(k_there ? k_page : 0) * a.s.kvh + g) * a.s.block();
+        const uint8_t* kp = kb + k_in * (HD / 2) + k_t * (HD / 8);
+        if constexpr (kSteps == 4) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(kp);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) kw[s] = w[s];
+        } else {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(kp);
+            kw[0] = w.x;
+            kw[1] = w.y;
+        }
+        ks = *reinterpret_cast<const typename PairsOf<GN>::type*>(kb + 2 * a.s.k_bytes() + k_in * (4 * GN));
+        if (has_v) {
+            const uint8_t* vb = a.cache + ((int64_t)(v_there ? v_page : 0) * a.s.kvh + g) * a.s.block();
+            vw = *reinterpret_cast<const u32x4*>(vb + a.s.k_bytes() + (v_in * kChunks + v_j) * 16);
+            const uint8_t* sp = vb + 2 * a.s.k_bytes() + a.s.scale_bytes() + (v_in * GN + v_g) * 16;
+            vs = *reinterpret_cast<const half4_t*>(sp);
+            vz = *reinterpret_cast<const half4_t*>(sp + 8);
+        }
+    };
+    const uint32_t base = base16_vgpr();
+    auto store = [&](int buf, int key, int k_page, int v_page) {
+        half_t *lk = lds[buf], *lv = lk + kK, *lz = lv + kV;
+        if (k_page < 0 || k_page >= a.s.num_pages) {     // outside the cache: NaN for the queries that see it
+#pragma unroll
+            for (int i = 0; i < 2 * GN; ++i) ks[i] = (half_t)NAN;
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const half_t sc = ks[2 * (32 * s / G)];
+            const half2_t s2 = {sc, sc};
+            half2_t o[4];
+            scaled_codes(kw[s], base, s2, times_minus16(s2), o);
+            *reinterpret_cast<half8_t*>(lk + k_tok * HD + 8 * k_chunk<kChunks>(k_tok, 4 * s + k_t)) =
+                half8_t{o[0].x, o[0].y, o[1].x, o[1].y, o[2].x, o[2].y, o[3].x, o[3].y};
+        }
+        half_t zk = ks[1];
+#pragma unroll
+        for (int i = 1; i < GN; ++i)
+            if (k_t == i) zk = ks[2 * i + 1];
+        if (k_t < GN) lz[k_tok * 4 + k_t] = zk;
+        if (has_v) {
+            const bool v_there = v_page >= 0 && v_page < a.s.num_pages;
+            if (!v_there || key + kTileKeys > n) {       // tokens past the length may hold anything
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!v_there || key + 4 * v_tb + r >= n) vs[r] = vz[r] = (half_t)0.0f;
+            }
+            const int chunk = 4 * (v_tb >> 3) + (v_tb & 3), sub = 4 * (v_tb >> 2 & 1);
+            const half2_t s01 = {vs[0], vs[1]}, s23 = {vs[2], vs[3]};
+            const half2_t m01 = times_minus16(s01), m23 = times_minus16(s23);
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                const uint32_t half = part ? 0x07060302u : 0x05040100u;
+                half2_t p01[4], p23[4];
+                scaled_codes(__builtin_amdgcn_perm(vw[1], vw[0], half), base, s01, m01, p01);
+                scaled_codes(__builtin_amdgcn_perm(vw[3], vw[2], half), base, s23, m23, p23);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int d = 8 * v_j + 4 * part + u;
+                    *reinterpret_cast<half4_t*>(lv + d * kTileKeys + 8 * v_chunk(d, chunk) + sub) =
+                        half4_t{p01[u].x, p01[u].y, p23[u].x, p23[u].y};
+                }
+            }
+            if (8 * v_j % G == 0) {
+                const int d = HD + v_g;
+                *reinterpret_cast<half4_t*>(lv + d * kTileKeys + 8 * v_chunk(d, chunk) + sub) = vz;
+            }
+        }
+    };
+    auto pages = [&](int key, int& k_page, int& v_page) {
+        k_page = page_at(a, table, key + k_tok, n);
+        v_page = page_at(a, table, key + 4 * v_tb, n);
+    };
+
+    int kp0 = -1, vp0 = -1, kp1 = -1, vp1 = -1;          // pages of the tile in registers, and of the one after
+    if (tiles > 0) {
+        pages(start, kp0, vp0);
+        load(start, kp0, vp0);
+        pages(start + kTileKeys, kp1, vp1);
+    }
+
+    half8_t q[NQ][kSteps], qz[NQ];
+    float unit[NQ];
+    int exp[NQ], lim[NQ];
+    const float factor = a.scale * 1.4426950408889634f;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        const int c = c0 + 16 * (NQ * wave + i) + col, cc = c < all_cols ? c : all_cols - 1;
+        lim[i] = limit_of(cc);
+        exp[i] = load_query<HD, GN, BF16>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + cc / group) * a.ld +
+                                              (int64_t)(g * group + cc % group) * HD, t, q[i], qz[i]);
+        unit[i] = __builtin_ldexpf(factor, -exp[i]);
+    }
+    const int lim_min = __builtin_amdgcn_readlane(lim[0], 0), lim_max = __builtin_amdgcn_readlane(lim[NQ - 1], 15);
+
+    float m[NQ];
+    floatx4 acc[NQ][kDb + 1];                            // [kDb]: rows 0 .. GN - 1 the groups' zeros, row 4 the sum
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        m[i] = -INFINITY;
+#pragma unroll
+        for (int d = 0; d <= kDb; ++d) acc[i][d] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (tiles > 0) {
+        store(0, start, kp0, vp0);
+        kp0 = kp1;
+        vp0 = vp1;
+        if (tiles > 1) {
+            load(start + kTileKeys, kp0, vp0);
+            pages(start + 2 * kTileKeys, kp1, vp1);
+        }
+    }
+    for (int tile = 0; tile < tiles; ++tile) {
+        lds_barrier();                                   // this tile's buffer is written, the other one read
+        const int key0 = start + tile * kTileKeys;
+        // The next tile goes into the other buffer and the one after it is fetched
+        // before this one is computed.
+        if (tile + 1 < tiles) {
+            store((tile + 1) & 1, key0 + kTileKeys, kp0, vp0);
+            kp0 = kp1;
+            vp0 = vp1;
+            if (tile + 2 < tiles) {
+                load(key0 + 2 * kTileKeys, kp0, vp0);
+                pages(key0 + 3 * kTileKeys, kp1, vp1);
+            }
+        }
+        if (key0 < lim_max) {
+            const half_t *lk = lds[tile & 1], *lv = lk + kK, *lz = lv + kV;
+            floatx4 s[NQ][4];
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) {
+                const int row = 16 * kb + col;
+                const half_t zk = lz[row * 4 + t];
+                const half8_t z = {zk, zk, zk, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) s[i][kb] = mfma16x16x32(z, qz[i], floatx4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int st = 0; st < kSteps; ++st) {
+                    const half8_t k =
+                        *reinterpret_cast<const half8_t*>(lk + row * HD + 8 * k_chunk<kChunks>(row, 4 * st + t));
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) s[i][kb] = mfma16x16x32(k, q[i][st], s[i][kb]);
+                }
+            }
+            if (key0 + kTileKeys > lim_min) {
+#pragma unroll
+                for (int i = 0; i < NQ; ++i)
+#pragma unroll
+                    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (key0 + 16 * kb + 4 * t + r >= lim[i]) s[i][kb][r] = -INFINITY;
+            }
+            half8_t phi[NQ][2], plo[NQ][2];
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                float mx = s[i][0][0];
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[i][kb][r]);
+                if (__any((mx - m[i]) * unit[i] > kSlack)) {
+                    const float mn = fmaxf(m[i], column_max(mx));
+                    const float alpha = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : (m[i] - mn) * unit[i]);
+#pragma unroll
+                    for (int d = 0; d <= kDb; ++d) acc[i][d] *= alpha;
+                    m[i] = mn;
+                }
+                const float ref = m[i] == -INFINITY ? 0.0f : m[i];   // nothing yet: every exponential is 0
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float p[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        p[j] = __builtin_amdgcn_exp2f((s[i][2 * h + (j >> 2)][j & 3] - ref) * unit[i]);
+                    split16(p, kPExp, phi[i][h], plo[i][h]);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int d = 0; d <= kDb; ++d) {
+                    const int row = 16 * d + col;
+                    const half8_t v =
+                        *reinterpret_cast<const half8_t*>(lv + row * kTileKeys + 8 * v_chunk(row, 4 * h + t));
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+                        acc[i][d] = mfma16x16x32(v, plo[i][h], acc[i][d]);
+                        acc[i][d] = mfma16x16x32(v, phi[i][h], acc[i][d]);
+                    }
+                }
+        }
+    }
+
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        float zero[GN];
+#pragma unroll
+        for (int j = 0; j < GN; ++j) zero[j] = __shfl(acc[i][kDb][j], col);
+        const float l = __shfl(acc[i][kDb][0], 16 + col);
+        const int local = 16 * (NQ * wave + i) + col, c = c0 + local;
+        if (c >= all_cols) continue;
+        if (it.splits == 1) {
+            uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) +
+                            ((int64_t)(it.r.row0 + c / group) * a.nh + g * group + c % group) * HD + 4 * t;
+#pragma unroll
+            for (int d = 0; d < kDb; ++d) {
+                uint32_t w[2];
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    const float z = zero[16 * d / G];
+                    const float y0 = lim[i] == 0 ? 0.0f : (acc[i][d][r] + z) / l;
+                    const float y1 = lim[i] == 0 ? 0.0f : (acc[i][d][r + 1] + z) / l;
+                    w[r / 2] = (uint32_t)to16<BF16>(y0) | ((uint32_t)to16<BF16>(y1) << 16);
+                }
+                *reinterpret_cast<u32x2*>(dst + 16 * d) = u32x2{w[0], w[1]};
+            }
+        } else {
+            float* dst = a.tile_part + (((int64_t)blockIdx.x * a.s.kvh + g) * COLS + local) * (HD + 2);
+#pragma unroll
+            for (int d = 0; d < kDb; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2)
+                    *reinterpret_cast<float2*>(dst + 16 * d + 4 * t + r) =
+                        float2{acc[i][d][r] + zero[16 * d / G], acc[i][d][r + 1] + zero[16 * d / G]};
+            if (t == 0) {
+                dst[HD] = __builtin_ldexpf(m[i], -exp[i]);
+                dst[HD + 1] = l;
+            }
+        }
     }
 }
 
-int64_t most_items(const Kv4AttnArgs& a) {
-    const int64_t rows = (int64_t)a.requests * a.max_query < a.total ? (int64_t)a.requests * a.max_query : a.total;
-    return items_per_head(a.s.kvh) + a.requests + rows * (a.nh / a.s.kvh) / kCols;
+// ---- joining the items of a row -----------------------------------------------------
+
+// out[row, head] = sum of its items' parts, each weighted by exp2(its maximum -
+// the overall maximum).  WAVES waves have a row and head: each every WAVES-th item,
+// a lane an item's weight and two columns' sums, eight loads in flight; the
+// waves meet in LDS.  All four where rows and heads are few (and items many), else one.
+template <int HD, int TCOLS, int WAVES, bool BF16>
+__global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a) {
+    constexpr int W = HD / 64;                           // columns a lane
+    __shared__ float m_lds[kWaves], l_lds[kWaves], o_lds[kWaves][HD];
+    const int group = a.nh / a.s.kvh;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int first = WAVES == 1 ? 0 : wave;
+    const int64_t all = (int64_t)a.total * a.nh;
+    const float factor = a.scale * 1.4426950408889634f;
+    constexpr int kUnits = kWaves / WAVES;               // of a workgroup
+    for (int64_t unit = (int64_t)blockIdx.x * kUnits + (WAVES == 1 ? wave : 0); unit < all;
+         unit += (int64_t)gridDim.x * kUnits) {
+        const int row = (int)(unit / a.nh), head = (int)(unit % a.nh), g = head / group;
+        const i32x4 rec = a.records[row];
+        if (rec[3] == 1) continue;
+        uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + unit * HD;
+        if (rec[3] == 0) {
+            if (first == 0)
+#pragma unroll
+                for (int i = 0; i < W; ++i) out[W * lane + i] = 0;
+            continue;
+        }
+        const bool tile = rec[1] < 0;
+        const int c = rec[0] * group + head % group, cols = tile ? TCOLS : kCols, block = c / cols, splits = rec[3];
+        const int item = tile ? ~rec[1] + rec[2] - 1 - block : rec[1] + block;
+        const int64_t step = (int64_t)rec[2] * a.s.kvh * cols * (HD + 2);
+        const float* base = (tile ? a.tile_part : a.part) + (((int64_t)item * a.s.kvh + g) * cols + c % cols) * (HD + 2);
+
+        float mx = -INFINITY, l = 0.0f, sum[W] = {};
+        for (int s0 = 0; s0 < splits; s0 += 64 * WAVES) {
+            const int mine = s0 + first + WAVES * lane;
+            const bool have = mine < splits;
+            const float* p = base + (have ? mine : 0) * step;
+            const int left = splits - s0 - first;
+            const int count = left <= 0 ? 0 : left < 64 * WAVES ? (left + WAVES - 1) / WAVES : 64;
+            float v[8][W];
+            auto fetch = [&](int j0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int at = j0 + j < count ? s0 + first + WAVES * (j0 + j) : 0;
+#pragma unroll
+                    for (int i = 0; i < W; ++i) v[j][i] = base[at * step + W * lane + i];
+                }
+            };
+            const float pm = p[HD], pl = p[HD + 1];
+            fetch(0);
+            const float own = have ? pm : -INFINITY;
+            const float top = fmaxf(mx, wave_max(own)), ref = top == -INFINITY ? 0.0f : top;
+            const float w = __builtin_amdgcn_exp2f((own - ref) * factor), old = __builtin_amdgcn_exp2f((mx - ref) * factor);
+            l = l * old + wave_sum(have ? pl * w : 0.0f);
+#pragma unroll
+            for (int i = 0; i < W; ++i) sum[i] *= old;
+            mx = top;
+            for (int j0 = 0; j0 < count; j0 += 8) {
+                if (j0) fetch(j0);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float wj = __builtin_bit_cast(
+                        float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), (j0 + j) & 63));
+#pragma unroll
+                    for (int i = 0; i < W; ++i) sum[i] = j0 + j < count ? fmaf(wj, v[j][i], sum[i]) : sum[i];
+                }
+            }
+        }
+        if constexpr (WAVES == 1) {
+            uint32_t y = 0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) y |= (uint32_t)to16<BF16>(sum[i] / l) << (16 * i);
+            if constexpr (W == 2) reinterpret_cast<uint32_t*>(out)[lane] = y;
+            else out[lane] = (uint16_t)y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) o_lds[wave][W * lane + i] = sum[i];
+            if (lane == 0) {
+                m_lds[wave] = mx;
+                l_lds[wave] = l;
+            }
+            __syncthreads();
+            if (threadIdx.x < HD) {
+                float top = m_lds[0];
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_lds[w]);
+                const float ref = top == -INFINITY ? 0.0f : top;
+                float y = 0.0f, ls = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    const float al = __builtin_amdgcn_exp2f((m_lds[w] - ref) * factor);
+                    y = fmaf(al, o_lds[w][threadIdx.x], y);
+                    ls = fmaf(al, l_lds[w], ls);
+                }
+                out[threadIdx.x] = to16<BF16>(y / ls);
+            }
+            __syncthreads();                             // the buffers are read
+        }
+    }
+}
+
+// ---- launches ----------------------------------------------------------------------------
+
+constexpr int kDecodeItems = 768;     // items that a launch aims at, all kv heads together
+constexpr int kTileItems = 512;
+constexpr int kDecodeColumns = 64;     // a request of more columns goes to the tile kernel
+constexpr int kCombineGroups = 8192;   // workgroups of the combining launch at most
+
+struct Plan {
+    bool decode, combine;
+    int tile_nq;                       // 0: no request can be the tile kernel's
+    int limit, decode_target, tile_target;
+    int64_t decode_items, tile_items;  // at most, of one kv head
+    size_t bytes(int total, int kvh, int hd) const {     // row records, then parts
+        return (size_t)total * sizeof(i32x4) +
+               (size_t)(decode_items * kCols + (tile_target ? tile_items * 64 * tile_nq : 0)) * kvh * (hd + 2) * sizeof(float);
+    }
+};
+Plan plan(int requests, int total, int max_query, int group, int kvh, bool wide) {
+    Plan p = {};
+    const int64_t rows = (int64_t)requests * max_query < total ? (int64_t)requests * max_query : total;
+    const bool tile = (int64_t)max_query * group > kDecodeColumns;
+    p.decode = !tile || requests > 1;
+    p.limit = p.decode ? kDecodeColumns : 0;             // of one request the tile kernel has whatever it is
+    if (p.decode) {
+        p.decode_target = kvh < kDecodeItems ? kDecodeItems / kvh : 1;
+        const int64_t most = (int64_t)requests * ((kDecodeColumns + kCols - 1) / kCols);
+        const int64_t blocks = requests + rows * group / kCols;
+        p.decode_items = p.decode_target + (tile && most < blocks ? most : blocks) + 1;
+    }
+    if (tile) {
+        p.tile_nq = wide && rows * group * kvh >= 3 * 256 * 128 ? 2 : 1;
+        const int64_t blocks = requests + rows * group / (64 * p.tile_nq);
+        p.tile_target = blocks * kvh < 256 ? (kvh < kTileItems ? kTileItems / kvh : 1) : 0;
+        p.tile_items = blocks + p.tile_target + 1;
+    }
+    p.combine = p.decode || p.tile_target;
+    return p;
 }
 
 template <int HD, int GN, bool BF16>
-hipError_t launch(const Kv4AttnArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL((awq_kv4_decode_kernel<HD, GN, BF16>), dim3((unsigned)most_items(a), a.s.kvh), dim3(kThreads), 0,
-                       stream, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((awq_kv4_combine_kernel<HD, BF16>), dim3(a.total, a.s.kvh), dim3(kThreads), 0, stream, a);
-    return hipGetLastError();
+hipError_t launch(Kv4AttnArgs a, hipStream_t stream) {
+    constexpr bool kWide = GN < 4;         // 128 columns of four groups would not fit the registers
+    const Plan p = plan(a.requests, a.total, a.max_query, a.nh / a.s.kvh, a.s.kvh, kWide);
+    a.limit = p.limit;
+    a.decode_target = p.decode_target;
+    a.tile_target = p.tile_target;
+    a.records = reinterpret_cast<i32x4*>(a.part);
+    a.part += (size_t)a.total * (sizeof(i32x4) / sizeof(float));
+    a.tile_part = a.part + p.decode_items * a.s.kvh * kCols * (HD + 2);
+    if (p.decode) {
+        hipLaunchKernelGGL((awq_kv4_decode_kernel<HD, GN, BF16>), dim3((unsigned)p.decode_items, a.s.kvh), dim3(kThreads),
+                           0, stream, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (p.tile_nq) {
+        auto kernel = p.tile_nq == 1 ? awq_kv4_tile_kernel<HD, GN, 1, BF16> : awq_kv4_tile_kernel<HD, GN, kWide ? 2 : 1, BF16>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)p.tile_items, a.s.kvh), dim3(kThreads), 0, stream, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (p.combine) {
+        // Four waves a row and head up to 2048 of them: the items along the tokens are many where rows are few.
+        const int64_t all = (int64_t)a.total * a.nh, groups = all <= 2048 ? all : (all + 3) / 4;
+        auto kernel = all <= 2048 ? (p.tile_nq == 1 ? awq_kv4_combine_kernel<HD, 64, 4, BF16> : awq_kv4_combine_kernel<HD, 128, 4, BF16>)
+                                  : (p.tile_nq == 1 ? awq_kv4_combine_kernel<HD, 64, 1, BF16> : awq_kv4_combine_kernel<HD, 128, 1, BF16>);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < kCombineGroups ? groups : kCombineGroups)), dim3(kThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    return hipSuccess;
 }
 
 }  // namespace
 
 size_t kv4_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd) {
-    Kv4AttnArgs a = {};
-    a.requests = requests;
-    a.total = total;
-    a.max_query = max_query;
-    a.nh = nh;
-    a.s.kvh = kvh;
-    return (size_t)most_items(a) * kvh * kCols * (hd + 2) * sizeof(float);
+    // (the group size is not known here: the larger of both)
+    const size_t one = plan(requests, total, max_query, nh / kvh, kvh, false).bytes(total, kvh, hd);
+    const size_t two = plan(requests, total, max_query, nh / kvh, kvh, true).bytes(total, kvh, hd);
+    return one > two ? one : two;
 }
 
 hipError_t launch_kv4_attention(const Kv4AttnArgs& a, bool bf16, hipStream_t stream) {

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(kThreads) void awq_page_step_kernel(PageStepArgs a)
     __shared__ int all_taken;
     const int B = a.requests, tid = threadIdx.x;
     const int count_in = a.state[B];
-    const int64_t count = count_in < 0 ? 0 : count_in < a.num_pages ? count_in : a.num_pages;
+    const int64_t count = count_in < 0 ? 0 : count_in < a.capacity ? count_in : a.capacity;
     const int64_t room = (int64_t)a.width << a.page_log2;
     if (tid == 0) all_taken = 0;
 
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kThreads) void awq_page_step_kernel(PageStepArgs a)
                 } else {
                     page = *entry;
                 }
-                slot = page >= 0 && page < a.num_pages ? (page << a.page_log2) + offset : -1;
+                slot = page >= 0 && page < (1 << (31 - a.page_log2)) ? (page << a.page_log2) + offset : -1;
             }
         }
         a.slots[row] = slot;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kThreads) void awq_page_release_kernel(PageStepArgs
     __shared__ int64_t mine[2];        // this request's pages: first place, number
     const int B = a.requests, tid = threadIdx.x, me = blockIdx.x;
     const int count_in = a.state[B];
-    const int64_t count = count_in < 0 ? 0 : count_in < a.num_pages ? count_in : a.num_pages;
+    const int64_t count = count_in < 0 ? 0 : count_in < a.capacity ? count_in : a.capacity;
     int64_t before = 0;
     for (int b0 = 0; b0 < B; b0 += kThreads) {
         const int b = b0 + tid;
@@ -133,13 +133,13 @@ __global__ __launch_bounds__(kThreads) void awq_page_release_kernel(PageStepArgs
         }
     }
     __syncthreads();
-    if (me == 0 && tid == 0) a.new_state[B] = (int)(count + before < a.num_pages ? count + before : a.num_pages);
+    if (me == 0 && tid == 0) a.new_state[B] = (int)(count + before < a.capacity ? count + before : a.capacity);
     const int64_t room = (int64_t)a.width << a.page_log2;
     int64_t len = a.state[me];
     len = len < 0 ? 0 : len < room ? len : room;
     const int64_t first = pages_of(len, a.page_log2) - mine[1];
     for (int64_t i = tid; i < mine[1]; i += kThreads)
-        if (mine[0] + i < a.num_pages) a.free_pages[mine[0] + i] = a.tables[(int64_t)me * a.width + first + i];
+        if (mine[0] + i < a.capacity) a.free_pages[mine[0] + i] = a.tables[(int64_t)me * a.width + first + i];
 }
 
 }  // namespace

@@ -7,13 +7,15 @@
 
 namespace awq {
 
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
 struct PageStepArgs {
     const int32_t* state;       // [requests + 1]: lengths, free pages
     const int32_t* tokens;      // [requests]: new tokens (step), tokens kept (release)
     int32_t* tables;            // [requests, width]
-    int32_t* free_pages;        // [num_pages]
+    int32_t* free_pages;        // [capacity]
     int32_t *new_state, *query_start, *slots, *positions, *failed;
-    int requests, total, width, num_pages, page_log2;
+    int requests, total, width, capacity, page_log2;
 };
 hipError_t launch_page_step(const PageStepArgs& a, hipStream_t stream);
 hipError_t launch_page_release(const PageStepArgs& a, hipStream_t stream);
@@ -57,6 +59,11 @@ struct Kv4AttnArgs {
     int requests, total, max_query, nh, width;
     float scale;
     Kv4Shape s;
+    // set by the launch
+    float* tile_part;
+    i32x4* records;             // [total]: what the combining launch has to know of a row
+    int limit;                  // columns up to which a request is the decode kernel's
+    int decode_target, tile_target;   // items of one kv head that the kernels aim at
 };
 size_t kv4_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd);
 hipError_t launch_kv4_attention(const Kv4AttnArgs& a, bool bf16, hipStream_t stream);

@@ -181,6 +181,8 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_tables: torch.Tensor, 
     requests, width = block_tables.shape
     if not 0 < requests <= _native.SERVE_MAX_REQUESTS or width < 1:
         raise ValueError(f"block_tables {tuple(block_tables.shape)}: need 1 to {_native.SERVE_MAX_REQUESTS} requests")
+    if width > 2**30 // cache.page_size:
+        raise ValueError("a request's tokens pass 2^30")
     _check_index(seq_lens, "seq_lens", requests, dev)
     _check_index(query_start, "query_start", requests + 1, dev)
     if max_query < 1:

@@ -37,8 +37,8 @@ def _check_i32(t: torch.Tensor, what: str, shape: tuple, dev: torch.device) -> N
 class PagedTables:
     """``block_tables`` int32 ``[requests, width]``: the pages of each request in
     order; ``state`` int32 ``[requests + 1]``: the requests' lengths, then the
-    number of free pages; ``free_pages`` int32 ``[num_pages]``, the first
-    ``state[-1]`` of them free, taken from the end."""
+    number of free pages; ``free_pages`` int32 ``[capacity]``, as many as can be free
+    at once, the first ``state[-1]`` of them free, taken from the end."""
 
     block_tables: torch.Tensor
     state: torch.Tensor
@@ -75,7 +75,7 @@ class PagedTables:
         if not 0 < requests <= MAX_REQUESTS or width < 1 or free_pages.shape[0] < 1:
             raise ValueError(f"{requests} requests of {width} pages, {free_pages.shape[0]} pages in all: need 1 to "
                              f"{MAX_REQUESTS} requests and at least one page")
-        if width > _INT_MAX // page_size - 1 or free_pages.shape[0] > _INT_MAX // page_size:
+        if width > 2**30 // page_size or free_pages.shape[0] > _INT_MAX // page_size:
             raise ValueError("token numbers pass 32 bits")
         self.block_tables, self.state, self.free_pages, self.page_size = block_tables, state, free_pages, page_size
 

@@ -94,6 +94,15 @@ def test_steps_and_releases(gpu, requests, page):
             _same(tables, walk)
 
 
+def test_free_pages_that_are_part_of_a_cache(gpu):
+    """A stack of a few pages with large numbers: numbers are not bounded by the stack's length."""
+    free = _i32([7, 2**26 - 1, 9000], gpu)
+    tables = PagedTables.of(torch.full((2, 4), -1, dtype=torch.int32, device=gpu), _i32([0, 0, 3], gpu), free, 16)
+    r = paged_step(tables, _i32([17, 1], gpu), 18)
+    assert r.slots.tolist() == [9000 * 16 + i for i in range(16)] + [(2**26 - 1) * 16, 7 * 16]
+    assert r.state.tolist() == [17, 1, 0] and tables.block_tables[:, :2].tolist() == [[9000, 2**26 - 1], [7, -1]]
+
+
 def test_refused_requests(gpu):
     """Too few pages, rows past the batch, tokens past the table, a negative number."""
     tables, walk = PagedTables(6, 4, 9, 16, gpu), Walk(6, 4, 9, 16)
