@@ -2,7 +2,7 @@
 
 ``python qwen2-7b-triton_engine_amd/build.py`` compiles every ``csrc/*.hip``
 with hipcc for gfx950 and links ``lib/libawq_w4a16.so``, then compiles the
-torch binding of the eager entry point (``csrc/awq_torch_binding.cpp``, host
+torch binding (``csrc/awq_torch_binding.cpp``, ``awq_serving_binding.cpp``, host
 C++) into ``lib/_awq_torch*.so``.  Objects go to ``_build/`` next to this
 file.  hipcc cross-compiles without a GPU.
 """
@@ -72,6 +72,7 @@ def _compile(src: str, verbose: bool) -> str:
 # host C++ against torch's headers and libraries, linked to the library
 # above and found next to it at run time.
 BINDING_SRC = os.path.join(CSRC, "awq_torch_binding.cpp")
+SERVING_BINDING_SRC = os.path.join(CSRC, "awq_serving_binding.cpp")   # the serving operators' part of it
 
 
 def _binding_path() -> str:
@@ -92,7 +93,7 @@ def build_binding(verbose: bool = False) -> str:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
            "-DTORCH_EXTENSION_NAME=_awq_torch", "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__=1",
            "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-isystem{d}" for d in incs], BINDING_SRC, "-o", tmp,
+           *[f"-isystem{d}" for d in incs], BINDING_SRC, SERVING_BINDING_SRC, "-o", tmp,
            f"-L{LIB_DIR}", "-lawq_w4a16", f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
            "-ltorch_python", "-lamdhip64", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
     if verbose:

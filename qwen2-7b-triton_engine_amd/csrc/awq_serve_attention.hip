@@ -23,6 +23,8 @@ constexpr int kCols = 16;              // (row, query head) pairs of a decode wo
 constexpr int kWaveKeys = 32;          // tokens of one inner pass of a decode wave
 constexpr int kKeys = kWaveKeys * kWaves;
 constexpr int kTileKeys = 64;          // tokens of a tile kernel's step
+constexpr int kTileThreads = 256, kTileCols = kTileThreads / 4;   // 16 columns a wave
+
 constexpr int kPExp = 14;              // the probabilities' scale before they are split: 2^14
 constexpr int kQExp = 8;               // q's largest value lies in 2^7 .. 2^8: a group's sum stays below 2^15
 
@@ -30,7 +32,7 @@ constexpr int kQExp = 8;               // q's largest value lies in 2^7 .. 2^8: 
 
 // Requests of few columns (rows times the heads that share a kv head) go to the
 // decode kernel in blocks of 16 columns, the others to the tile kernel in
-// blocks of 64 or 128.  An item is a block and a stretch of tokens.
+// blocks of kTileCols.  An item is a block and a stretch of tokens.
 struct Request {
     int row0, rows, len;               // first row, rows, tokens
 };
@@ -148,7 +150,7 @@ struct RowRecord {
 // Written by the first item of a request.
 __device__ __forceinline__ void write_records(const Kv4AttnArgs& a, const Item& it, bool tile) {
     if (it.rel != 0 || blockIdx.y != 0) return;
-    for (int i = threadIdx.x; i < it.r.rows; i += kThreads) {
+    for (int i = threadIdx.x; i < it.r.rows; i += (int)blockDim.x) {
         const bool blind = (int64_t)it.r.len - it.r.rows + i < 0;
         a.records[it.r.row0 + i] = i32x4{i, tile ? ~it.base : it.base, it.blocks,
                                          i >= a.max_query || it.splits == 1 ? 1 : blind ? 0 : it.splits};
@@ -160,8 +162,8 @@ __device__ __forceinline__ void zero_rows(const Kv4AttnArgs& a) {
     const int pieces = a.nh * a.s.hd / 8;                // of 16 bytes
     auto clear = [&](int lo, int hi) {
         u32x4* out = reinterpret_cast<u32x4*>(a.out);
-        for (int64_t i = (int64_t)lo * pieces + threadIdx.x; i < (int64_t)hi * pieces; i += kThreads) out[i] = u32x4{0, 0, 0, 0};
-        for (int i = lo + (int)threadIdx.x; i < hi; i += kThreads) a.records[i] = i32x4{0, 0, 0, 1};
+        for (int64_t i = (int64_t)lo * pieces + threadIdx.x; i < (int64_t)hi * pieces; i += blockDim.x) out[i] = u32x4{0, 0, 0, 0};
+        for (int i = lo + (int)threadIdx.x; i < hi; i += (int)blockDim.x) a.records[i] = i32x4{0, 0, 0, 1};
     };
     const int lane = threadIdx.x & 63;
     for (int b0 = 0; b0 < a.requests; b0 += 64) {
@@ -565,23 +567,26 @@ __device__ __forceinline__ int k_chunk(int row, int chunk) {
 // V: reads as K's; writes go to the same chunk of rows that are 8 apart.
 __device__ __forceinline__ int v_chunk(int row, int chunk) { return chunk ^ ((row ^ (row >> 3)) & 7); }
 
-// One workgroup: 64 NQ columns of one kv head, 16 NQ per wave, over an item's
-// tokens in tiles of 64.  The tile's codes are multiplied out once per workgroup,
-// exactly, into LDS -- K as it is, V transposed, its zeros and a row of ones as
-// rows of their own -- and every wave reads its operands there.  The codes of the
-// next tile are on their way in registers meanwhile (36 bytes a thread), so
-// that two LDS buffers and one barrier a tile suffice.
-template <int HD, int GN, int NQ, bool BF16>
-__global__ __launch_bounds__(kThreads, 2) void awq_kv4_tile_kernel(Kv4AttnArgs a) {
+// One workgroup: 16 columns of one kv head per wave, over an item's tokens in tiles of
+// 64.  The tile's codes are multiplied out once per workgroup, exactly, into LDS --
+// K as it is, V transposed, its zeros and a row of ones as rows of their own -- and
+// every wave reads its operands there.  The codes of the next tile are on their way
+// in registers meanwhile.  One LDS buffer and two barriers a tile: the room goes to
+// a third workgroup on the CU, which has work while the others wait.
+// ONE_PAGE: pages of 64 tokens and more, where a tile lies in one of them and its
+// address is the workgroup's, not a lane's.
+template <int HD, int GN, bool ONE_PAGE, bool BF16>
+__global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel(Kv4AttnArgs a) {
     constexpr int kSteps = HD / 32, kDb = HD / 16, kChunks = HD / 8, G = HD / GN;
-    constexpr int COLS = 64 * NQ;
     constexpr int kRows = HD + 16;                       // of the transposed V: columns, zeros, ones
     constexpr int kK = kTileKeys * HD, kV = kRows * kTileKeys, kZ = kTileKeys * 4;   // halfs
-    __shared__ __align__(16) half_t lds[2][kK + kV + kZ];
+    constexpr int kParts = kTileThreads / kThreads;      // threads that share 16 bytes of codes: 1 or 2
+    constexpr int kWords = kSteps / kParts;              // words of K a thread brings
+    __shared__ __align__(16) half_t buf[kK + kV + kZ];
 
     Item it;
     const int tid = threadIdx.x, lane = tid & 63;
-    if (!find_item<COLS, kTileKeys>(a, blockIdx.x, a.tile_target, it)) {
+    if (!find_item<kTileCols, kTileKeys>(a, blockIdx.x, a.tile_target, it)) {
         if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && a.limit == 0) zero_rows(a);
         return;
     }
@@ -591,94 +596,110 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv4_tile_kernel(Kv4AttnArgs a
     const int col = lane & 15, t = lane >> 4;
     // The last blocks, which see the most tokens, start first.
     const int block = it.blocks - 1 - it.rel % it.blocks, split = it.rel / it.blocks;
-    const int all_cols = columns(a, it.r.rows), c0 = block * COLS;
+    const int all_cols = columns(a, it.r.rows), c0 = block * kTileCols;
     const int n = walked(a, it.r.len);
     auto limit_of = [&](int c) {                         // tokens that a column sees
         const int64_t pos = (int64_t)it.r.len - it.r.rows + c / group;
         return pos < 0 ? 0 : pos + 1 < n ? (int)(pos + 1) : n;
     };
-    const int c_last = c0 + COLS < all_cols ? c0 + COLS - 1 : all_cols - 1;
+    const int c_last = c0 + kTileCols < all_cols ? c0 + kTileCols - 1 : all_cols - 1;
     const int start = split * it.chunk, lim_wg = limit_of(c_last);
     const int end = lim_wg < start + it.chunk ? lim_wg : start + it.chunk;
     const int tiles = end > start ? (end - start + kTileKeys - 1) / kTileKeys : 0;
     const int32_t* table = a.tables + (int64_t)it.b * a.width;
 
     // Rows of the zeros' block that no tile writes: ones at 4, else zero; zeros of no group.
-    for (int i = tid; i < 2 * (16 * kTileKeys + kZ); i += kThreads) {
-        const int b = i / (16 * kTileKeys + kZ), j = i % (16 * kTileKeys + kZ);
-        if (j < 16 * kTileKeys) {
-            const int r = j / kTileKeys;
-            if (r >= GN) lds[b][kK + HD * kTileKeys + j] = (half_t)(r == 4 ? 1.0f : 0.0f);
-        } else if ((j - 16 * kTileKeys) % 4 >= GN) {
-            lds[b][kK + kV + j - 16 * kTileKeys] = (half_t)0.0f;
+    for (int i = tid; i < 16 * kTileKeys + kZ; i += kTileThreads) {
+        const int r = i / kTileKeys;
+        if (i < 16 * kTileKeys) {
+            if (r >= GN) buf[kK + HD * kTileKeys + i] = (half_t)(r == 4 ? 1.0f : 0.0f);
+        } else if (i % 4 >= GN) {
+            buf[kK + kV + i - 16 * kTileKeys] = (half_t)0.0f;
         }
     }
 
-    // What this thread brings of a tile: K, token tid / 4, columns 32 s + 8 (tid % 4) ..; V, four
-    // tokens, eight columns (heads of 64: half of the threads).
-    const int k_tok = tid >> 2, k_t = tid & 3;
-    const int v_tb = tid / kChunks, v_j = tid % kChunks, v_g = 8 * v_j / G;
-    const bool has_v = v_tb < kTileKeys / 4;
-    uint32_t kw[kSteps];
+    // What this thread brings of a tile: of K kWords words (columns 32 s + 8 k_t .., s from
+    // k_s) of token k_tok; of V four tokens' eight columns, or half of them.
+    const int k_tok = tid / (4 * kParts), k_t = tid / kParts % 4, k_s = tid % kParts * kWords;
+    const int v_tb = tid / kParts / kChunks, v_j = tid / kParts % kChunks, v_part = tid % kParts, v_g = 8 * v_j / G;
+    const bool has_v = v_tb < kTileKeys / 4;             // (heads of 64: half of the threads)
+    typedef uint32_t words_t __attribute__((ext_vector_type(kWords > 1 ? kWords : 2)));
+    words_t kw;
     typename PairsOf<GN>::type ks;
     u32x4 vw;
     half4_t vs, vz;
-    auto load = [&](int key, int k_page, int v_page) {
-        const bool k_there = k_page >= 0 && k_page < a.s.num_pages, v_there = v_page >= 0 && v_page < a.s.num_pages;
-        const int k_in = (key + k_tok) & (a.s.page() - 1), v_in = ((key + 4 * v_tb) & (a.s.page() - 1)) >> 2;
-        const uint8_t* kb = a.cache + ((int64_t)(k_there ? k_page : 0) * a.s.kvh + g) * a.s.block();
-        const uint8_t* kp = kb + k_in * (HD / 2) + k_t * (HD / 8);
-        if constexpr (kSteps == 4) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(kp);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) kw[s] = w[s];
+    struct Pages {
+        int k, v;                                        // of this thread's token of K, of its four of V
+    };
+    auto pages = [&](int key) {
+        if constexpr (ONE_PAGE) {
+            const int p = page_at(a, table, key, n);
+            return Pages{p, p};
         } else {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(kp);
-            kw[0] = w.x;
-            kw[1] = w.y;
+            return Pages{page_at(a, table, key + k_tok, n), page_at(a, table, key + 4 * v_tb, n)};
         }
-        ks = *reinterpret_cast<const typename PairsOf<GN>::type*>(kb + 2 * a.s.k_bytes() + k_in * (4 * GN));
+    };
+    auto there = [&](int page) { return page >= 0 && page < a.s.num_pages; };
+    auto block_of = [&](int page) { return a.cache + ((int64_t)(there(page) ? page : 0) * a.s.kvh + g) * a.s.block(); };
+    const uint32_t k_ofs = k_t * (HD / 8) + 4 * k_s, v_ofs = a.s.k_bytes() + v_j * 16;
+    const uint32_t ks_ofs = 2 * a.s.k_bytes(), vs_ofs = 2 * a.s.k_bytes() + a.s.scale_bytes() + v_g * 16;
+    auto load = [&](int key, Pages p) {
+        // The token of the page that the tile or the thread begins with, and the thread's after it.
+        const int in = ONE_PAGE ? key & (a.s.page() - 1) : 0;
+        const uint8_t* kb = block_of(p.k);
+        const uint8_t* vb = ONE_PAGE ? kb : block_of(p.v);
+        const uint32_t k_in = ONE_PAGE ? k_tok : (key + k_tok) & (a.s.page() - 1);
+        const uint32_t v_in = ONE_PAGE ? v_tb : ((key + 4 * v_tb) & (a.s.page() - 1)) >> 2;
+        const uint8_t* kp = kb + in * (HD / 2);
+        if constexpr (kWords > 1) kw = *reinterpret_cast<const words_t*>(kp + k_in * (HD / 2) + k_ofs);
+        else kw.x = *reinterpret_cast<const uint32_t*>(kp + k_in * (HD / 2) + k_ofs);
+        ks = *reinterpret_cast<const typename PairsOf<GN>::type*>(kb + in * (4 * GN) + k_in * (4 * GN) + ks_ofs);
         if (has_v) {
-            const uint8_t* vb = a.cache + ((int64_t)(v_there ? v_page : 0) * a.s.kvh + g) * a.s.block();
-            vw = *reinterpret_cast<const u32x4*>(vb + a.s.k_bytes() + (v_in * kChunks + v_j) * 16);
-            const uint8_t* sp = vb + 2 * a.s.k_bytes() + a.s.scale_bytes() + (v_in * GN + v_g) * 16;
+            vw = *reinterpret_cast<const u32x4*>(vb + in * (HD / 2) + v_in * (kChunks * 16) + v_ofs);
+            const uint8_t* sp = vb + in * (4 * GN) + v_in * (16 * GN) + vs_ofs;
             vs = *reinterpret_cast<const half4_t*>(sp);
             vz = *reinterpret_cast<const half4_t*>(sp + 8);
         }
     };
     const uint32_t base = base16_vgpr();
-    auto store = [&](int buf, int key, int k_page, int v_page) {
-        half_t *lk = lds[buf], *lv = lk + kK, *lz = lv + kV;
-        if (k_page < 0 || k_page >= a.s.num_pages) {     // outside the cache: NaN for the queries that see it
+    const int v_place = 4 * (v_tb >> 3) + (v_tb & 3), v_sub = 4 * (v_tb >> 2 & 1);
+    auto store = [&](int key, Pages p) {
+        half_t *lk = buf, *lv = lk + kK, *lz = lv + kV;
+        if (!there(p.k)) {                               // outside the cache: NaN for the queries that see it
 #pragma unroll
             for (int i = 0; i < 2 * GN; ++i) ks[i] = (half_t)NAN;
         }
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const half_t sc = ks[2 * (32 * s / G)];
+        for (int j = 0; j < kWords; ++j) {
+            half_t sc;                                   // of the group of step k_s + j
+            if constexpr (kParts == 1) {
+                sc = ks[2 * (32 * j / G)];
+            } else {
+                const int of0 = 32 * j / G, of1 = 32 * (kWords + j) / G;
+                sc = of0 == of1 ? ks[2 * of0] : k_s ? ks[2 * of1] : ks[2 * of0];
+            }
             const half2_t s2 = {sc, sc};
             half2_t o[4];
-            scaled_codes(kw[s], base, s2, times_minus16(s2), o);
-            *reinterpret_cast<half8_t*>(lk + k_tok * HD + 8 * k_chunk<kChunks>(k_tok, 4 * s + k_t)) =
+            scaled_codes(kw[j], base, s2, times_minus16(s2), o);
+            *reinterpret_cast<half8_t*>(lk + k_tok * HD + 8 * k_chunk<kChunks>(k_tok, 4 * (k_s + j) + k_t)) =
                 half8_t{o[0].x, o[0].y, o[1].x, o[1].y, o[2].x, o[2].y, o[3].x, o[3].y};
         }
         half_t zk = ks[1];
 #pragma unroll
         for (int i = 1; i < GN; ++i)
             if (k_t == i) zk = ks[2 * i + 1];
-        if (k_t < GN) lz[k_tok * 4 + k_t] = zk;
+        if (k_t < GN && k_s == 0) lz[k_tok * 4 + k_t] = zk;
         if (has_v) {
-            const bool v_there = v_page >= 0 && v_page < a.s.num_pages;
-            if (!v_there || key + kTileKeys > n) {       // tokens past the length may hold anything
+            if (!there(p.v) || key + kTileKeys > n) {    // tokens past the length may hold anything
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (!v_there || key + 4 * v_tb + r >= n) vs[r] = vz[r] = (half_t)0.0f;
+                    if (!there(p.v) || key + 4 * v_tb + r >= n) vs[r] = vz[r] = (half_t)0.0f;
             }
-            const int chunk = 4 * (v_tb >> 3) + (v_tb & 3), sub = 4 * (v_tb >> 2 & 1);
             const half2_t s01 = {vs[0], vs[1]}, s23 = {vs[2], vs[3]};
             const half2_t m01 = times_minus16(s01), m23 = times_minus16(s23);
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
+            for (int j = 0; j < 2 / kParts; ++j) {
+                const int part = kParts == 1 ? j : v_part;
                 const uint32_t half = part ? 0x07060302u : 0x05040100u;
                 half2_t p01[4], p23[4];
                 scaled_codes(__builtin_amdgcn_perm(vw[1], vw[0], half), base, s01, m01, p01);
@@ -686,176 +707,128 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv4_tile_kernel(Kv4AttnArgs a
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const int d = 8 * v_j + 4 * part + u;
-                    *reinterpret_cast<half4_t*>(lv + d * kTileKeys + 8 * v_chunk(d, chunk) + sub) =
+                    *reinterpret_cast<half4_t*>(lv + d * kTileKeys + 8 * v_chunk(d, v_place) + v_sub) =
                         half4_t{p01[u].x, p01[u].y, p23[u].x, p23[u].y};
                 }
             }
-            if (8 * v_j % G == 0) {
+            if (8 * v_j % G == 0 && v_part == 0) {
                 const int d = HD + v_g;
-                *reinterpret_cast<half4_t*>(lv + d * kTileKeys + 8 * v_chunk(d, chunk) + sub) = vz;
+                *reinterpret_cast<half4_t*>(lv + d * kTileKeys + 8 * v_chunk(d, v_place) + v_sub) = vz;
             }
         }
     };
-    auto pages = [&](int key, int& k_page, int& v_page) {
-        k_page = page_at(a, table, key + k_tok, n);
-        v_page = page_at(a, table, key + 4 * v_tb, n);
-    };
 
-    int kp0 = -1, vp0 = -1, kp1 = -1, vp1 = -1;          // pages of the tile in registers, and of the one after
+    Pages now = {-1, -1}, next = {-1, -1};               // of the tile in registers, and of the one after it
     if (tiles > 0) {
-        pages(start, kp0, vp0);
-        load(start, kp0, vp0);
-        pages(start + kTileKeys, kp1, vp1);
+        now = pages(start);
+        load(start, now);
+        next = pages(start + kTileKeys);
     }
 
-    half8_t q[NQ][kSteps], qz[NQ];
-    float unit[NQ];
-    int exp[NQ], lim[NQ];
-    const float factor = a.scale * 1.4426950408889634f;
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-        const int c = c0 + 16 * (NQ * wave + i) + col, cc = c < all_cols ? c : all_cols - 1;
-        lim[i] = limit_of(cc);
-        exp[i] = load_query<HD, GN, BF16>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + cc / group) * a.ld +
-                                              (int64_t)(g * group + cc % group) * HD, t, q[i], qz[i]);
-        unit[i] = __builtin_ldexpf(factor, -exp[i]);
-    }
-    const int lim_min = __builtin_amdgcn_readlane(lim[0], 0), lim_max = __builtin_amdgcn_readlane(lim[NQ - 1], 15);
+    half8_t q[kSteps], qz;
+    const int local = 16 * wave + col, c = c0 + local, cc = c < all_cols ? c : all_cols - 1;
+    const int lim = limit_of(cc);
+    const int exp = load_query<HD, GN, BF16>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + cc / group) * a.ld +
+                                                 (int64_t)(g * group + cc % group) * HD, t, q, qz);
+    const float factor = a.scale * 1.4426950408889634f, unit = __builtin_ldexpf(factor, -exp);
+    const int lim_min = __builtin_amdgcn_readlane(lim, 0), lim_max = __builtin_amdgcn_readlane(lim, 15);
 
-    float m[NQ];
-    floatx4 acc[NQ][kDb + 1];                            // [kDb]: rows 0 .. GN - 1 the groups' zeros, row 4 the sum
+    float m = -INFINITY;
+    floatx4 acc[kDb + 1];                                // [kDb]: rows 0 .. GN - 1 the groups' zeros, row 4 the sum
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-        m[i] = -INFINITY;
+    for (int d = 0; d <= kDb; ++d) acc[d] = floatx4{0.f, 0.f, 0.f, 0.f};
+    // Operand addresses: the swizzles only flip bits that the rows' starts leave free.
+    const uint32_t k_at = col * HD + 8 * k_chunk<kChunks>(col, t);
+    uint32_t v_at[4];
 #pragma unroll
-        for (int d = 0; d <= kDb; ++d) acc[i][d] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
-    if (tiles > 0) {
-        store(0, start, kp0, vp0);
-        kp0 = kp1;
-        vp0 = vp1;
-        if (tiles > 1) {
-            load(start + kTileKeys, kp0, vp0);
-            pages(start + 2 * kTileKeys, kp1, vp1);
-        }
-    }
+    for (int d = 0; d < 4; ++d) v_at[d] = kK + (16 * d + col) * kTileKeys + 8 * v_chunk(16 * d + col, t);
     for (int tile = 0; tile < tiles; ++tile) {
-        lds_barrier();                                   // this tile's buffer is written, the other one read
         const int key0 = start + tile * kTileKeys;
-        // The next tile goes into the other buffer and the one after it is fetched
-        // before this one is computed.
-        if (tile + 1 < tiles) {
-            store((tile + 1) & 1, key0 + kTileKeys, kp0, vp0);
-            kp0 = kp1;
-            vp0 = vp1;
-            if (tile + 2 < tiles) {
-                load(key0 + 2 * kTileKeys, kp0, vp0);
-                pages(key0 + 3 * kTileKeys, kp1, vp1);
-            }
+        if (tile) lds_barrier();                         // every wave has read the tile before
+        store(key0, now);
+        if (tile + 1 < tiles) {                          // the next tile's codes, in flight under this one
+            now = next;
+            load(key0 + kTileKeys, now);
+            next = pages(key0 + 2 * kTileKeys);
         }
-        if (key0 < lim_max) {
-            const half_t *lk = lds[tile & 1], *lv = lk + kK, *lz = lv + kV;
-            floatx4 s[NQ][4];
+        lds_barrier();
+        if (key0 >= lim_max) continue;                   // past every column of this wave
+        // 32 tokens at a time: half the scores are alive.
 #pragma unroll
-            for (int kb = 0; kb < 4; ++kb) {
-                const int row = 16 * kb + col;
-                const half_t zk = lz[row * 4 + t];
+        for (int h = 0; h < 2; ++h) {
+            floatx4 s[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int kb = 2 * h + b;
+                const half_t zk = buf[kK + kV + (16 * kb + col) * 4 + t];
                 const half8_t z = {zk, zk, zk, 0, 0, 0, 0, 0};
+                s[b] = mfma16x16x32(z, qz, floatx4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-                for (int i = 0; i < NQ; ++i) s[i][kb] = mfma16x16x32(z, qz[i], floatx4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                for (int st = 0; st < kSteps; ++st) {
-                    const half8_t k =
-                        *reinterpret_cast<const half8_t*>(lk + row * HD + 8 * k_chunk<kChunks>(row, 4 * st + t));
-#pragma unroll
-                    for (int i = 0; i < NQ; ++i) s[i][kb] = mfma16x16x32(k, q[i][st], s[i][kb]);
-                }
+                for (int st = 0; st < kSteps; ++st)
+                    s[b] = mfma16x16x32(*reinterpret_cast<const half8_t*>(buf + (k_at ^ (32 * st)) + 16 * kb * HD), q[st], s[b]);
             }
-            if (key0 + kTileKeys > lim_min) {
+            if (key0 + 32 * h + 32 > lim_min) {
 #pragma unroll
-                for (int i = 0; i < NQ; ++i)
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (key0 + 16 * kb + 4 * t + r >= lim[i]) s[i][kb][r] = -INFINITY;
+                    for (int r = 0; r < 4; ++r)
+                        if (key0 + 32 * h + 16 * b + 4 * t + r >= lim) s[b][r] = -INFINITY;
             }
-            half8_t phi[NQ][2], plo[NQ][2];
+            float mx = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) {
-                float mx = s[i][0][0];
+            for (int r = 1; r < 4; ++r) mx = fmaxf(mx, fmaxf(s[0][r], s[1][r]));
+            if (__any((mx - m) * unit > kSlack)) {
+                const float mn = fmaxf(m, column_max(mx));
+                const float alpha = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : (m - mn) * unit);
 #pragma unroll
-                for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[i][kb][r]);
-                if (__any((mx - m[i]) * unit[i] > kSlack)) {
-                    const float mn = fmaxf(m[i], column_max(mx));
-                    const float alpha = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : (m[i] - mn) * unit[i]);
-#pragma unroll
-                    for (int d = 0; d <= kDb; ++d) acc[i][d] *= alpha;
-                    m[i] = mn;
-                }
-                const float ref = m[i] == -INFINITY ? 0.0f : m[i];   // nothing yet: every exponential is 0
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float p[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        p[j] = __builtin_amdgcn_exp2f((s[i][2 * h + (j >> 2)][j & 3] - ref) * unit[i]);
-                    split16(p, kPExp, phi[i][h], plo[i][h]);
-                }
+                for (int d = 0; d <= kDb; ++d) acc[d] *= alpha;
+                m = mn;
             }
+            const float ref = m == -INFINITY ? 0.0f : m;     // nothing yet: every exponential is 0
+            float p[8];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f((s[j >> 2][j & 3] - ref) * unit);
+            half8_t phi, plo;
+            split16(p, kPExp, phi, plo);
 #pragma unroll
-                for (int d = 0; d <= kDb; ++d) {
-                    const int row = 16 * d + col;
-                    const half8_t v =
-                        *reinterpret_cast<const half8_t*>(lv + row * kTileKeys + 8 * v_chunk(row, 4 * h + t));
-#pragma unroll
-                    for (int i = 0; i < NQ; ++i) {
-                        acc[i][d] = mfma16x16x32(v, plo[i][h], acc[i][d]);
-                        acc[i][d] = mfma16x16x32(v, phi[i][h], acc[i][d]);
-                    }
-                }
+            for (int d = 0; d <= kDb; ++d) {
+                const half8_t v = *reinterpret_cast<const half8_t*>(buf + (v_at[d & 3] ^ (32 * h)) + (d & ~3) * 16 * kTileKeys);
+                acc[d] = mfma16x16x32(v, plo, acc[d]);
+                acc[d] = mfma16x16x32(v, phi, acc[d]);
+            }
         }
     }
 
+    float zero[GN];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-        float zero[GN];
+    for (int j = 0; j < GN; ++j) zero[j] = __shfl(acc[kDb][j], col);
+    const float l = __shfl(acc[kDb][0], 16 + col);
+    if (c >= all_cols) return;
+    if (it.splits == 1) {
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) +
+                        ((int64_t)(it.r.row0 + c / group) * a.nh + g * group + c % group) * HD + 4 * t;
 #pragma unroll
-        for (int j = 0; j < GN; ++j) zero[j] = __shfl(acc[i][kDb][j], col);
-        const float l = __shfl(acc[i][kDb][0], 16 + col);
-        const int local = 16 * (NQ * wave + i) + col, c = c0 + local;
-        if (c >= all_cols) continue;
-        if (it.splits == 1) {
-            uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) +
-                            ((int64_t)(it.r.row0 + c / group) * a.nh + g * group + c % group) * HD + 4 * t;
+        for (int d = 0; d < kDb; ++d) {
+            uint32_t w[2];
 #pragma unroll
-            for (int d = 0; d < kDb; ++d) {
-                uint32_t w[2];
-#pragma unroll
-                for (int r = 0; r < 4; r += 2) {
-                    const float z = zero[16 * d / G];
-                    const float y0 = lim[i] == 0 ? 0.0f : (acc[i][d][r] + z) / l;
-                    const float y1 = lim[i] == 0 ? 0.0f : (acc[i][d][r + 1] + z) / l;
-                    w[r / 2] = (uint32_t)to16<BF16>(y0) | ((uint32_t)to16<BF16>(y1) << 16);
-                }
-                *reinterpret_cast<u32x2*>(dst + 16 * d) = u32x2{w[0], w[1]};
+            for (int r = 0; r < 4; r += 2) {
+                const float z = zero[16 * d / G];
+                const float y0 = lim == 0 ? 0.0f : (acc[d][r] + z) / l, y1 = lim == 0 ? 0.0f : (acc[d][r + 1] + z) / l;
+                w[r / 2] = (uint32_t)to16<BF16>(y0) | ((uint32_t)to16<BF16>(y1) << 16);
             }
-        } else {
-            float* dst = a.tile_part + (((int64_t)blockIdx.x * a.s.kvh + g) * COLS + local) * (HD + 2);
+            *reinterpret_cast<u32x2*>(dst + 16 * d) = u32x2{w[0], w[1]};
+        }
+    } else {
+        float* dst = a.tile_part + (((int64_t)blockIdx.x * a.s.kvh + g) * kTileCols + local) * (HD + 2);
 #pragma unroll
-            for (int d = 0; d < kDb; ++d)
+        for (int d = 0; d < kDb; ++d)
 #pragma unroll
-                for (int r = 0; r < 4; r += 2)
-                    *reinterpret_cast<float2*>(dst + 16 * d + 4 * t + r) =
-                        float2{acc[i][d][r] + zero[16 * d / G], acc[i][d][r + 1] + zero[16 * d / G]};
-            if (t == 0) {
-                dst[HD] = __builtin_ldexpf(m[i], -exp[i]);
-                dst[HD + 1] = l;
-            }
+            for (int r = 0; r < 4; r += 2)
+                *reinterpret_cast<float2*>(dst + 16 * d + 4 * t + r) =
+                    float2{acc[d][r] + zero[16 * d / G], acc[d][r + 1] + zero[16 * d / G]};
+        if (t == 0) {
+            dst[HD] = __builtin_ldexpf(m, -exp);
+            dst[HD + 1] = l;
         }
     }
 }
@@ -866,7 +839,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv4_tile_kernel(Kv4AttnArgs a
 // the overall maximum).  WAVES waves have a row and head: each every WAVES-th item,
 // a lane an item's weight and two columns' sums, eight loads in flight; the
 // waves meet in LDS.  All four where rows and heads are few (and items many), else one.
-template <int HD, int TCOLS, int WAVES, bool BF16>
+template <int HD, int WAVES, bool BF16>
 __global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a) {
     constexpr int W = HD / 64;                           // columns a lane
     __shared__ float m_lds[kWaves], l_lds[kWaves], o_lds[kWaves][HD];
@@ -889,7 +862,7 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a
             continue;
         }
         const bool tile = rec[1] < 0;
-        const int c = rec[0] * group + head % group, cols = tile ? TCOLS : kCols, block = c / cols, splits = rec[3];
+        const int c = rec[0] * group + head % group, cols = tile ? kTileCols : kCols, block = c / cols, splits = rec[3];
         const int item = tile ? ~rec[1] + rec[2] - 1 - block : rec[1] + block;
         const int64_t step = (int64_t)rec[2] * a.s.kvh * cols * (HD + 2);
         const float* base = (tile ? a.tile_part : a.part) + (((int64_t)item * a.s.kvh + g) * cols + c % cols) * (HD + 2);
@@ -965,36 +938,34 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a
 
 // ---- launches ----------------------------------------------------------------------------
 
-constexpr int kDecodeItems = 768;     // items that a launch aims at, all kv heads together
+constexpr int kDecodeItems = 512;     // items that a launch aims at, all kv heads together
 constexpr int kTileItems = 512;
 constexpr int kDecodeColumns = 64;     // a request of more columns goes to the tile kernel
 constexpr int kCombineGroups = 8192;   // workgroups of the combining launch at most
 
 struct Plan {
-    bool decode, combine;
-    int tile_nq;                       // 0: no request can be the tile kernel's
+    bool decode, tile, combine;
     int limit, decode_target, tile_target;
     int64_t decode_items, tile_items;  // at most, of one kv head
     size_t bytes(int total, int kvh, int hd) const {     // row records, then parts
         return (size_t)total * sizeof(i32x4) +
-               (size_t)(decode_items * kCols + (tile_target ? tile_items * 64 * tile_nq : 0)) * kvh * (hd + 2) * sizeof(float);
+               (size_t)(decode_items * kCols + (tile_target ? tile_items * kTileCols : 0)) * kvh * (hd + 2) * sizeof(float);
     }
 };
-Plan plan(int requests, int total, int max_query, int group, int kvh, bool wide) {
+Plan plan(int requests, int total, int max_query, int group, int kvh) {
     Plan p = {};
     const int64_t rows = (int64_t)requests * max_query < total ? (int64_t)requests * max_query : total;
-    const bool tile = (int64_t)max_query * group > kDecodeColumns;
-    p.decode = !tile || requests > 1;
+    p.tile = (int64_t)max_query * group > kDecodeColumns;
+    p.decode = !p.tile || requests > 1;
     p.limit = p.decode ? kDecodeColumns : 0;             // of one request the tile kernel has whatever it is
     if (p.decode) {
         p.decode_target = kvh < kDecodeItems ? kDecodeItems / kvh : 1;
         const int64_t most = (int64_t)requests * ((kDecodeColumns + kCols - 1) / kCols);
         const int64_t blocks = requests + rows * group / kCols;
-        p.decode_items = p.decode_target + (tile && most < blocks ? most : blocks) + 1;
+        p.decode_items = p.decode_target + (p.tile && most < blocks ? most : blocks) + 1;
     }
-    if (tile) {
-        p.tile_nq = wide && rows * group * kvh >= 3 * 256 * 128 ? 2 : 1;
-        const int64_t blocks = requests + rows * group / (64 * p.tile_nq);
+    if (p.tile) {
+        const int64_t blocks = requests + rows * group / kTileCols;
         p.tile_target = blocks * kvh < 256 ? (kvh < kTileItems ? kTileItems / kvh : 1) : 0;
         p.tile_items = blocks + p.tile_target + 1;
     }
@@ -1004,8 +975,7 @@ Plan plan(int requests, int total, int max_query, int group, int kvh, bool wide)
 
 template <int HD, int GN, bool BF16>
 hipError_t launch(Kv4AttnArgs a, hipStream_t stream) {
-    constexpr bool kWide = GN < 4;         // 128 columns of four groups would not fit the registers
-    const Plan p = plan(a.requests, a.total, a.max_query, a.nh / a.s.kvh, a.s.kvh, kWide);
+    const Plan p = plan(a.requests, a.total, a.max_query, a.nh / a.s.kvh, a.s.kvh);
     a.limit = p.limit;
     a.decode_target = p.decode_target;
     a.tile_target = p.tile_target;
@@ -1018,17 +988,16 @@ hipError_t launch(Kv4AttnArgs a, hipStream_t stream) {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (p.tile_nq) {
-        auto kernel = p.tile_nq == 1 ? awq_kv4_tile_kernel<HD, GN, 1, BF16> : awq_kv4_tile_kernel<HD, GN, kWide ? 2 : 1, BF16>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)p.tile_items, a.s.kvh), dim3(kThreads), 0, stream, a);
+    if (p.tile) {
+        auto kernel = a.s.page() >= kTileKeys ? awq_kv4_tile_kernel<HD, GN, true, BF16> : awq_kv4_tile_kernel<HD, GN, false, BF16>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)p.tile_items, a.s.kvh), dim3(kTileThreads), 0, stream, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     if (p.combine) {
         // Four waves a row and head up to 2048 of them: the items along the tokens are many where rows are few.
         const int64_t all = (int64_t)a.total * a.nh, groups = all <= 2048 ? all : (all + 3) / 4;
-        auto kernel = all <= 2048 ? (p.tile_nq == 1 ? awq_kv4_combine_kernel<HD, 64, 4, BF16> : awq_kv4_combine_kernel<HD, 128, 4, BF16>)
-                                  : (p.tile_nq == 1 ? awq_kv4_combine_kernel<HD, 64, 1, BF16> : awq_kv4_combine_kernel<HD, 128, 1, BF16>);
+        auto kernel = all <= 2048 ? awq_kv4_combine_kernel<HD, 4, BF16> : awq_kv4_combine_kernel<HD, 1, BF16>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < kCombineGroups ? groups : kCombineGroups)), dim3(kThreads), 0, stream, a);
         return hipGetLastError();
     }
@@ -1038,10 +1007,7 @@ hipError_t launch(Kv4AttnArgs a, hipStream_t stream) {
 }  // namespace
 
 size_t kv4_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd) {
-    // (the group size is not known here: the larger of both)
-    const size_t one = plan(requests, total, max_query, nh / kvh, kvh, false).bytes(total, kvh, hd);
-    const size_t two = plan(requests, total, max_query, nh / kvh, kvh, true).bytes(total, kvh, hd);
-    return one > two ? one : two;
+    return plan(requests, total, max_query, nh / kvh, kvh).bytes(total, kvh, hd);
 }
 
 hipError_t launch_kv4_attention(const Kv4AttnArgs& a, bool bf16, hipStream_t stream) {

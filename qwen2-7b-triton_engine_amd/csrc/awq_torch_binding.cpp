@@ -36,6 +36,10 @@
 #include <vector>
 
 #include "../../include/awq_w4a16.h"
+#include "awq_binding.h"
+
+using awq_binding::aligned16;
+using awq_binding::check_status;
 
 namespace {
 
@@ -69,12 +73,24 @@ std::unordered_map<int, std::vector<at::Tensor>> g_workspaces;
 // when the module is loaded and held until the process ends.
 PyObject* g_status_error = nullptr;
 
+}  // namespace
+
+namespace awq_binding {
+
 void check_status(int st, const char* where) {
     if (st == AWQ_OK) return;
     TORCH_CHECK(g_status_error != nullptr, where, ": status ", st, ": ", awq_w4a16_error_string(st));
     PyErr_SetObject(g_status_error, py::make_tuple(st, where).ptr());
     throw py::error_already_set();
 }
+
+at::Tensor aligned16(const at::Tensor& t) {
+    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0 ? t : t.clone();
+}
+
+}  // namespace awq_binding
+
+namespace {
 
 // The plan for a shape on a device (the planner sizes grids by the device's
 // compute units, so the device must be current when it plans).
@@ -99,12 +115,6 @@ at::Tensor& workspace_for(const at::Device& device, uint64_t bytes, hipStream_t 
     const int64_t size = ((int64_t)bytes + kWorkspaceAlign - 1) / kWorkspaceAlign * kWorkspaceAlign;
     bufs.push_back(at::zeros({size / 4}, at::TensorOptions().dtype(at::kFloat).device(device)));
     return bufs.back();
-}
-
-// `t` when its data starts on a 16-byte boundary, else a copy (the kernels use
-// 16-byte vector accesses; the reference's Triton path takes any view).
-at::Tensor aligned16(const at::Tensor& t) {
-    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0 ? t : t.clone();
 }
 
 // The operands of one projection, checked: ValueError for a bad one.
@@ -343,5 +353,6 @@ PYBIND11_MODULE(_awq_torch, m) {
     m.def("workspace_buffers", &workspace_buffers, "every workspace buffer of a device", py::arg("device_index"));
     m.def("set_status_error", [](const py::object& type) { g_status_error = type.inc_ref().ptr(); },
           "the exception class for a status of the C ABI", py::arg("type"));
+    awq_binding::define_serving(m);
     m.def("abi_version", [] { return awq_w4a16_abi_version(); });
 }

@@ -18,7 +18,6 @@ import dataclasses
 import torch
 
 from . import _native
-from .awq_gemm import _OnDevice, _stream_handle
 
 __all__ = ["PagedTables", "PagedStep", "paged_step", "paged_release", "MAX_REQUESTS", "PAGE_SIZES"]
 
@@ -128,45 +127,14 @@ def paged_step(tables: PagedTables, new_tokens: torch.Tensor, total: int, out: P
     rows pass ``total``, whose tokens pass its table's width, or for which and all
     before it the free pages do not suffice.  ``out``: a step of the same sizes
     whose tensors are reused (not the one whose ``state`` the tables hold)."""
-    requests, width = tables.block_tables.shape
-    dev = tables.state.device
-    if dev.type != "cuda":
-        raise ValueError(f"the tables must be on a ROCm device, got {dev}")
-    if new_tokens.dtype is not torch.int32 or new_tokens.shape != (requests,) or new_tokens.device != dev \
-            or not new_tokens.is_contiguous():
-        raise ValueError(f"new_tokens must be a contiguous int32 tensor {(requests,)} on {dev}")
-    if total < 0 or total > _INT_MAX // 2:
-        raise ValueError(f"total {total} must be in [0, {_INT_MAX // 2}]")
-    if out is None:
-        out = PagedStep.empty(requests, total, dev)
-    else:
-        for name, n in (("state", requests + 1), ("query_start", requests + 1), ("slots", total), ("positions", total),
-                        ("failed", requests)):
-            _check_i32(getattr(out, name), f"out.{name}", (n,), dev)
-        if out.state.data_ptr() == tables.state.data_ptr():
-            raise ValueError("out.state is the tables' own state: the step reads it while it writes")
-    with _OnDevice(dev):
-        st = _native.lib().awq_serve_page_step(
-            tables.state.data_ptr(), new_tokens.data_ptr(), tables.block_tables.data_ptr(),
-            tables.free_pages.data_ptr(), out.state.data_ptr(), out.query_start.data_ptr(), out.slots.data_ptr(),
-            out.positions.data_ptr(), out.failed.data_ptr(), requests, total, width, tables.free_pages.shape[0],
-            tables.page_size, _stream_handle(dev))
-    _native.check(st, "awq_serve_page_step")
-    return out
+    r = _native.binding().paged_step(
+        tables.state, new_tokens, tables.block_tables, tables.free_pages, tables.page_size, total,
+        None if out is None else [out.state, out.query_start, out.slots, out.positions, out.failed])
+    return PagedStep(*r) if out is None else out
 
 
 def paged_release(tables: PagedTables, keep: torch.Tensor) -> None:
     """Request b keeps its first ``keep[b]`` tokens (int32 ``[requests]``; 0: the request
     ended) and returns the pages past them."""
-    requests, width = tables.block_tables.shape
-    dev = tables.state.device
-    if dev.type != "cuda":
-        raise ValueError(f"the tables must be on a ROCm device, got {dev}")
-    _check_i32(keep, "keep", (requests,), dev)
-    state = torch.empty_like(tables.state)
-    with _OnDevice(dev):
-        st = _native.lib().awq_serve_page_release(
-            tables.state.data_ptr(), keep.data_ptr(), tables.block_tables.data_ptr(), tables.free_pages.data_ptr(),
-            state.data_ptr(), requests, width, tables.free_pages.shape[0], tables.page_size, _stream_handle(dev))
-    _native.check(st, "awq_serve_page_release")
-    tables.state = state
+    tables.state = _native.binding().paged_release(tables.state, keep, tables.block_tables, tables.free_pages,
+                                                   tables.page_size)
