@@ -86,7 +86,8 @@ extern "C" {
  * slots int32 [total], page * page_size + offset; positions int32 [total];
  * failed int32 [requests], 1 where refused.  Rows behind the last request's have
  * slot -1 and position -1.  No output may overlap an input.  page_size: a power of
- * two of 16 .. 256.  One launch. */
+ * two of 16 .. 256; total and capacity at most 2^24, table_width * page_size at
+ * most 2^30.  One launch. */
 int awq_serve_page_step(const int32_t* state, const int32_t* new_tokens, int32_t* block_tables,
                         const int32_t* free_pages, int32_t* new_state, int32_t* query_start, int32_t* slots,
                         int32_t* positions, int32_t* failed, int64_t requests, int64_t total, int64_t table_width,

@@ -10,6 +10,7 @@ using namespace awq;
 namespace {
 
 constexpr int64_t kIndexLimit = INT_MAX;
+constexpr int64_t kMostRows = 1 << 24, kMostPages = 1 << 24;   // of a step: 32-bit sums over a wave
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
@@ -45,6 +46,7 @@ int check_cache(int64_t kvh, int64_t hd, int64_t num_pages, int64_t page_size, i
 int check_step(const PageStepArgs& a, int64_t requests, int64_t width, int64_t capacity, int64_t page_size) {
     const int st = check_pages(requests, width, capacity, page_size);
     if (st != AWQ_OK) return st;
+    if (capacity > kMostPages) return AWQ_ERR_TOO_LARGE;
     if (!a.state || !a.tokens || !a.tables || !a.free_pages || !a.new_state) return AWQ_ERR_NULL_POINTER;
     if (!aligned(a.state, 4) || !aligned(a.tokens, 4) || !aligned(a.tables, 4) || !aligned(a.free_pages, 4) ||
         !aligned(a.new_state, 4))
@@ -73,7 +75,7 @@ int awq_serve_page_step(const int32_t* state, const int32_t* new_tokens, int32_t
     const int st = check_step(a, requests, table_width, capacity, page_size);
     if (st != AWQ_OK) return st;
     if (total < 0) return AWQ_ERR_BAD_DIMS;
-    if (total > kIndexLimit / 2) return AWQ_ERR_TOO_LARGE;
+    if (total > kMostRows) return AWQ_ERR_TOO_LARGE;
     if (!query_start || !failed || (total > 0 && (!slots || !positions))) return AWQ_ERR_NULL_POINTER;
     if (!aligned(query_start, 4) || !aligned(failed, 4) || !aligned(slots, 4) || !aligned(positions, 4))
         return AWQ_ERR_MISALIGNED;

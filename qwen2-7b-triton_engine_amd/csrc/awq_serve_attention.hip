@@ -72,17 +72,6 @@ struct Item {
     int base, rel;                     // number of the request's first item; this item's after it
 };
 
-// Sums over the lanes up to this one.
-__device__ __forceinline__ int wave_scan32(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);    // row_shr:1
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2 and 3
-    return v;
-}
-
 // Finds an item by its number.  Every wave walks over the requests' lengths by
 // itself, 64 at a time and without a barrier: no launch has to prepare a list,
 // and the host need not know the lengths.  The tokens of an item are a multiple of

@@ -7,10 +7,11 @@
 // occurs in the row's history.  A counter per token in memory would be a
 // second tensor as large as the logits, to be kept from step to step; here a
 // workgroup has a stretch of the vocabulary, counts the history's tokens that
-// fall into it in LDS (integers: the order of the atomics does not matter)
-// and then passes over its logits.  The history is read once per stretch, out
-// of the caches.  Of a token biased twice the last entry counts, found the
-// same way as the largest index.
+// fall into it in LDS (integers: the order of the atomics does not matter) and
+// lists each at its first count.  Of a token biased twice the last entry counts, found
+// as the largest index.  The listed tokens, few among many, get their new
+// logits by one thread each; then the stretch passes through, its logits loaded
+// before the counting began.  The history is read once per stretch, out of the caches.
 #include "awq_serving.h"
 
 #pragma clang fp contract(off)   // each step rounds as the same step in torch does
@@ -18,7 +19,7 @@
 namespace awq {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr uint32_t kInPrompt = 0x80000000u;   // of a counter; the rest counts generated tokens
 constexpr uint32_t kMinusInf = 0x007FFFFFu;   // order_of(-inf)
@@ -39,154 +40,198 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
     return v;
 }
 
-// VEC neighbouring logits as fp32, and back rounded once (x becomes what was stored).
-template <int DT, int VEC>
-__device__ __forceinline__ void load_logits(const void* p, int64_t at, float (&x)[VEC]) {
-    if constexpr (DT == AWQ_SERVE_FP32) {
-        const float* f = reinterpret_cast<const float*>(p) + at;
-        if constexpr (VEC == 8) {
-            const floatx4 lo = reinterpret_cast<const floatx4*>(f)[0], hi = reinterpret_cast<const floatx4*>(f)[1];
+// Eight neighbouring logits as they lie in memory, at any alignment of theirs
+// (vocabularies are odd, rows are strided), and as fp32.
+template <int DT>
+struct Piece {
+    static constexpr int kWords = DT == AWQ_SERVE_FP32 ? 8 : 4;
+    static constexpr int kBytes = DT == AWQ_SERVE_FP32 ? 4 : 2;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const uint8_t* p) { __builtin_memcpy(w, p, sizeof(w)); }
+    __device__ __forceinline__ void store(uint8_t* p) const { __builtin_memcpy(p, w, sizeof(w)); }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = lo[e];
-                x[4 + e] = hi[e];
-            }
-        } else {
-            x[0] = f[0];
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (DT == AWQ_SERVE_FP32) x[e] = __builtin_bit_cast(float, w[e]);
+            else if constexpr (DT == AWQ_SERVE_BF16) x[e] = __builtin_bit_cast(float, e % 2 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
+            else x[e] = (float)as_h2(w[e / 2])[e % 2];
         }
-    } else {
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + at;
-        if constexpr (VEC == 8)
-            load8<DT == AWQ_SERVE_BF16>(h, x);
-        else if constexpr (DT == AWQ_SERVE_BF16)
-            x[0] = __builtin_bit_cast(float, (uint32_t)h[0] << 16);
-        else
-            x[0] = (float)__builtin_bit_cast(half_t, h[0]);
     }
+    __device__ __forceinline__ void set(const float (&x)[8]) {   // values that the type holds
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (DT == AWQ_SERVE_FP32) w[i] = __builtin_bit_cast(uint32_t, x[i]);
+            else if constexpr (DT == AWQ_SERVE_BF16)
+                w[i] = __builtin_bit_cast(uint32_t, x[2 * i]) >> 16 | (__builtin_bit_cast(uint32_t, x[2 * i + 1]) & 0xFFFF0000u);
+            else w[i] = as_u32(half2_t{(half_t)x[2 * i], (half_t)x[2 * i + 1]});
+        }
+    }
+};
+template <int DT>
+__device__ __forceinline__ float load_one(const uint8_t* p) {
+    if constexpr (DT == AWQ_SERVE_FP32) return *reinterpret_cast<const float*>(p);
+    const uint16_t h = *reinterpret_cast<const uint16_t*>(p);
+    if constexpr (DT == AWQ_SERVE_BF16) return __builtin_bit_cast(float, (uint32_t)h << 16);
+    return (float)__builtin_bit_cast(half_t, h);
 }
-template <int DT, int VEC>
-__device__ __forceinline__ void store_logits(void* p, int64_t at, float (&x)[VEC]) {
-    if constexpr (DT == AWQ_SERVE_FP32) {
-        float* f = reinterpret_cast<float*>(p) + at;
-#pragma unroll
-        for (int e = 0; e < VEC; e += 4) {
-            if constexpr (VEC == 8) *reinterpret_cast<floatx4*>(f + e) = floatx4{x[e], x[e + 1], x[e + 2], x[e + 3]};
-            else f[0] = x[0];
-        }
-    } else {
-        constexpr bool BF16 = DT == AWQ_SERVE_BF16;
-        uint16_t* h = reinterpret_cast<uint16_t*>(p) + at;
-        uint16_t r[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            r[e] = to16<BF16>(x[e]);
-            if constexpr (BF16) x[e] = __builtin_bit_cast(float, (uint32_t)r[e] << 16);
-            else x[e] = (float)__builtin_bit_cast(half_t, r[e]);
-        }
-        if constexpr (VEC == 8) {
-            u32x4 w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = (uint32_t)r[2 * e] | ((uint32_t)r[2 * e + 1] << 16);
-            *reinterpret_cast<u32x4*>(h) = w;
-        } else {
-            h[0] = r[0];
-        }
-    }
+template <int DT>
+__device__ __forceinline__ void store_one(uint8_t* p, float x) {
+    if constexpr (DT == AWQ_SERVE_FP32) *reinterpret_cast<float*>(p) = x;
+    else *reinterpret_cast<uint16_t*>(p) = to16<DT == AWQ_SERVE_BF16>(x);
+}
+// x rounded to the type.
+template <int DT>
+__device__ __forceinline__ float rounded(float x) {
+    if constexpr (DT == AWQ_SERVE_FP32) return x;
+    const uint16_t h = to16<DT == AWQ_SERVE_BF16>(x);
+    if constexpr (DT == AWQ_SERVE_BF16) return __builtin_bit_cast(float, (uint32_t)h << 16);
+    return (float)__builtin_bit_cast(half_t, h);
 }
 
 // One workgroup: the stretch blockIdx.x of CH logits of row blockIdx.y.
-template <int DT, int VEC, int CH>
+template <int DT, int CH>
 __global__ __launch_bounds__(kThreads) void awq_logits_kernel(LogitsArgs a) {
-    __shared__ __align__(16) uint32_t seen[CH];     // the history's tokens
+    constexpr int kPieces = (CH / 8 + kThreads - 1) / kThreads;   // of a thread
+    constexpr int kBytes = Piece<DT>::kBytes;
+    __shared__ __align__(16) uint32_t word[CH];     // counts of the history's tokens, then the new logits
     __shared__ __align__(16) uint32_t entry[CH];    // 1 + the last bias entry, 0: none
+    __shared__ uint32_t touched[CH / 32];           // bit of each token with a new logit
+    __shared__ uint16_t list[CH];                   // those tokens
+    __shared__ int listed;
     __shared__ uint64_t best[kWaves];
     const int row = blockIdx.y, tid = threadIdx.x;
     const int v0 = blockIdx.x * CH;
     const int n = a.vocab - v0 < CH ? a.vocab - v0 : CH;
-    const bool history = a.tokens != nullptr, biases = a.bias_start != nullptr;
-    if (history || biases) {
-        for (int i = 4 * tid; i < CH; i += 4 * kThreads) {
-            *reinterpret_cast<u32x4*>(&seen[i]) = u32x4{0, 0, 0, 0};
-            *reinterpret_cast<u32x4*>(&entry[i]) = u32x4{0, 0, 0, 0};
-        }
-        __syncthreads();
-    }
-    if (history) {
-        const int64_t len = a.lengths[row] < a.width ? a.lengths[row] : a.width;
-        const int64_t prompt = a.prompt_lens[row];
-        auto count = [&](int64_t i, int64_t token) {
-            const uint64_t at = (uint64_t)(token - v0);
-            if (at >= (uint64_t)n) return;
-            if (i < prompt) atomicOr(&seen[at], kInPrompt);
-            else atomicAdd(&seen[at], 1u);
-        };
-        auto scan = [&](auto* text) {
-            text += (int64_t)row * a.width;
-            int64_t i = tid;
-            for (; i + 7 * kThreads < len; i += 8 * kThreads) {   // eight loads in flight
-                int64_t t[8];
+    const uint8_t* in = reinterpret_cast<const uint8_t*>(a.logits) + ((int64_t)row * a.ld + v0) * kBytes;
+    uint8_t* out = reinterpret_cast<uint8_t*>(a.out) + ((int64_t)row * a.vocab + v0) * kBytes;
+    Piece<DT> x[kPieces];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) t[u] = text[i + u * kThreads];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) count(i + u * kThreads, t[u]);
-            }
-            for (; i < len; i += kThreads) count(i, text[i]);
-        };
-        if (a.token_bytes == 8) scan(reinterpret_cast<const int64_t*>(a.tokens));
-        else scan(reinterpret_cast<const int32_t*>(a.tokens));
+    for (int j = 0; j < kPieces; ++j) {
+        const int at = 8 * (j * kThreads + tid);
+        if (at + 8 <= n) x[j].load(in + (int64_t)at * kBytes);
     }
-    if (biases) {
-        int lo = a.bias_start[row], hi = a.bias_start[row + 1];
-        lo = lo < 0 ? 0 : lo;
-        hi = hi < a.bias_count ? hi : a.bias_count;
-        for (int i = lo + tid; i < hi; i += kThreads) {
-            const uint32_t at = (uint32_t)(a.bias_tokens[i] - v0);
-            if (at < (uint32_t)n) atomicMax(&entry[at], (uint32_t)i + 1u);
-        }
-    }
-    if (history || biases) __syncthreads();
+    const uint32_t* mask = a.mask ? a.mask + (int64_t)row * ((a.vocab + 31) / 32) + v0 / 32 : nullptr;
 
+    // Everything that hangs on nothing else is loaded at once: a workgroup is a
+    // chain of latencies, the row's numbers, its history, the listed logits.
+    const bool history = a.tokens != nullptr, biases = a.bias_start != nullptr;
+    int64_t len = history ? a.lengths[row] : 0;
+    const int64_t prompt = history ? a.prompt_lens[row] : 0;
+    int bias_lo = biases ? a.bias_start[row] : 0, bias_hi = biases ? a.bias_start[row + 1] : 0;
     const float rep = history && a.repetition ? a.repetition[row] : 1.0f;
     const float pres = history && a.presence ? a.presence[row] : 0.0f;
     const float freq = history && a.frequency ? a.frequency[row] : 0.0f;
-    const uint32_t* mask = a.mask ? a.mask + (int64_t)row * ((a.vocab + 31) / 32) + v0 / 32 : nullptr;
-    uint64_t top = 0;
-    for (int i = VEC * tid; i < n; i += VEC * kThreads) {
-        float x[VEC];
-        load_logits<DT, VEC>(a.logits, (int64_t)row * a.ld + v0 + i, x);
-        uint32_t allowed = 0xFFu;
-        if (mask) allowed = mask[i / 32] >> (i % 32);
+    len = len < a.width ? len : a.width;
+    bias_lo = bias_lo < 0 ? 0 : bias_lo;
+    bias_hi = bias_hi < a.bias_count ? bias_hi : a.bias_count;
+    constexpr int kFlight = 8;                      // tokens of a thread in flight
+    int64_t t[kFlight];
+    const bool wide_ids = a.token_bytes == 8;
+    auto fetch = [&](int64_t i0) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            if (history) {
-                const uint32_t s = seen[i + e];
-                if (s) x[e] = x[e] > 0.0f ? x[e] / rep : x[e] * rep;
-                const uint32_t times = s & ~kInPrompt;
-                if (times) {
-                    x[e] = x[e] - freq * (float)times;
-                    x[e] = x[e] - pres;
-                }
-            }
-            if (biases) {
-                const uint32_t b = entry[i + e];
-                if (b) x[e] = x[e] + a.bias_values[b - 1];
-            }
-            if (!((allowed >> e) & 1u)) x[e] = -INFINITY;
+        for (int u = 0; u < kFlight; ++u) {
+            const int64_t i = i0 + u * kThreads, at = (int64_t)row * a.width + i;
+            t[u] = i >= len ? -1 : wide_ids ? reinterpret_cast<const int64_t*>(a.tokens)[at]
+                                            : (int64_t)reinterpret_cast<const int32_t*>(a.tokens)[at];
         }
-        store_logits<DT, VEC>(a.out, (int64_t)row * a.vocab + v0 + i, x);
+    };
+    if (len > 0) fetch(tid);
+    const int first_bias = bias_lo + tid < bias_hi ? a.bias_tokens[bias_lo + tid] : -1;
+
+    for (int i = 4 * tid; i < CH; i += 4 * kThreads) {
+        *reinterpret_cast<u32x4*>(&word[i]) = u32x4{0, 0, 0, 0};
+        *reinterpret_cast<u32x4*>(&entry[i]) = u32x4{0, 0, 0, 0};
+    }
+    for (int i = tid; i < CH / 32; i += kThreads) touched[i] = 0;
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    for (int64_t i0 = tid; i0 < len; i0 += kFlight * kThreads) {
+        if (i0 != tid) fetch(i0);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const uint64_t key = ((uint64_t)order_of(x[e]) << 32) | (0xFFFFFFFFu - (uint32_t)(v0 + i + e));
-            top = key > top ? key : top;
+        for (int u = 0; u < kFlight; ++u) {
+            const uint64_t at = (uint64_t)(t[u] - v0);
+            if (at >= (uint64_t)n) continue;
+            const uint32_t before = i0 + u * kThreads < prompt ? atomicOr(&word[at], kInPrompt) : atomicAdd(&word[at], 1u);
+            if (before == 0) list[atomicAdd(&listed, 1)] = (uint16_t)at;
         }
     }
-    top = wave_max64(top);
-    if ((tid & 63) == 0) best[tid >> 6] = top;
+    __syncthreads();
+    if (bias_lo < bias_hi) {
+        for (int i = bias_lo + tid; i < bias_hi; i += kThreads) {
+            const uint32_t at = (uint32_t)((i == bias_lo + tid ? first_bias : a.bias_tokens[i]) - v0);
+            if (at >= (uint32_t)n) continue;
+            if (atomicMax(&entry[at], (uint32_t)i + 1u) == 0 && word[at] == 0) list[atomicAdd(&listed, 1)] = (uint16_t)at;
+        }
+        __syncthreads();
+    }
+
+    for (int i = tid; i < listed; i += kThreads) {
+        const int at = list[i];
+        const uint32_t s = word[at], b = entry[at], times = s & ~kInPrompt;
+        float y = load_one<DT>(in + (int64_t)at * kBytes);
+        if (s) y = y > 0.0f ? y / rep : y * rep;
+        if (times) {
+            y = y - freq * (float)times;
+            y = y - pres;
+        }
+        if (b) y = y + a.bias_values[b - 1];
+        word[at] = __builtin_bit_cast(uint32_t, rounded<DT>(y));
+        atomicOr(&touched[at / 32], 1u << (at % 32));
+    }
+    // In place the pieces below overwrite what is read above (and only that).
+    __syncthreads();
+
+    float top = -INFINITY;
+    uint64_t top_key = 0;
+    auto see = [&](float v, int at) {               // by key: ties, zeros and NaN in order
+        const uint64_t key = ((uint64_t)order_of(v) << 32) | (0xFFFFFFFFu - (uint32_t)(v0 + at));
+        top_key = key > top_key ? key : top_key;
+    };
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+        const int at = 8 * (j * kThreads + tid);
+        if (at >= n) continue;
+        const uint32_t changed = touched[at / 32] >> (at % 32) & 0xFFu;
+        const uint32_t allowed = mask ? mask[at / 32] >> (at % 32) : 0xFFu;
+        if (at + 8 > n) {                           // the vocabulary's last piece, one by one
+            for (int e = 0; at + e < n; ++e) {
+                float y = changed >> e & 1 ? __builtin_bit_cast(float, word[at + e]) : load_one<DT>(in + (int64_t)(at + e) * kBytes);
+                if (!(allowed >> e & 1)) y = -INFINITY;
+                store_one<DT>(out + (int64_t)(at + e) * kBytes, y);
+                see(y, at + e);
+            }
+            continue;
+        }
+        float y[8];
+        x[j].get(y);
+        if (changed) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (changed >> e & 1) y[e] = __builtin_bit_cast(float, word[at + e]);
+        }
+        float most = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            y[e] = allowed >> e & 1 ? y[e] : -INFINITY;
+            most = fmaxf(most, y[e]);
+            sum += y[e];
+        }
+        x[j].set(y);
+        x[j].store(out + (int64_t)at * kBytes);
+        // Few pieces raise the thread's maximum; a NaN, which it passes over, shows in the sum.
+        if (most > top || !(sum == sum) || top_key == 0) {
+            top = fmaxf(top, most);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) see(y[e], at + e);
+        }
+    }
+    top_key = wave_max64(top_key);
+    if ((tid & 63) == 0) best[tid >> 6] = top_key;
     __syncthreads();
     if (tid == 0) {
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = best[w] > top ? best[w] : top;
-        a.keys[(int64_t)row * gridDim.x + blockIdx.x] = top;
+        for (int w = 1; w < kWaves; ++w) top_key = best[w] > top_key ? best[w] : top_key;
+        a.keys[(int64_t)row * gridDim.x + blockIdx.x] = top_key;
     }
 }
 
@@ -203,18 +248,10 @@ __global__ __launch_bounds__(64) void awq_greedy_kernel(const uint64_t* __restri
         next[blockIdx.x] = (uint32_t)(top >> 32) == kMinusInf ? -1 : (int64_t)(0xFFFFFFFFu - (uint32_t)top);
 }
 
-constexpr int kShort = 2048, kLong = 8192;
+constexpr int kShort = 1024, kLong = 4096;
 
 // Short stretches where long ones would leave CUs without work.
 int stretch_of(int rows, int vocab) { return (int64_t)rows * ((vocab + kLong - 1) / kLong) >= 512 ? kLong : kShort; }
-
-template <int DT, int VEC>
-void launch(const LogitsArgs& a, hipStream_t stream) {
-    const int ch = stretch_of(a.rows, a.vocab);
-    const dim3 grid((a.vocab + ch - 1) / ch, a.rows);
-    if (ch == kLong) hipLaunchKernelGGL((awq_logits_kernel<DT, VEC, kLong>), grid, dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL((awq_logits_kernel<DT, VEC, kShort>), grid, dim3(kThreads), 0, stream, a);
-}
 
 }  // namespace
 
@@ -224,22 +261,18 @@ size_t logits_workspace(int rows, int vocab) {
 }
 
 hipError_t launch_logits(const LogitsArgs& a, hipStream_t stream) {
-    // Eight logits a thread where every row starts on 16 bytes and ends on a whole piece.
-    const int bytes = a.dtype == AWQ_SERVE_FP32 ? 4 : 2;
-    const bool wide = a.vocab % 8 == 0 && (a.ld * bytes) % 16 == 0 &&
-                      ((reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0;
+    const int ch = stretch_of(a.rows, a.vocab), stretches = (a.vocab + ch - 1) / ch;
     using std::integral_constant;
     auto typed = [&](auto dt) {
-        if (wide) launch<dt(), 8>(a, stream);
-        else launch<dt(), 1>(a, stream);
+        auto kernel = ch == kLong ? awq_logits_kernel<dt(), kLong> : awq_logits_kernel<dt(), kShort>;
+        hipLaunchKernelGGL(kernel, dim3(stretches, a.rows), dim3(kThreads), 0, stream, a);
+        return hipGetLastError();
     };
-    if (a.dtype == AWQ_SERVE_FP16) typed(integral_constant<int, AWQ_SERVE_FP16>{});
-    else if (a.dtype == AWQ_SERVE_BF16) typed(integral_constant<int, AWQ_SERVE_BF16>{});
-    else typed(integral_constant<int, AWQ_SERVE_FP32>{});
-    hipError_t e = hipGetLastError();
+    const hipError_t e = a.dtype == AWQ_SERVE_FP16   ? typed(integral_constant<int, AWQ_SERVE_FP16>{})
+                         : a.dtype == AWQ_SERVE_BF16 ? typed(integral_constant<int, AWQ_SERVE_BF16>{})
+                                                     : typed(integral_constant<int, AWQ_SERVE_FP32>{});
     if (e != hipSuccess) return e;
-    const int ch = stretch_of(a.rows, a.vocab);
-    hipLaunchKernelGGL(awq_greedy_kernel, dim3(a.rows), dim3(64), 0, stream, a.keys, a.next, (a.vocab + ch - 1) / ch);
+    hipLaunchKernelGGL(awq_greedy_kernel, dim3(a.rows), dim3(64), 0, stream, a.keys, a.next, stretches);
     return hipGetLastError();
 }
 

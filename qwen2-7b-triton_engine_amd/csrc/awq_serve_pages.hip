@@ -10,8 +10,8 @@
 //
 // What bounds it: latency -- a few kilobytes pass.  One launch, no atomics and
 // nothing between workgroups: each has the two prefix sums of all requests to
-// itself (16 requests a thread at most) and keeps them in LDS, then places
-// kThreads rows by binary search.  The torch form is some forty launches.
+// itself (16 requests a thread at most) and keeps them in LDS, then places one row
+// a thread by binary search.  The torch form is some forty launches.
 #include "awq_serving.h"
 
 namespace awq {
@@ -20,14 +20,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMax = AWQ_SERVE_MAX_REQUESTS;
-constexpr int kRowsPerThread = 4;   // rows a thread places: a workgroup's sums serve 1024 rows
 
 __device__ __forceinline__ int64_t pages_of(int64_t tokens, int page_log2) {
     return (tokens + (1 << page_log2) - 1) >> page_log2;
 }
 
 __global__ __launch_bounds__(kThreads) void awq_page_step_kernel(PageStepArgs a) {
-    __shared__ int64_t sums[kWaves];
+    __shared__ int sums[kWaves];
     __shared__ int start[kMax + 1];    // first row, at most a.total
     __shared__ int taken[kMax];        // pages taken before it; -1: refused
     __shared__ int all_taken;
@@ -42,11 +41,14 @@ __global__ __launch_bounds__(kThreads) void awq_page_step_kernel(PageStepArgs a)
         const int b = b0 + tid;
         const int64_t len = b < B ? a.state[b] : 0;
         const int64_t add = b < B ? a.tokens[b] : 0;
-        int64_t all, add_rows = add < 0 ? 0 : add;
+        int64_t all;
+        // What passes `total` or the free pages is refused however much it is: one more stands for it.
+        const int add_rows = add < 0 ? 0 : add <= a.total ? (int)add : a.total + 1;
         const int64_t end = rows + block_scan<kWaves>(add_rows, sums, all);
         rows += all;
         const bool fits = add >= 0 && len >= 0 && end <= a.total && len + add <= room;
-        const int64_t need = fits ? pages_of(len + add, a.page_log2) - pages_of(len, a.page_log2) : 0;
+        const int64_t pages = fits ? pages_of(len + add, a.page_log2) - pages_of(len, a.page_log2) : 0;
+        const int need = (int)(pages <= count ? pages : count + 1);
         const int64_t upto = used + block_scan<kWaves>(need, sums, all);
         used += all;
         const bool served = fits && (need == 0 || upto <= count);
@@ -72,44 +74,40 @@ __global__ __launch_bounds__(kThreads) void awq_page_step_kernel(PageStepArgs a)
         a.new_state[B] = (int)(count - all_taken);
     }
 
-    const int64_t row0 = (int64_t)blockIdx.x * (kThreads * kRowsPerThread);
-#pragma unroll
-    for (int j = 0; j < kRowsPerThread; ++j) {
-        const int64_t row = row0 + j * kThreads + tid;
-        if (row >= a.total) break;
-        int slot = -1, pos = -1;
-        if (row < rows_in) {
-            int lo = 0, hi = B;        // start[lo] <= row < start[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (start[mid] <= row) lo = mid;
-                else hi = mid;
-            }
-            const int before = taken[lo];
-            if (before >= 0) {
-                const int len = a.state[lo];
-                pos = len + (int)(row - start[lo]);
-                const int index = pos >> a.page_log2, held = (int)pages_of(len, a.page_log2);
-                const int offset = pos & ((1 << a.page_log2) - 1);
-                int32_t* entry = a.tables + (int64_t)lo * a.width + index;
-                int page;
-                if (index >= held) {   // one of the step's: its first token writes the table
-                    page = a.free_pages[count - 1 - (before + index - held)];
-                    if (offset == 0) *entry = page;
-                } else {
-                    page = *entry;
-                }
-                slot = page >= 0 && page < (1 << (31 - a.page_log2)) ? (page << a.page_log2) + offset : -1;
-            }
+    const int64_t row = (int64_t)blockIdx.x * kThreads + tid;
+    if (row >= a.total) return;
+    int slot = -1, pos = -1;
+    if (row < rows_in) {
+        int lo = 0, hi = B;            // start[lo] <= row < start[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= row) lo = mid;
+            else hi = mid;
         }
-        a.slots[row] = slot;
-        a.positions[row] = pos;
+        const int before = taken[lo];
+        if (before >= 0) {
+            const int len = a.state[lo];
+            pos = len + (int)(row - start[lo]);
+            const int index = pos >> a.page_log2, held = (int)pages_of(len, a.page_log2);
+            const int offset = pos & ((1 << a.page_log2) - 1);
+            int32_t* entry = a.tables + (int64_t)lo * a.width + index;
+            int page;
+            if (index >= held) {       // one of the step's: its first token writes the table
+                page = a.free_pages[count - 1 - (before + index - held)];
+                if (offset == 0) *entry = page;
+            } else {
+                page = *entry;
+            }
+            slot = page >= 0 && page < (1 << (31 - a.page_log2)) ? (page << a.page_log2) + offset : -1;
+        }
     }
+    a.slots[row] = slot;
+    a.positions[row] = pos;
 }
 
 // One workgroup per request: the sums again, then its own pages.
 __global__ __launch_bounds__(kThreads) void awq_page_release_kernel(PageStepArgs a) {
-    __shared__ int64_t sums[kWaves];
+    __shared__ int sums[kWaves];
     __shared__ int64_t mine[2];        // this request's pages: first place, number
     const int B = a.requests, tid = threadIdx.x, me = blockIdx.x;
     const int count_in = a.state[B];
@@ -122,7 +120,8 @@ __global__ __launch_bounds__(kThreads) void awq_page_release_kernel(PageStepArgs
         len = len < 0 ? 0 : len < room ? len : room;
         int64_t keep = b < B ? a.tokens[b] : 0;
         keep = keep < 0 ? 0 : keep < len ? keep : len;
-        const int64_t give = pages_of(len, a.page_log2) - pages_of(keep, a.page_log2);
+        const int64_t all_give = pages_of(len, a.page_log2) - pages_of(keep, a.page_log2);
+        const int give = (int)(all_give <= a.capacity ? all_give : a.capacity);   // no request holds more
         int64_t all;
         const int64_t upto = before + block_scan<kWaves>(give, sums, all);
         before += all;
@@ -145,8 +144,7 @@ __global__ __launch_bounds__(kThreads) void awq_page_release_kernel(PageStepArgs
 }  // namespace
 
 hipError_t launch_page_step(const PageStepArgs& a, hipStream_t stream) {
-    const int each = kThreads * kRowsPerThread;
-    const int grid = a.total > 0 ? (a.total + each - 1) / each : 1;
+    const int grid = a.total > 0 ? (a.total + kThreads - 1) / kThreads : 1;
     hipLaunchKernelGGL(awq_page_step_kernel, dim3(grid), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }

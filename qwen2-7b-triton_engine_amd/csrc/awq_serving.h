@@ -130,14 +130,25 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
     }
     return v;
 }
-// The same over a workgroup of WAVES waves: inclusive sum, and the whole in `all`.
-// lds: WAVES values, free for use before the call and after it.
+// The same of 32-bit values by DPP steps, without the LDS pipe.
+__device__ __forceinline__ int wave_scan32(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);    // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2 and 3
+    return v;
+}
+// The same over a workgroup of WAVES waves, and the whole in `all`.  Values of at
+// most 2^24 + 1: a wave's sum fits 32 bits, the waves' are added in 64.
+// lds: free for use before the call and after it.
 template <int WAVES>
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int64_t& all) {
+__device__ __forceinline__ int64_t block_scan(int v, int (&lds)[WAVES], int64_t& all) {
     const int wave = threadIdx.x >> 6;
-    v = wave_scan(v);
+    const int upto = wave_scan32(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 63) lds[wave] = v;
+    if ((threadIdx.x & 63) == 63) lds[wave] = upto;
     __syncthreads();
     all = 0;
     int64_t before = 0;
@@ -146,7 +157,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int64_t& 
         if (w < wave) before += lds[w];
         all += lds[w];
     }
-    return v + before;
+    return before + upto;
 }
 
 }  // namespace awq

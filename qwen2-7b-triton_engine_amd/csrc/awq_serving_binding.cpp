@@ -55,6 +55,37 @@ struct Cache {
     int64_t heads() const { return data.size(1); }
 };
 
+// Tables as kernels/paged.py holds them.
+void check_tables(const Tensor& block_tables, const Tensor& state, const Tensor& free_pages, int64_t page_size) {
+    TORCH_CHECK_VALUE(block_tables.dim() == 2 && free_pages.dim() == 1, "block_tables must be 2-D and free_pages 1-D");
+    const int64_t requests = block_tables.size(0), width = block_tables.size(1), capacity = free_pages.size(0);
+    const at::Device device = block_tables.device();
+    check_i32(block_tables, "block_tables", {requests, width}, device);
+    check_i32(state, "state", {requests + 1}, device);
+    check_i32(free_pages, "free_pages", {capacity}, device);
+    TORCH_CHECK_VALUE(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128 || page_size == 256, "page_size ",
+                      page_size, " must be 16, 32, 64, 128 or 256");
+    TORCH_CHECK_VALUE(requests > 0 && requests <= AWQ_SERVE_MAX_REQUESTS && width > 0 && capacity > 0, requests, " requests of ",
+                      width, " pages, ", capacity, " pages in all: need 1 to ", AWQ_SERVE_MAX_REQUESTS,
+                      " requests and at least one page");
+    TORCH_CHECK_VALUE(width <= (1 << 30) / page_size && capacity <= (1 << 24), "a request's tokens pass 2^30, or the free pages 2^24");
+}
+// A cache as kernels/kv4.py holds it.
+void check_cache(const Tensor& data, int64_t head_dim, int64_t page_size, int64_t group_size) {
+    TORCH_CHECK_VALUE(head_dim == 64 || head_dim == 128, "head_dim ", head_dim, " must be 64 or 128");
+    TORCH_CHECK_VALUE(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128 || page_size == 256, "page_size ",
+                      page_size, " must be 16, 32, 64, 128 or 256");
+    TORCH_CHECK_VALUE((group_size == 32 || group_size == 64 || group_size == 128) && group_size <= head_dim, "group_size ", group_size,
+                      " must be 32, 64 or 128 and at most head_dim ", head_dim);
+    const int64_t block = page_size * (head_dim + 8 * (head_dim / group_size));
+    TORCH_CHECK_VALUE(data.scalar_type() == at::kByte && data.dim() == 3 && data.size(2) == block && data.is_contiguous(),
+                      "data must be a contiguous uint8 tensor [pages, kv heads, ", block, "], got ", data.scalar_type(), " ",
+                      data.sizes());
+    TORCH_CHECK_VALUE(data.size(0) >= 1 && data.size(1) >= 1 && (reinterpret_cast<uintptr_t>(data.data_ptr()) & 15u) == 0,
+                      "data must hold a page and a head and start on 16 bytes");
+    TORCH_CHECK_VALUE(data.size(0) <= kIntMax / page_size, "slot numbers pass 32 bits");
+}
+
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_step(const Tensor& state, const Tensor& new_tokens,
                                                               const Tensor& block_tables, const Tensor& free_pages,
                                                               int64_t page_size, int64_t total,
@@ -63,7 +94,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_step(const Tensor& stat
     check_on_gpu(state, "the tables");
     const int64_t requests = block_tables.size(0), width = block_tables.size(1);
     check_i32(new_tokens, "new_tokens", {requests}, device);
-    TORCH_CHECK_VALUE(total >= 0 && total <= kIntMax / 2, "total ", total, " must be in [0, ", kIntMax / 2, "]");
+    TORCH_CHECK_VALUE(total >= 0 && total <= (1 << 24), "total ", total, " must be in [0, 2^24]");
     Tensor o[5];
     const int64_t sizes[5] = {requests + 1, requests + 1, total, total, requests};
     if (out.has_value()) {
@@ -72,8 +103,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_step(const Tensor& stat
         TORCH_CHECK_VALUE(o[0].data_ptr() != state.data_ptr(),
                           "out.state is the tables' own state: the step reads it while it writes");
     } else {
-        const Tensor flat = at::empty({3 * requests + 2 + 2 * total}, state.options());   // one allocation
-        for (int64_t i = 0, at = 0; i < 5; at += sizes[i++]) o[i] = flat.narrow(0, at, sizes[i]);
+        // one allocation, one call for its parts
+        const std::vector<Tensor> parts =
+            at::empty({3 * requests + 2 + 2 * total}, state.options()).unsafe_split_with_sizes(sizes, 0);
+        for (int i = 0; i < 5; ++i) o[i] = parts[i];
     }
     const at::DeviceGuard guard(device);
     check_status(awq_serve_page_step(i32(state), i32(new_tokens), block_tables.data_ptr<int32_t>(), i32(free_pages),
@@ -285,6 +318,8 @@ std::tuple<Tensor, Tensor> process_logits(const Tensor& logits_in, const OptTens
 }  // namespace
 
 void define_serving(py::module_& m) {
+    m.def("check_tables", &check_tables);
+    m.def("check_cache", &check_cache);
     m.def("paged_step", &paged_step);
     m.def("paged_release", &paged_release);
     m.def("kv4_append", &kv4_append);

@@ -18,11 +18,11 @@ import torch
 
 from . import _native
 
-__all__ = ["Kv4Cache", "kv4_append", "kv4_gather", "kv4_attention", "GROUP_SIZES", "HEAD_DIMS"]
+__all__ = ["Kv4Cache", "kv4_append", "kv4_gather", "kv4_attention", "GROUP_SIZES", "HEAD_DIMS", "PAGE_SIZES"]
 
 GROUP_SIZES = (32, 64, 128)
 HEAD_DIMS = (64, 128)
-_PAGE_SIZES = (16, 32, 64, 128, 256)
+PAGE_SIZES = (16, 32, 64, 128, 256)
 
 
 class Kv4Cache:
@@ -32,7 +32,8 @@ class Kv4Cache:
 
     def __init__(self, num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 64, group_size: int = 64,
                  device: torch.device | str = "cuda:0"):
-        self._check(head_dim, page_size, group_size)
+        if group_size not in GROUP_SIZES:
+            raise ValueError(f"group_size {group_size} must be one of {GROUP_SIZES}")
         data = torch.zeros((num_pages, num_kv_heads, self.block_bytes(head_dim, page_size, group_size)),
                            dtype=torch.uint8, device=device)
         self._set(data, head_dim, page_size, group_size)
@@ -40,29 +41,12 @@ class Kv4Cache:
     @classmethod
     def of(cls, data: torch.Tensor, head_dim: int, page_size: int = 64, group_size: int = 64) -> "Kv4Cache":
         """A cache over a tensor that exists (a layer's part of a larger one, say)."""
-        cls._check(head_dim, page_size, group_size)
         cache = cls.__new__(cls)
         cache._set(data, head_dim, page_size, group_size)
         return cache
 
-    @staticmethod
-    def _check(head_dim, page_size, group_size):
-        if head_dim not in HEAD_DIMS:
-            raise ValueError(f"head_dim {head_dim} must be one of {HEAD_DIMS}")
-        if page_size not in _PAGE_SIZES:
-            raise ValueError(f"page_size {page_size} must be one of {_PAGE_SIZES}")
-        if group_size not in GROUP_SIZES or group_size > head_dim:
-            raise ValueError(f"group_size {group_size} must be one of {GROUP_SIZES} and at most head_dim {head_dim}")
-
     def _set(self, data, head_dim, page_size, group_size):
-        block = self.block_bytes(head_dim, page_size, group_size)
-        if data.dtype is not torch.uint8 or data.dim() != 3 or data.shape[2] != block or not data.is_contiguous():
-            raise ValueError(f"data must be a contiguous uint8 tensor [pages, kv heads, {block}], got {data.dtype} "
-                             f"{tuple(data.shape)}")
-        if data.shape[0] < 1 or data.shape[1] < 1 or data.data_ptr() % 16 != 0:
-            raise ValueError("data must hold a page and a head and start on 16 bytes")
-        if data.shape[0] > (2**31 - 1) // page_size:
-            raise ValueError("slot numbers pass 32 bits")
+        _native.binding().check_cache(data, head_dim, page_size, group_size)
         self.data, self.head_dim, self.page_size, self.group_size = data, head_dim, page_size, group_size
 
     @staticmethod

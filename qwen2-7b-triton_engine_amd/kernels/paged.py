@@ -23,13 +23,6 @@ __all__ = ["PagedTables", "PagedStep", "paged_step", "paged_release", "MAX_REQUE
 
 MAX_REQUESTS = _native.SERVE_MAX_REQUESTS
 PAGE_SIZES = (16, 32, 64, 128, 256)
-_INT_MAX = 2**31 - 1
-
-
-def _check_i32(t: torch.Tensor, what: str, shape: tuple, dev: torch.device) -> None:
-    if t.dtype is not torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev:
-        raise ValueError(f"{what} must be a contiguous int32 tensor {shape} on {dev}, got {t.dtype} {tuple(t.shape)} "
-                         f"on {t.device}")
 
 
 @dataclasses.dataclass
@@ -62,20 +55,7 @@ class PagedTables:
         return t
 
     def _set(self, block_tables, state, free_pages, page_size):
-        if block_tables.dim() != 2 or free_pages.dim() != 1:
-            raise ValueError("block_tables must be 2-D and free_pages 1-D")
-        requests, width = block_tables.shape
-        dev = block_tables.device
-        _check_i32(block_tables, "block_tables", (requests, width), dev)
-        _check_i32(state, "state", (requests + 1,), dev)
-        _check_i32(free_pages, "free_pages", (free_pages.shape[0],), dev)
-        if page_size not in PAGE_SIZES:
-            raise ValueError(f"page_size {page_size} must be one of {PAGE_SIZES}")
-        if not 0 < requests <= MAX_REQUESTS or width < 1 or free_pages.shape[0] < 1:
-            raise ValueError(f"{requests} requests of {width} pages, {free_pages.shape[0]} pages in all: need 1 to "
-                             f"{MAX_REQUESTS} requests and at least one page")
-        if width > 2**30 // page_size or free_pages.shape[0] > _INT_MAX // page_size:
-            raise ValueError("token numbers pass 32 bits")
+        _native.binding().check_tables(block_tables, state, free_pages, page_size)
         self.block_tables, self.state, self.free_pages, self.page_size = block_tables, state, free_pages, page_size
 
     @property
