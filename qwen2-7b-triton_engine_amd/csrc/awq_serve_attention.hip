@@ -23,7 +23,7 @@ constexpr int kCols = 16;              // (row, query head) pairs of a decode wo
 constexpr int kWaveKeys = 32;          // tokens of one inner pass of a decode wave
 constexpr int kKeys = kWaveKeys * kWaves;
 constexpr int kTileKeys = 64;          // tokens of a tile kernel's step
-constexpr int kTileThreads = 256, kTileCols = kTileThreads / 4;   // 16 columns a wave
+constexpr int kTileCols = 16 * kWaves;   // columns of a tile workgroup, 16 a wave
 
 constexpr int kPExp = 14;              // the probabilities' scale before they are split: 2^14
 constexpr int kQExp = 8;               // q's largest value lies in 2^7 .. 2^8: a group's sum stays below 2^15
@@ -211,42 +211,60 @@ struct PairsOf {
 };
 
 // A column's query as the B operand of the k-steps: lane (column, t) holds
-// columns 32 s + 8 t + e of the head; the sums of the groups in three parts, lane
-// t those of group t.  Returns the exponent of the row's power of two.
+// columns 32 s + 8 t + e of the head, times the power of two that brings the row's
+// largest value to 2^7 .. 2^8 (2^15 times at most, which is exact for whatever is
+// smaller).  The groups' sums come from the matrix cores too, as products with rows
+// of ones, and enter in three fp16 parts (33 bits), lane t those of group t.
+// Returns the exponent of the row's power of two.
 template <int HD, int GN, bool BF16>
-__device__ __forceinline__ int load_query(const uint16_t* src, int t, half8_t (&q)[HD / 32], half8_t& qz) {
+__device__ __forceinline__ int load_query(const uint16_t* src, int col, int t, half8_t (&q)[HD / 32], half8_t& qz) {
     constexpr int kSteps = HD / 32, G = HD / GN;
-    float x[kSteps][8], mx = 0.0f;
+    int exp;
+    if constexpr (BF16) {
+        float x[kSteps][8], mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            load8<true>(src + 32 * s + 8 * t, x[s]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[s][e]));
+        }
+        exp = kQExp - __builtin_amdgcn_frexp_expf(column_max(mx));
+        exp = exp < 100 ? exp : 100;
+        const float up = __builtin_ldexpf(1.0f, exp);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[s][e] = (half_t)(x[s][e] * up);
+    } else {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) q[s] = *reinterpret_cast<const half8_t*>(src + 32 * s + 8 * t);
+        half2_t mx = {};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                mx = __builtin_elementwise_max(mx, as_h2(as_u32(half2_t{q[s][e], q[s][e + 1]}) & 0x7FFF7FFFu));
+        exp = kQExp - __builtin_amdgcn_frexp_expf(column_max(fmaxf((float)mx.x, (float)mx.y)));
+        exp = exp < 15 ? exp : 15;
+        const half_t up = (half_t)__builtin_ldexpf(1.0f, exp);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) q[s] *= up;
+    }
+    floatx4 sums = {0.f, 0.f, 0.f, 0.f};   // row g: group g
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-        load8<BF16>(src + 32 * s + 8 * t, x[s]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[s][e]));
+        const half_t one = (half_t)(col == 32 * s / G ? 1.0f : 0.0f);
+        sums = mfma16x16x32(half8_t{one, one, one, one, one, one, one, one}, q[s], sums);
     }
-    mx = column_max(mx);
-    int exp = kQExp - __builtin_amdgcn_frexp_expf(mx);
-    exp = exp < 100 ? exp : 100;
-    const float up = __builtin_ldexpf(1.0f, exp);
-    float sum[GN];
-#pragma unroll
-    for (int i = 0; i < GN; ++i) sum[i] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            q[s][e] = (half_t)(x[s][e] * up);
-            sum[32 * s / G] += (float)q[s][e];
-        }
     float mine = 0.0f;
 #pragma unroll
     for (int i = 0; i < GN; ++i) {
-        sum[i] += __shfl_xor(sum[i], 16);
-        sum[i] += __shfl_xor(sum[i], 32);
-        if (t == i) mine = sum[i];
+        const float sum = __shfl(sums[i], col);
+        if (t == i) mine = sum;
     }
     qz = half8_t{};
 #pragma unroll
-    for (int e = 0; e < 3; ++e) {          // 33 bits
+    for (int e = 0; e < 3; ++e) {
         qz[e] = (half_t)mine;
         mine -= (float)qz[e];
     }
@@ -257,6 +275,12 @@ __device__ __forceinline__ int load_query(const uint16_t* src, int t, half8_t (&
 __device__ __forceinline__ int page_at(const Kv4AttnArgs& a, const int32_t* table, int key, int n) {
     const int index = key >> a.s.page_log2;
     return key < n && index < a.width ? table[index] : -1;
+}
+
+// The same where key is the same for the whole wave: the number in a scalar register, and what
+// is addressed by it from there.
+__device__ __forceinline__ int wave_page_at(const Kv4AttnArgs& a, const int32_t* table, int key, int n) {
+    return __builtin_amdgcn_readfirstlane(page_at(a, table, __builtin_amdgcn_readfirstlane(key), n));
 }
 
 // ---- few columns: decode ---------------------------------------------------------------
@@ -351,13 +375,13 @@ __global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs
     const int32_t* table = a.tables + (int64_t)it.b * a.width;
     int key0 = start + kWaveKeys * wave;
     Place now[2];
-    now[0] = place(page_at(a, table, key0, n), key0);
-    now[1] = place(page_at(a, table, key0 + 16, n), key0 + 16);
+    now[0] = place(wave_page_at(a, table, key0, n), key0);
+    now[1] = place(wave_page_at(a, table, key0 + 16, n), key0 + 16);
     if (key0 < end) {
         load_k(now);
         load_v(now);
     }
-    int page0 = page_at(a, table, key0 + kKeys, n), page1 = page_at(a, table, key0 + kKeys + 16, n);
+    int page0 = wave_page_at(a, table, key0 + kKeys, n), page1 = wave_page_at(a, table, key0 + kKeys + 16, n);
 
     // This lane's column: row c / group of the request, head c % group.
     const int c = c0 + (col < cols ? col : 0);
@@ -367,7 +391,7 @@ __global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs
     const int lim_min = __builtin_amdgcn_readlane(lim, 0);            // rows grow along the columns
     half8_t q[kSteps], qz;
     const int exp = load_query<HD, GN, BF16>(
-        reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + row) * a.ld + (int64_t)head * HD, t, q, qz);
+        reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + row) * a.ld + (int64_t)head * HD, col, t, q, qz);
     // exp(scale x) = exp2(x factor); the scores here are 2^exp times as large.
     // Every exponent is a difference of scores first: what they were rounded to
     // on the way must be the same wherever two meet.
@@ -385,8 +409,8 @@ __global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs
         Place next[2];
         next[0] = place(page0, key0 + kKeys);
         next[1] = place(page1, key0 + kKeys + 16);
-        page0 = page_at(a, table, key0 + 2 * kKeys, n);
-        page1 = page_at(a, table, key0 + 2 * kKeys + 16, n);
+        page0 = wave_page_at(a, table, key0 + 2 * kKeys, n);
+        page1 = wave_page_at(a, table, key0 + 2 * kKeys + 16, n);
 
         if (!now[0].there || !now[1].there) {   // a page outside the cache: NaN for the queries that see it
 #pragma unroll
@@ -565,12 +589,10 @@ __device__ __forceinline__ int v_chunk(int row, int chunk) { return chunk ^ ((ro
 // ONE_PAGE: pages of 64 tokens and more, where a tile lies in one of them and its
 // address is the workgroup's, not a lane's.
 template <int HD, int GN, bool ONE_PAGE, bool BF16>
-__global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel(Kv4AttnArgs a) {
     constexpr int kSteps = HD / 32, kDb = HD / 16, kChunks = HD / 8, G = HD / GN;
     constexpr int kRows = HD + 16;                       // of the transposed V: columns, zeros, ones
     constexpr int kK = kTileKeys * HD, kV = kRows * kTileKeys, kZ = kTileKeys * 4;   // halfs
-    constexpr int kParts = kTileThreads / kThreads;      // threads that share 16 bytes of codes: 1 or 2
-    constexpr int kWords = kSteps / kParts;              // words of K a thread brings
     __shared__ __align__(16) half_t buf[kK + kV + kZ];
 
     Item it;
@@ -598,7 +620,7 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
     const int32_t* table = a.tables + (int64_t)it.b * a.width;
 
     // Rows of the zeros' block that no tile writes: ones at 4, else zero; zeros of no group.
-    for (int i = tid; i < 16 * kTileKeys + kZ; i += kTileThreads) {
+    for (int i = tid; i < 16 * kTileKeys + kZ; i += kThreads) {
         const int r = i / kTileKeys;
         if (i < 16 * kTileKeys) {
             if (r >= GN) buf[kK + HD * kTileKeys + i] = (half_t)(r == 4 ? 1.0f : 0.0f);
@@ -607,12 +629,12 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
         }
     }
 
-    // What this thread brings of a tile: of K kWords words (columns 32 s + 8 k_t .., s from
-    // k_s) of token k_tok; of V four tokens' eight columns, or half of them.
-    const int k_tok = tid / (4 * kParts), k_t = tid / kParts % 4, k_s = tid % kParts * kWords;
-    const int v_tb = tid / kParts / kChunks, v_j = tid / kParts % kChunks, v_part = tid % kParts, v_g = 8 * v_j / G;
-    const bool has_v = v_tb < kTileKeys / 4;             // (heads of 64: half of the threads)
-    typedef uint32_t words_t __attribute__((ext_vector_type(kWords > 1 ? kWords : 2)));
+    // What this thread brings of a tile: of K the words of token k_tok and lane group
+    // k_t; of V eight columns of four tokens (heads of 64: half of the threads).
+    const int k_tok = tid >> 2, k_t = tid & 3;
+    const int v_tb = tid / kChunks, v_j = tid % kChunks, v_g = 8 * v_j / G;
+    const bool has_v = v_tb < kTileKeys / 4;
+    typedef uint32_t words_t __attribute__((ext_vector_type(kSteps)));
     words_t kw;
     typename PairsOf<GN>::type ks;
     u32x4 vw;
@@ -622,7 +644,7 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
     };
     auto pages = [&](int key) {
         if constexpr (ONE_PAGE) {
-            const int p = page_at(a, table, key, n);
+            const int p = wave_page_at(a, table, key, n);
             return Pages{p, p};
         } else {
             return Pages{page_at(a, table, key + k_tok, n), page_at(a, table, key + 4 * v_tb, n)};
@@ -630,7 +652,7 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
     };
     auto there = [&](int page) { return page >= 0 && page < a.s.num_pages; };
     auto block_of = [&](int page) { return a.cache + ((int64_t)(there(page) ? page : 0) * a.s.kvh + g) * a.s.block(); };
-    const uint32_t k_ofs = k_t * (HD / 8) + 4 * k_s, v_ofs = a.s.k_bytes() + v_j * 16;
+    const uint32_t k_ofs = k_t * (HD / 8), v_ofs = a.s.k_bytes() + v_j * 16;
     const uint32_t ks_ofs = 2 * a.s.k_bytes(), vs_ofs = 2 * a.s.k_bytes() + a.s.scale_bytes() + v_g * 16;
     auto load = [&](int key, Pages p) {
         // The token of the page that the tile or the thread begins with, and the thread's after it.
@@ -640,8 +662,7 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
         const uint32_t k_in = ONE_PAGE ? k_tok : (key + k_tok) & (a.s.page() - 1);
         const uint32_t v_in = ONE_PAGE ? v_tb : ((key + 4 * v_tb) & (a.s.page() - 1)) >> 2;
         const uint8_t* kp = kb + in * (HD / 2);
-        if constexpr (kWords > 1) kw = *reinterpret_cast<const words_t*>(kp + k_in * (HD / 2) + k_ofs);
-        else kw.x = *reinterpret_cast<const uint32_t*>(kp + k_in * (HD / 2) + k_ofs);
+        kw = *reinterpret_cast<const words_t*>(kp + k_in * (HD / 2) + k_ofs);
         ks = *reinterpret_cast<const typename PairsOf<GN>::type*>(kb + in * (4 * GN) + k_in * (4 * GN) + ks_ofs);
         if (has_v) {
             vw = *reinterpret_cast<const u32x4*>(vb + in * (HD / 2) + v_in * (kChunks * 16) + v_ofs);
@@ -659,25 +680,19 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
             for (int i = 0; i < 2 * GN; ++i) ks[i] = (half_t)NAN;
         }
 #pragma unroll
-        for (int j = 0; j < kWords; ++j) {
-            half_t sc;                                   // of the group of step k_s + j
-            if constexpr (kParts == 1) {
-                sc = ks[2 * (32 * j / G)];
-            } else {
-                const int of0 = 32 * j / G, of1 = 32 * (kWords + j) / G;
-                sc = of0 == of1 ? ks[2 * of0] : k_s ? ks[2 * of1] : ks[2 * of0];
-            }
+        for (int j = 0; j < kSteps; ++j) {
+            const half_t sc = ks[2 * (32 * j / G)];
             const half2_t s2 = {sc, sc};
             half2_t o[4];
             scaled_codes(kw[j], base, s2, times_minus16(s2), o);
-            *reinterpret_cast<half8_t*>(lk + k_tok * HD + 8 * k_chunk<kChunks>(k_tok, 4 * (k_s + j) + k_t)) =
+            *reinterpret_cast<half8_t*>(lk + k_tok * HD + 8 * k_chunk<kChunks>(k_tok, 4 * j + k_t)) =
                 half8_t{o[0].x, o[0].y, o[1].x, o[1].y, o[2].x, o[2].y, o[3].x, o[3].y};
         }
         half_t zk = ks[1];
 #pragma unroll
         for (int i = 1; i < GN; ++i)
             if (k_t == i) zk = ks[2 * i + 1];
-        if (k_t < GN && k_s == 0) lz[k_tok * 4 + k_t] = zk;
+        if (k_t < GN) lz[k_tok * 4 + k_t] = zk;
         if (has_v) {
             if (!there(p.v) || key + kTileKeys > n) {    // tokens past the length may hold anything
 #pragma unroll
@@ -687,8 +702,7 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
             const half2_t s01 = {vs[0], vs[1]}, s23 = {vs[2], vs[3]};
             const half2_t m01 = times_minus16(s01), m23 = times_minus16(s23);
 #pragma unroll
-            for (int j = 0; j < 2 / kParts; ++j) {
-                const int part = kParts == 1 ? j : v_part;
+            for (int part = 0; part < 2; ++part) {
                 const uint32_t half = part ? 0x07060302u : 0x05040100u;
                 half2_t p01[4], p23[4];
                 scaled_codes(__builtin_amdgcn_perm(vw[1], vw[0], half), base, s01, m01, p01);
@@ -700,7 +714,7 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
                         half4_t{p01[u].x, p01[u].y, p23[u].x, p23[u].y};
                 }
             }
-            if (8 * v_j % G == 0 && v_part == 0) {
+            if (8 * v_j % G == 0) {
                 const int d = HD + v_g;
                 *reinterpret_cast<half4_t*>(lv + d * kTileKeys + 8 * v_chunk(d, v_place) + v_sub) = vz;
             }
@@ -718,7 +732,7 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
     const int local = 16 * wave + col, c = c0 + local, cc = c < all_cols ? c : all_cols - 1;
     const int lim = limit_of(cc);
     const int exp = load_query<HD, GN, BF16>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + cc / group) * a.ld +
-                                                 (int64_t)(g * group + cc % group) * HD, t, q, qz);
+                                                 (int64_t)(g * group + cc % group) * HD, col, t, q, qz);
     const float factor = a.scale * 1.4426950408889634f, unit = __builtin_ldexpf(factor, -exp);
     const int lim_min = __builtin_amdgcn_readlane(lim, 0), lim_max = __builtin_amdgcn_readlane(lim, 15);
 
@@ -728,9 +742,7 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
     for (int d = 0; d <= kDb; ++d) acc[d] = floatx4{0.f, 0.f, 0.f, 0.f};
     // Operand addresses: the swizzles only flip bits that the rows' starts leave free.
     const uint32_t k_at = col * HD + 8 * k_chunk<kChunks>(col, t);
-    uint32_t v_at[4];
-#pragma unroll
-    for (int d = 0; d < 4; ++d) v_at[d] = kK + (16 * d + col) * kTileKeys + 8 * v_chunk(16 * d + col, t);
+    const uint32_t v_at = kK + col * kTileKeys + 8 * v_chunk(col, t);   // row 16 d + col flips by 2 d
     for (int tile = 0; tile < tiles; ++tile) {
         const int key0 = start + tile * kTileKeys;
         if (tile) lds_barrier();                         // every wave has read the tile before
@@ -781,7 +793,7 @@ __global__ __launch_bounds__(kTileThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_ke
             split16(p, kPExp, phi, plo);
 #pragma unroll
             for (int d = 0; d <= kDb; ++d) {
-                const half8_t v = *reinterpret_cast<const half8_t*>(buf + (v_at[d & 3] ^ (32 * h)) + (d & ~3) * 16 * kTileKeys);
+                const half8_t v = *reinterpret_cast<const half8_t*>(buf + (v_at ^ (32 * h) ^ (16 * (d & 3))) + 16 * d * kTileKeys);
                 acc[d] = mfma16x16x32(v, plo, acc[d]);
                 acc[d] = mfma16x16x32(v, phi, acc[d]);
             }
@@ -927,8 +939,8 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a
 
 // ---- launches ----------------------------------------------------------------------------
 
-constexpr int kDecodeItems = 512;     // items that a launch aims at, all kv heads together
-constexpr int kTileItems = 512;
+constexpr int kDecodeItems = 768;     // items that a launch aims at, all kv heads together
+constexpr int kTileItems = 1024;
 constexpr int kDecodeColumns = 64;     // a request of more columns goes to the tile kernel
 constexpr int kCombineGroups = 8192;   // workgroups of the combining launch at most
 
@@ -979,7 +991,7 @@ hipError_t launch(Kv4AttnArgs a, hipStream_t stream) {
     }
     if (p.tile) {
         auto kernel = a.s.page() >= kTileKeys ? awq_kv4_tile_kernel<HD, GN, true, BF16> : awq_kv4_tile_kernel<HD, GN, false, BF16>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)p.tile_items, a.s.kvh), dim3(kTileThreads), 0, stream, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)p.tile_items, a.s.kvh), dim3(kThreads), 0, stream, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
