@@ -86,9 +86,11 @@ __device__ __forceinline__ bool find_item(const Kv4AttnArgs& a, int want, int ta
     sizes<COLS, KEYS>(a, r, blocks, steps);
     if (target) {
         int64_t work = (int64_t)blocks * steps;
+        int all_blocks = blocks;
         for (int b0 = 64; b0 < a.requests; b0 += 64) {
             sizes<COLS, KEYS>(a, request(a, b0 + lane), blocks, steps);
             work += (int64_t)blocks * steps;
+            all_blocks += blocks;
         }
         // Sums below 2^24 a lane, as good as always, are added in 32 bits.
         int64_t all;
@@ -100,6 +102,10 @@ __device__ __forceinline__ bool find_item(const Kv4AttnArgs& a, int want, int ta
         } else {
             all = __shfl(wave_scan(work), 63);
         }
+        // Each block ends in a shorter item, half of one too many on average: with as many
+        // fewer to begin with, the items are one round of workgroups.
+        const int extra = a.requests == 1 ? 0 : __builtin_amdgcn_readlane(wave_scan32(all_blocks), 63) / 2;
+        target = extra < target - target / 4 ? target - extra : (target + 3) / 4;
         const int64_t most = (int64_t)target * kMost;
         const uint32_t few = all < 0x7FFFFFFF - target ? (uint32_t)(all + target - 1) / (uint32_t)target : 0;
         m = few ? (few < (uint32_t)kMost ? (int)few : kMost)
