@@ -6,6 +6,7 @@
 #include "awq_binding.h"
 
 #include <ATen/DeviceGuard.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -47,6 +48,9 @@ Tensor rows16(const Tensor& t) {
     return aligned16(t.contiguous());
 }
 int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// None of these is differentiable: their allocations and views go straight to the backend.
+using Plain = at::AutoDispatchBelowADInplaceOrView;
 
 struct Cache {
     const Tensor& data;
@@ -90,6 +94,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_step(const Tensor& stat
                                                               const Tensor& block_tables, const Tensor& free_pages,
                                                               int64_t page_size, int64_t total,
                                                               const c10::optional<std::vector<Tensor>>& out) {
+    const Plain plain;
     const at::Device device = state.device();
     check_on_gpu(state, "the tables");
     const int64_t requests = block_tables.size(0), width = block_tables.size(1);
@@ -135,6 +140,7 @@ Tensor paged_release(const Tensor& state, const Tensor& keep, const Tensor& bloc
 Tensor kv4_append(const Tensor& qkv_in, const Tensor& data, int64_t head_dim, int64_t page_size, int64_t group_size,
                   const Tensor& slots, const Tensor& positions, const OptTensor& cos_in, const OptTensor& sin_in,
                   int64_t num_heads) {
+    const Plain plain;
     const Cache cache{data, head_dim, page_size, group_size};
     const at::Device device = qkv_in.device();
     const int64_t columns = (num_heads + 2 * cache.heads()) * head_dim;
@@ -171,6 +177,7 @@ Tensor kv4_append(const Tensor& qkv_in, const Tensor& data, int64_t head_dim, in
 
 std::tuple<Tensor, Tensor> kv4_gather(const Tensor& data, int64_t head_dim, int64_t page_size, int64_t group_size,
                                       const Tensor& slots, at::ScalarType dtype) {
+    const Plain plain;
     const Cache cache{data, head_dim, page_size, group_size};
     TORCH_CHECK_VALUE(dtype == at::kHalf || dtype == at::kBFloat16, "dtype must be float16 or bfloat16, got ", dtype);
     check_on_gpu(data, "the cache");
@@ -178,8 +185,7 @@ std::tuple<Tensor, Tensor> kv4_gather(const Tensor& data, int64_t head_dim, int6
     const int64_t T = slots.size(0);
     check_i32(slots, "slots", {T}, data.device());
     const at::DeviceGuard guard(data.device());
-    const Tensor kv = at::empty({2, T, cache.heads(), head_dim}, data.options().dtype(dtype));
-    Tensor k = kv.select(0, 0), v = kv.select(0, 1);
+    Tensor k = at::empty({T, cache.heads(), head_dim}, data.options().dtype(dtype)), v = at::empty_like(k);
     check_status(awq_serve_kv4_gather(data.data_ptr(), i32(slots), k.data_ptr(), v.data_ptr(), T, cache.heads(), head_dim,
                                       cache.pages(), page_size, group_size,
                                       dtype == at::kHalf ? AWQ_SERVE_FP16 : AWQ_SERVE_BF16, stream_of(data.device())),
@@ -190,6 +196,7 @@ std::tuple<Tensor, Tensor> kv4_gather(const Tensor& data, int64_t head_dim, int6
 Tensor kv4_attention(const Tensor& q_in, const Tensor& data, int64_t head_dim, int64_t page_size, int64_t group_size,
                      const Tensor& block_tables, const Tensor& seq_lens, const Tensor& query_start, int64_t max_query,
                      c10::optional<double> scale_in) {
+    const Plain plain;
     const Cache cache{data, head_dim, page_size, group_size};
     const at::Device device = q_in.device();
     const int64_t kvh = cache.heads();
@@ -235,6 +242,7 @@ std::tuple<Tensor, Tensor> process_logits(const Tensor& logits_in, const OptTens
                                           const OptTensor& presence, const OptTensor& frequency,
                                           const c10::optional<std::tuple<Tensor, Tensor, Tensor>>& bias,
                                           const OptTensor& mask, const OptTensor& out_in) {
+    const Plain plain;
     const at::ScalarType type = logits_in.scalar_type();
     TORCH_CHECK_VALUE((type == at::kHalf || type == at::kBFloat16 || type == at::kFloat) && logits_in.dim() == 2 &&
                           logits_in.size(1) > 0,
