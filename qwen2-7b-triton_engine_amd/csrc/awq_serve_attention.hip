@@ -277,17 +277,25 @@ __device__ __forceinline__ int load_query(const uint16_t* src, int col, int t, h
     return exp;
 }
 
-// A page's number in a request's table: -1 past the length or the table.
-__device__ __forceinline__ int page_at(const Kv4AttnArgs& a, const int32_t* table, int key, int n) {
-    const int index = key >> a.s.page_log2;
-    return key < n && index < a.width ? table[index] : -1;
-}
-
-// The same where key is the same for the whole wave: the number in a scalar register, and what
-// is addressed by it from there.
-__device__ __forceinline__ int wave_page_at(const Kv4AttnArgs& a, const int32_t* table, int key, int n) {
-    return __builtin_amdgcn_readfirstlane(page_at(a, table, __builtin_amdgcn_readfirstlane(key), n));
-}
+// A request's pages from the one that holds `key` on: lane i has the i-th of 64, -1 past
+// the length or the table.  One load for 64 pages: a page's number then costs a lane
+// read and no wait for memory (a load of it would be waited for behind the codes'
+// loads that were issued before it).
+struct Pages64 {
+    const int32_t* table;
+    int first, entry;
+    __device__ __forceinline__ void fetch(const Kv4AttnArgs& a, int key, int n) {
+        first = key >> a.s.page_log2;
+        const int index = first + (int)(threadIdx.x & 63);
+        entry = index < a.width && ((int64_t)index << a.s.page_log2) < n ? table[index] : -1;
+    }
+    // Of a key that is the same for the whole wave.
+    __device__ __forceinline__ int page(const Kv4AttnArgs& a, int key, int n) {
+        const int index = key >> a.s.page_log2;
+        if ((uint32_t)(index - first) >= 64u) fetch(a, key, n);
+        return __builtin_amdgcn_readlane(entry, index - first);
+    }
+};
 
 // ---- few columns: decode ---------------------------------------------------------------
 
@@ -378,16 +386,16 @@ __global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs
         }
     };
 
-    const int32_t* table = a.tables + (int64_t)it.b * a.width;
     int key0 = start + kWaveKeys * wave;
+    Pages64 pages = {a.tables + (int64_t)it.b * a.width, 0, 0};
+    pages.fetch(a, key0, n);
     Place now[2];
-    now[0] = place(wave_page_at(a, table, key0, n), key0);
-    now[1] = place(wave_page_at(a, table, key0 + 16, n), key0 + 16);
+    now[0] = place(pages.page(a, key0, n), key0);
+    now[1] = place(pages.page(a, key0 + 16, n), key0 + 16);
     if (key0 < end) {
         load_k(now);
         load_v(now);
     }
-    int page0 = wave_page_at(a, table, key0 + kKeys, n), page1 = wave_page_at(a, table, key0 + kKeys + 16, n);
 
     // This lane's column: row c / group of the request, head c % group.
     const int c = c0 + (col < cols ? col : 0);
@@ -413,10 +421,9 @@ __global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs
     while (key0 < end) {
         const bool more = key0 + kKeys < end;
         Place next[2];
-        next[0] = place(page0, key0 + kKeys);
-        next[1] = place(page1, key0 + kKeys + 16);
-        page0 = wave_page_at(a, table, key0 + 2 * kKeys, n);
-        page1 = wave_page_at(a, table, key0 + 2 * kKeys + 16, n);
+        const int key1 = more ? key0 + kKeys : key0;
+        next[0] = place(pages.page(a, key1, n), key1);
+        next[1] = place(pages.page(a, key1 + 16, n), key1 + 16);
 
         if (!now[0].there || !now[1].there) {   // a page outside the cache: NaN for the queries that see it
 #pragma unroll
@@ -623,7 +630,8 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
     const int start = split * it.chunk, lim_wg = limit_of(c_last);
     const int end = lim_wg < start + it.chunk ? lim_wg : start + it.chunk;
     const int tiles = end > start ? (end - start + kTileKeys - 1) / kTileKeys : 0;
-    const int32_t* table = a.tables + (int64_t)it.b * a.width;
+    Pages64 window = {a.tables + (int64_t)it.b * a.width, 0, 0};
+    window.fetch(a, start, n);
 
     // Rows of the zeros' block that no tile writes: ones at 4, else zero; zeros of no group.
     for (int i = tid; i < 16 * kTileKeys + kZ; i += kThreads) {
@@ -650,10 +658,12 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
     };
     auto pages = [&](int key) {
         if constexpr (ONE_PAGE) {
-            const int p = wave_page_at(a, table, key, n);
+            const int p = window.page(a, key, n);
             return Pages{p, p};
         } else {
-            return Pages{page_at(a, table, key + k_tok, n), page_at(a, table, key + 4 * v_tb, n)};
+            if (((key + kTileKeys - 1) >> a.s.page_log2) - window.first >= 64) window.fetch(a, key, n);
+            return Pages{__shfl(window.entry, ((key + k_tok) >> a.s.page_log2) - window.first),
+                         has_v ? __shfl(window.entry, ((key + 4 * v_tb) >> a.s.page_log2) - window.first) : -1};
         }
     };
     auto there = [&](int page) { return page >= 0 && page < a.s.num_pages; };
@@ -727,11 +737,10 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
         }
     };
 
-    Pages now = {-1, -1}, next = {-1, -1};               // of the tile in registers, and of the one after it
+    Pages now = {-1, -1};                                // of the tile in registers
     if (tiles > 0) {
         now = pages(start);
         load(start, now);
-        next = pages(start + kTileKeys);
     }
 
     half8_t q[kSteps], qz;
@@ -754,9 +763,8 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
         if (tile) lds_barrier();                         // every wave has read the tile before
         store(key0, now);
         if (tile + 1 < tiles) {                          // the next tile's codes, in flight under this one
-            now = next;
+            now = pages(key0 + kTileKeys);
             load(key0 + kTileKeys, now);
-            next = pages(key0 + 2 * kTileKeys);
         }
         lds_barrier();
         if (key0 >= lim_max) continue;                   // past every column of this wave
