@@ -277,6 +277,20 @@ __device__ __forceinline__ int load_query(const uint16_t* src, int col, int t, h
     return exp;
 }
 
+// Tells the scheduler how to mix READS reads of LDS and MFMAS products: FIRST reads, then
+// one after every EACH products.
+template <int READS, int MFMAS, int EACH, int FIRST>
+__device__ __forceinline__ void ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
+    constexpr int kRest = READS - FIRST;
+#pragma unroll
+    for (int i = 0; i < kRest; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, MFMAS > EACH * kRest ? MFMAS - EACH * kRest : 1, 0);
+}
+
 // A request's pages from the one that holds `key` on: lane i has the i-th of 64, -1 past
 // the length or the table.  One load for 64 pages: a page's number then costs a lane
 // read and no wait for memory (a load of it would be waited for behind the codes'
@@ -782,6 +796,11 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
                 for (int st = 0; st < kSteps; ++st)
                     s[b] = mfma16x16x32(*reinterpret_cast<const half8_t*>(buf + (k_at ^ (32 * st)) + 16 * kb * HD), q[st], s[b]);
             }
+            // Operands are read several products ahead (the scheduler by itself keeps
+            // two in flight, and waits for LDS at every product): first the scores'
+            // alone, then the first half's sums with the second half's scores.
+            if (h == 0) ahead<2 * kSteps + 2, 2 * (kSteps + 1), 1, 5>();
+            else ahead<kDb + 1 + 2 * kSteps + 2, 2 * (kDb + 1) + 2 * (kSteps + 1), 2, 4>();
             if (key0 + 32 * h + 32 > lim_min) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
@@ -811,6 +830,7 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
                 acc[d] = mfma16x16x32(v, plo, acc[d]);
                 acc[d] = mfma16x16x32(v, phi, acc[d]);
             }
+            if (h == 1) ahead<kDb + 1, 2 * (kDb + 1), 2, 4>();
         }
     }
 
