@@ -975,8 +975,9 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a
 
 constexpr int kDecodeItems = 768;     // items that a launch aims at, all kv heads together
 constexpr int kTileItems = 1024;
-constexpr int kDecodeColumns = 64;     // a request of more columns goes to the tile kernel
+constexpr int kDecodeColumns = 128;     // a request of more columns goes to the tile kernel
 constexpr int kCombineGroups = 8192;   // workgroups of the combining launch at most
+constexpr int kFewUnits = 512;
 
 struct Plan {
     bool decode, tile, combine;
@@ -1030,9 +1031,8 @@ hipError_t launch(Kv4AttnArgs a, hipStream_t stream) {
         if (e != hipSuccess) return e;
     }
     if (p.combine) {
-        // Four waves a row and head up to 2048 of them: the items along the tokens are many where rows are few.
-        const int64_t all = (int64_t)a.total * a.nh, groups = all <= 2048 ? all : (all + 3) / 4;
-        auto kernel = all <= 2048 ? awq_kv4_combine_kernel<HD, 4, BF16> : awq_kv4_combine_kernel<HD, 1, BF16>;
+        const int64_t all = (int64_t)a.total * a.nh, groups = all <= kFewUnits ? all : (all + 3) / 4;
+        auto kernel = all <= kFewUnits ? awq_kv4_combine_kernel<HD, 4, BF16> : awq_kv4_combine_kernel<HD, 1, BF16>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < kCombineGroups ? groups : kCombineGroups)), dim3(kThreads), 0, stream, a);
         return hipGetLastError();
     }

@@ -79,6 +79,11 @@ CASES = [
     (2, 2, 128, 16, 32, "fp16", [(70, 65)]),
     (2, 1, 64, 16, 64, "fp16", [(5000, 1), (3, 1)]),             # several items along the tokens
     (4, 1, 64, 64, 32, "fp16", [(2100, 40), (900, 1)]),
+    (2, 2, 128, 64, 32, "fp16", [(200, 150)]),                   # more than 128 columns of a kv head
+    (4, 2, 128, 16, 32, "bf16", [(190, 100), (40, 1), (66, 65)]),
+    (8, 2, 128, 64, 128, "bf16", [(140, 70), (90, 33)]),
+    (64, 1, 64, 64, 32, "fp16", [(70, 3), (65, 1)]),
+    (12, 4, 64, 128, 64, "fp16", [(1500, 90)]),
 ]
 
 
@@ -95,7 +100,7 @@ def test_attention(gpu, nh, kvh, hd, page, group, dtype, requests):
     _close(y, ref, dtype, "attention")
 
 
-@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("rows", [1, 40, 70])
 def test_attention_rows_that_see_nothing_and_rows_of_no_request(gpu, rows):
     """Three tokens under `rows` rows more than that: the first rows stand before the
     first token; a request without tokens; rows past the last request's."""
@@ -112,7 +117,7 @@ def test_attention_rows_that_see_nothing_and_rows_of_no_request(gpu, rows):
     assert (y[rows] != 0).any()
 
 
-@pytest.mark.parametrize("rows", [1, 33])
+@pytest.mark.parametrize("rows", [1, 33, 70])
 def test_attention_reads_nothing_of_what_lies_past_the_length(gpu, rows):
     """Bytes that are NaN scales everywhere but in the request's tokens, and table
     entries outside the cache past its pages."""
@@ -130,7 +135,7 @@ def test_attention_reads_nothing_of_what_lies_past_the_length(gpu, rows):
     _close(y, O.attend(q.double().numpy().reshape(-1, 4, hd), k, v, lengths, starts, table, page), "fp16", "past the length")
 
 
-@pytest.mark.parametrize("rows", [4, 40])
+@pytest.mark.parametrize("rows", [4, 40, 70])
 def test_a_token_that_is_not_finite_reaches_only_the_rows_that_see_it(gpu, rows):
     """k or v with a NaN or an infinity at the next to last position: the rows before it are as without it."""
     rng = np.random.default_rng(5)
