@@ -12,6 +12,14 @@
 // as further columns of V, with a column of ones that gives the softmax's sum).
 // q is scaled by its row's power of two and held in fp16, which is exact for fp16
 // input; the probabilities are fp32 and enter as two fp16 parts, hi and lo.
+// Outputs are as far from the 64-bit result as plain fp32 torch's (2.1e-4 of their
+// norm in fp16, 1.7e-3 in bf16: the output's own rounding).
+//
+// Three launches at most: requests of few columns (decode), requests of many (tiles), and the
+// joining of what was split along the tokens.  28 heads of 128 over 4 kv heads, groups
+// of 64, pages of 64, graph replays, us: one request of 1100 tokens 10.3, 64 of up to
+// 4096 (2150 on average) 34.5, 16 of up to 16000 30.3; prompts of 256, 1024, 1777 and 4096
+// tokens 22, 42, 84 and 278 (433 TFLOP/s of useful work).
 #include "awq_serving.h"
 
 namespace awq {
@@ -31,8 +39,8 @@ constexpr int kQExp = 8;               // q's largest value lies in 2^7 .. 2^8: 
 // ---- which item a workgroup has --------------------------------------------------
 
 // Requests of few columns (rows times the heads that share a kv head) go to the
-// decode kernel in blocks of 16 columns, the others to the tile kernel in
-// blocks of kTileCols.  An item is a block and a stretch of tokens.
+// decode kernel in blocks of 16 columns, the others to the tile kernel in blocks
+// of 64.  An item is a block and a stretch of tokens.
 struct Request {
     int row0, rows, len;               // first row, rows, tokens
 };
@@ -322,6 +330,14 @@ struct Pages64 {
 // products.  K's registers are loaded again as soon as its product is made, V's
 // likewise: each is in flight under the other half of the pass, without a second
 // set of registers.  The waves' results meet once, at the end.
+//
+// What bounds it: at one request latency -- 7.1 us of launch, item, page, codes and
+// the waves' meeting, one after another; at 64 requests of up to 4096 tokens (85 MB
+// of codes and scales, 30 us) the start and end of a workgroup, 9 us, and the vector
+// unit in between: 300 instructions a wave for 32 tokens, a third of them the
+// multiplying out of 8192 codes, against 28 products.  Three waves a SIMD (146 to 163
+// registers; four spilled 44 to 68 bytes).  A second set of K and V registers and a page number loaded
+// in the pass before were 33 to 36 us.
 template <int HD, int GN, bool BF16>
 __global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs a) {
     constexpr int kSteps = HD / 32;
@@ -612,7 +628,16 @@ __device__ __forceinline__ int v_chunk(int row, int chunk) { return chunk ^ ((ro
 // K as it is, V transposed, its zeros and a row of ones as rows of their own -- and
 // every wave reads its operands there.  The codes of the next tile are on their way
 // in registers meanwhile.  One LDS buffer and two barriers a tile: the room goes to
-// a third workgroup on the CU, which has work while the others wait.
+// a third workgroup on the CU, which has work while the others wait (two buffers and two
+// workgroups: 105 us at a prompt of 1777 tokens, then 97).
+//
+// What bounds it: at 4096 tokens the issue of vector instructions beside the
+// products, some 380 a wave and tile -- sixteen scores a lane with their exponentials
+// and two parts, 130 to multiply the codes out -- against 56 products; LDS is
+// busy 40 % of the time.  At 1777 the longest of the 784 workgroups, 28 tiles where the
+// average is 14.5.  128 columns a workgroup, in two column blocks a wave or in eight
+// waves, multiply out half as much and were slower (107 and 116 us against 97 and 105): fewer, coarser
+// workgroups, and no registers to read operands ahead.
 // ONE_PAGE: pages of 64 tokens and more, where a tile lies in one of them and its
 // address is the workgroup's, not a lane's.
 template <int HD, int GN, bool ONE_PAGE, bool BF16>
@@ -873,7 +898,9 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
 // out[row, head] = sum of its items' parts, each weighted by exp2(its maximum -
 // the overall maximum).  WAVES waves have a row and head: each every WAVES-th item,
 // a lane an item's weight and two columns' sums, eight loads in flight; the
-// waves meet in LDS.  All four where rows and heads are few (and items many), else one.
+// waves meet in LDS.  All four where rows and heads are few (and items many), else
+// one: 2 requests of 32768 tokens, 64 rows and heads, 29.0 us with one and 25.6
+// with four; 64 of up to 4096, 1792 rows and heads, 33.8 and 37.5.
 template <int HD, int WAVES, bool BF16>
 __global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a) {
     constexpr int W = HD / 64;                           // columns a lane
@@ -973,11 +1000,20 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a
 
 // ---- launches ----------------------------------------------------------------------------
 
-constexpr int kDecodeItems = 768;     // items that a launch aims at, all kv heads together
-constexpr int kTileItems = 1024;
-constexpr int kDecodeColumns = 128;     // a request of more columns goes to the tile kernel
+// Items that a launch aims at, all kv heads together.  Decode: three workgroups on each
+// of 256 CUs, one round of them.  512 / 768 / 1024: 64 requests of up to 4096 tokens 46.8 /
+// 37.8 / 41.8 us, 16 of up to 16000 38.5 / 30.5 / 35.8, one of 16000 14.7 / 15.7 / 16.2.
+constexpr int kDecodeItems = 768;
+// Tiles, only where the blocks of columns are fewer than CUs: 256 / 512 / 1024 items for
+// 3 chunks of 389 rows behind 4000 tokens 77 / 59 / 51 us.  Prompts with more blocks than that are
+// not split: a prompt of 1024 tokens 46 us whole, 50 to 73 split (partial sums of every row).
+constexpr int kTileItems = 1024, kSplitBelow = 256;
+// A request of more columns goes to the tile kernel.  8 requests behind up to 4000 tokens, all by
+// the decode kernel / by the tile kernel: 56 columns 24.9 / 30.4 us, 112 28.3 / 32.4, 224 42.9 /
+// 41.0, 448 68 / 57.
+constexpr int kDecodeColumns = 128;
 constexpr int kCombineGroups = 8192;   // workgroups of the combining launch at most
-constexpr int kFewUnits = 512;
+constexpr int kFewUnits = 512;         // rows times heads that get four waves each there
 
 struct Plan {
     bool decode, tile, combine;
@@ -1002,7 +1038,7 @@ Plan plan(int requests, int total, int max_query, int group, int kvh) {
     }
     if (p.tile) {
         const int64_t blocks = requests + rows * group / kTileCols;
-        p.tile_target = blocks * kvh < 256 ? (kvh < kTileItems ? kTileItems / kvh : 1) : 0;
+        p.tile_target = blocks * kvh < kSplitBelow ? (kvh < kTileItems ? kTileItems / kvh : 1) : 0;
         p.tile_items = blocks + p.tile_target + 1;
     }
     p.combine = p.decode || p.tile_target;

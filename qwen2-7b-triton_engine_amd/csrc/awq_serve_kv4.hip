@@ -14,7 +14,10 @@
 // a token's head is stored as NaN when either cannot be held.  The arithmetic
 // is unfused fp32 in the order of the formulas (contraction is off): codes are
 // decided at the middle between two values, where one more or less rounding
-// moves a value by a whole step.
+// moves a value by a whole step.  For the same reason the quotients are true
+// divisions, not products with a reciprocal.
+// Measured, 28 query and 4 kv heads of 128, groups of 64, us: append 4.2 for 64 tokens,
+// 12.7 for 2011 (37 MB: 2.9 TB/s), gather 2.9 and 4.0.
 #include "awq_serving.h"
 
 #pragma clang fp contract(off)

@@ -12,6 +12,10 @@
 // as the largest index.  The listed tokens, few among many, get their new
 // logits by one thread each; then the stretch passes through, its logits loaded
 // before the counting began.  The history is read once per stretch, out of the caches.
+// Both launches, us: one row of 152064 logits 7.4, sixty-four with histories of 4096
+// 29.6 (41 MB in and out: 6.6 at the memory's rate), where the workgroups' chains of
+// latencies -- lengths, history, listed logits, store -- take three rounds; LDS holds three on
+// a CU.  With a counter and a bias entry read for every logit 45.
 #include "awq_serving.h"
 
 #pragma clang fp contract(off)   // each step rounds as the same step in torch does

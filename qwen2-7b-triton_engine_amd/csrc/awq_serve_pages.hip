@@ -11,7 +11,9 @@
 // What bounds it: latency -- a few kilobytes pass.  One launch, no atomics and
 // nothing between workgroups: each has the two prefix sums of all requests to
 // itself (16 requests a thread at most) and keeps them in LDS, then places one row
-// a thread by binary search.  The torch form is some forty launches.
+// a thread by binary search.  The torch form is some forty launches.  Measured: 64
+// requests of a token each 3.0 us, 16384 rows of 256 requests 6.1 (9.7 with
+// 64-bit wave sums).
 #include "awq_serving.h"
 
 namespace awq {
