@@ -13,9 +13,12 @@
 // logits by one thread each; then the stretch passes through, its logits loaded
 // before the counting began.  The history is read once per stretch, out of the caches.
 // Both launches, us: one row of 152064 logits 7.4, sixty-four with histories of 4096
-// 29.6 (41 MB in and out: 6.6 at the memory's rate), where the workgroups' chains of
-// latencies -- lengths, history, listed logits, store -- take three rounds; LDS holds three on
-// a CU.  With a counter and a bias entry read for every logit 45.
+// 29.1 (41 MB in and out: 6.6 at the memory's rate): some 500 vector instructions a wave,
+// half of them the history's tokens, and chains of LDS latencies between barriers.  With a
+// counter and a bias entry read for every logit 45.  A fourth workgroup on a CU (4032 logits
+// each) changed nothing; a wave that gathers its tokens of the stretch before it counts them was
+// faster where histories are long (eight rows of 50257 with 16000: 13.5 -> 11.6) and slower for
+// one row (7.0 -> 7.2).
 #include "awq_serving.h"
 
 #pragma clang fp contract(off)   // each step rounds as the same step in torch does
