@@ -20,6 +20,7 @@
 // of 64, pages of 64, graph replays, us: one request of 1100 tokens 10.3, 64 of up to
 // 4096 (2150 on average) 34.5, 16 of up to 16000 30.3; prompts of 256, 1024, 1777 and 4096
 // tokens 22, 42, 84 and 278 (433 TFLOP/s of useful work).
+#include "awq_serve_items.h"
 #include "awq_serving.h"
 
 namespace awq {
@@ -27,11 +28,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kCols = 16;              // (row, query head) pairs of a decode workgroup: the columns of an MFMA
-constexpr int kWaveKeys = 32;          // tokens of one inner pass of a decode wave
-constexpr int kKeys = kWaveKeys * kWaves;
-constexpr int kTileKeys = 64;          // tokens of a tile kernel's step
-constexpr int kTileCols = 16 * kWaves;   // columns of a tile workgroup, 16 a wave
+static_assert(kKeys == kWaveKeys * kWaves && kTileCols == 16 * kWaves, "awq_serve_items.h");
 
 constexpr int kPExp = 14;              // the probabilities' scale before they are split: 2^14
 constexpr int kQExp = 8;               // q's largest value lies in 2^7 .. 2^8: a group's sum stays below 2^15
@@ -48,29 +45,21 @@ __device__ __forceinline__ Request request(const Kv4AttnArgs& a, int b) {
     Request r = {0, 0, 0};
     if (b < a.requests) {
         const int lo = a.query_start[b], hi = a.query_start[b + 1], len = a.seq_lens[b];
-        r.row0 = lo < 0 ? 0 : lo < a.total ? lo : a.total;
-        const int end = hi < r.row0 ? r.row0 : hi < a.total ? hi : a.total;
-        r.rows = end - r.row0;
+        r.row0 = first_row(lo, a.total);
+        r.rows = end_row(r.row0, hi, a.total) - r.row0;
         r.len = len < 0 ? 0 : len;
     }
     return r;
 }
-// Tokens to walk over: one past the table where the length is (that one is not
-// there, and gives NaN).
-__device__ __forceinline__ int walked(const Kv4AttnArgs& a, int len) {
-    const int64_t room = (int64_t)a.width << a.s.page_log2;
-    return len <= room ? len : (int)room + 1;
-}
+__device__ __forceinline__ int walked(const Kv4AttnArgs& a, int len) { return walked_tokens(a.width, a.s.page_log2, len); }
 __device__ __forceinline__ int columns(const Kv4AttnArgs& a, int rows) {
-    return (rows < a.max_query ? rows : a.max_query) * (a.nh / a.s.kvh);
+    return request_columns(rows, a.max_query, a.nh / a.s.kvh);
 }
 // Blocks of COLS columns that a request has in this kernel, and its tokens in steps of KEYS.
 template <int COLS, int KEYS>
 __device__ __forceinline__ void sizes(const Kv4AttnArgs& a, const Request& r, int& blocks, int& steps) {
-    const int c = columns(a, r.rows);
-    const bool mine = (c <= a.limit) == (COLS == kCols);
-    blocks = mine ? (c + COLS - 1) / COLS : 0;
-    steps = (int)(((int64_t)walked(a, r.len) + KEYS - 1) / KEYS);
+    blocks = request_blocks<COLS>(columns(a, r.rows), a.limit);
+    steps = request_steps<KEYS>(walked(a, r.len));
 }
 
 struct Item {
@@ -83,14 +72,12 @@ struct Item {
 // Finds an item by its number.  Every wave walks over the requests' lengths by
 // itself, 64 at a time and without a barrier: no launch has to prepare a list,
 // and the host need not know the lengths.  The tokens of an item are a multiple of
-// KEYS, as few as `target` items in all allow (at most target + the blocks of all
-// requests come out); without a target an item has all of its request's.
+// KEYS (item_steps).
 template <int COLS, int KEYS>
 __device__ __forceinline__ bool find_item(const Kv4AttnArgs& a, int want, int target, Item& it) {
-    constexpr int kMost = (1 << 29) / KEYS;
     const int lane = threadIdx.x & 63;
     Request r = request(a, lane);
-    int blocks, steps, m = kMost;
+    int blocks, steps, m = item_steps<KEYS>(0, 0, 0, a.requests);
     sizes<COLS, KEYS>(a, r, blocks, steps);
     if (target) {
         int64_t work = (int64_t)blocks * steps;
@@ -110,21 +97,15 @@ __device__ __forceinline__ bool find_item(const Kv4AttnArgs& a, int want, int ta
         } else {
             all = __shfl(wave_scan(work), 63);
         }
-        // Each block ends in a shorter item, half of one too many on average: with as many
-        // fewer to begin with, the items are one round of workgroups.
-        const int extra = a.requests == 1 ? 0 : __builtin_amdgcn_readlane(wave_scan32(all_blocks), 63) / 2;
-        target = extra < target - target / 4 ? target - extra : (target + 3) / 4;
-        const int64_t most = (int64_t)target * kMost;
-        const uint32_t few = all < 0x7FFFFFFF - target ? (uint32_t)(all + target - 1) / (uint32_t)target : 0;
-        m = few ? (few < (uint32_t)kMost ? (int)few : kMost)
-                : all == 0 ? 1 : all < most ? (int)((all + target - 1) / target) : kMost;
+        const int blocks_sum = a.requests == 1 ? 0 : __builtin_amdgcn_readlane(wave_scan32(all_blocks), 63);
+        m = item_steps<KEYS>(target, all, blocks_sum, a.requests);
         m = __builtin_amdgcn_readfirstlane(m);
     }
     int before = 0;
     for (int b0 = 0; b0 < a.requests; b0 += 64) {
         if (a.requests > 64) r = request(a, b0 + lane);
         sizes<COLS, KEYS>(a, r, blocks, steps);
-        const int splits = (int)((uint32_t)(steps + m - 1) / (uint32_t)m), mine = blocks * splits;
+        const int splits = request_splits(steps, m), mine = blocks * splits;
         const int upto = before + wave_scan32(mine);
         const uint64_t hit = __ballot(want >= upto - mine && want < upto);
         if (hit) {
@@ -366,7 +347,7 @@ __global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs
     const int64_t last_pos = (int64_t)it.r.len - it.r.rows + (c0 + cols - 1) / group;
     const int lim_max = last_pos < 0 ? 0 : last_pos + 1 < n ? (int)(last_pos + 1) : n;
     const int start = split * it.chunk;
-    const int end = lim_max < start + it.chunk ? lim_max : start + it.chunk;
+    const int end = item_end(start, it.chunk, lim_max);
 
     // What this lane reads of 16 tokens, from where they begin in the codes and in the scales.
     const int j8 = HD == 128 ? col : col >> 1;
@@ -667,7 +648,7 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
     };
     const int c_last = c0 + kTileCols < all_cols ? c0 + kTileCols - 1 : all_cols - 1;
     const int start = split * it.chunk, lim_wg = limit_of(c_last);
-    const int end = lim_wg < start + it.chunk ? lim_wg : start + it.chunk;
+    const int end = item_end(start, it.chunk, lim_wg);
     const int tiles = end > start ? (end - start + kTileKeys - 1) / kTileKeys : 0;
     Pages64 window = {a.tables + (int64_t)it.b * a.width, 0, 0};
     window.fetch(a, start, n);
@@ -1000,54 +981,16 @@ __global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a
 
 // ---- launches ----------------------------------------------------------------------------
 
-// Items that a launch aims at, all kv heads together.  Decode: three workgroups on each
-// of 256 CUs, one round of them.  512 / 768 / 1024: 64 requests of up to 4096 tokens 46.8 /
-// 37.8 / 41.8 us, 16 of up to 16000 38.5 / 30.5 / 35.8, one of 16000 14.7 / 15.7 / 16.2.
-constexpr int kDecodeItems = 768;
-// Tiles, only where the blocks of columns are fewer than CUs: 256 / 512 / 1024 items for
-// 3 chunks of 389 rows behind 4000 tokens 77 / 59 / 51 us.  Prompts with more blocks than that are
-// not split: a prompt of 1024 tokens 46 us whole, 50 to 73 split (partial sums of every row).
-constexpr int kTileItems = 1024, kSplitBelow = 256;
-// A request of more columns goes to the tile kernel.  8 requests behind up to 4000 tokens, all by
-// the decode kernel / by the tile kernel: 56 columns 24.9 / 30.4 us, 112 28.3 / 32.4, 224 42.9 /
-// 41.0, 448 68 / 57.
-constexpr int kDecodeColumns = 128;
 constexpr int kCombineGroups = 8192;   // workgroups of the combining launch at most
 constexpr int kFewUnits = 512;         // rows times heads that get four waves each there
 
-struct Plan {
-    bool decode, tile, combine;
-    int limit, decode_target, tile_target;
-    int64_t decode_items, tile_items;  // at most, of one kv head
-    size_t bytes(int total, int kvh, int hd) const {     // row records, then parts
-        return (size_t)total * sizeof(i32x4) +
-               (size_t)(decode_items * kCols + (tile_target ? tile_items * kTileCols : 0)) * kvh * (hd + 2) * sizeof(float);
-    }
-};
-Plan plan(int requests, int total, int max_query, int group, int kvh) {
-    Plan p = {};
-    const int64_t rows = (int64_t)requests * max_query < total ? (int64_t)requests * max_query : total;
-    p.tile = (int64_t)max_query * group > kDecodeColumns;
-    p.decode = !p.tile || requests > 1;
-    p.limit = p.decode ? kDecodeColumns : 0;             // of one request the tile kernel has whatever it is
-    if (p.decode) {
-        p.decode_target = kvh < kDecodeItems ? kDecodeItems / kvh : 1;
-        const int64_t most = (int64_t)requests * ((kDecodeColumns + kCols - 1) / kCols);
-        const int64_t blocks = requests + rows * group / kCols;
-        p.decode_items = p.decode_target + (p.tile && most < blocks ? most : blocks) + 1;
-    }
-    if (p.tile) {
-        const int64_t blocks = requests + rows * group / kTileCols;
-        p.tile_target = blocks * kvh < kSplitBelow ? (kvh < kTileItems ? kTileItems / kvh : 1) : 0;
-        p.tile_items = blocks + p.tile_target + 1;
-    }
-    p.combine = p.decode || p.tile_target;
-    return p;
+size_t part_bytes(const AttentionPlan& p, int total, int kvh, int hd) {   // row records, then the items' sums
+    return (size_t)total * sizeof(i32x4) + p.part_floats(kvh, hd) * sizeof(float);
 }
 
 template <int HD, int GN, bool BF16>
 hipError_t launch(Kv4AttnArgs a, hipStream_t stream) {
-    const Plan p = plan(a.requests, a.total, a.max_query, a.nh / a.s.kvh, a.s.kvh);
+    const AttentionPlan p = attention_plan(a.requests, a.total, a.max_query, a.nh / a.s.kvh, a.s.kvh);
     a.limit = p.limit;
     a.decode_target = p.decode_target;
     a.tile_target = p.tile_target;
@@ -1078,7 +1021,7 @@ hipError_t launch(Kv4AttnArgs a, hipStream_t stream) {
 }  // namespace
 
 size_t kv4_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd) {
-    return plan(requests, total, max_query, nh / kvh, kvh).bytes(total, kvh, hd);
+    return part_bytes(attention_plan(requests, total, max_query, nh / kvh, kvh), total, kvh, hd);
 }
 
 hipError_t launch_kv4_attention(const Kv4AttnArgs& a, bool bf16, hipStream_t stream) {
