@@ -124,7 +124,8 @@ int awq_serve_kv4_gather(const void* cache, const int32_t* slots, void* k, void*
  * (q_stride elements from row to row) and seq_lens[b] tokens in the cache, the
  * rows' own among them: row i of n stands at position seq_lens[b] - n + i and
  * sees the tokens 0 .. position.  A row that sees none (a negative position) and a
- * row of no request give zeros.  out [total, num_heads * head_dim] in q's type.
+ * row of no request give zeros.  No row is two requests': an entry of query_start below an
+ * earlier one counts as that one.  out [total, num_heads * head_dim] in q's type.
  * A request of more than table_width * page_size tokens gives NaN.
  * max_query: at least the largest number of rows of a request (it sizes the grid and the
  * workspace; rows past it are not computed).

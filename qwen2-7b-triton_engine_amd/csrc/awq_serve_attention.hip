@@ -41,14 +41,18 @@ constexpr int kQExp = 8;               // q's largest value lies in 2^7 .. 2^8: 
 struct Request {
     int row0, rows, len;               // first row, rows, tokens
 };
-__device__ __forceinline__ Request request(const Kv4AttnArgs& a, int b) {
-    Request r = {0, 0, 0};
-    if (b < a.requests) {
-        const int lo = a.query_start[b], hi = a.query_start[b + 1], len = a.seq_lens[b];
-        r.row0 = first_row(lo, a.total);
-        r.rows = end_row(r.row0, hi, a.total) - r.row0;
-        r.len = len < 0 ? 0 : len;
-    }
+// 64 requests, one a lane, from b0 on.  before: the largest start of those below b0, and
+// afterwards of those below b0 + 64.
+__device__ __forceinline__ Request requests64(const Kv4AttnArgs& a, int b0, int& before) {
+    const int b = b0 + (int)(threadIdx.x & 63);
+    const bool there = b < a.requests;
+    const int lo = there ? a.query_start[b] : 0, hi = there ? a.query_start[b + 1] : 0, len = there ? a.seq_lens[b] : 0;
+    Request r;
+    r.row0 = first_row(before, lo, a.total);
+    if (a.requests > 1) r.row0 = wave_scan_max(r.row0);
+    r.rows = there ? end_row(r.row0, hi, a.total) - r.row0 : 0;
+    r.len = len < 0 ? 0 : len;
+    before = __builtin_amdgcn_readlane(r.row0, 63);
     return r;
 }
 __device__ __forceinline__ int walked(const Kv4AttnArgs& a, int len) { return walked_tokens(a.width, a.s.page_log2, len); }
@@ -75,15 +79,15 @@ struct Item {
 // KEYS (item_steps).
 template <int COLS, int KEYS>
 __device__ __forceinline__ bool find_item(const Kv4AttnArgs& a, int want, int target, Item& it) {
-    const int lane = threadIdx.x & 63;
-    Request r = request(a, lane);
+    int start = 0;
+    Request r = requests64(a, 0, start);
     int blocks, steps, m = item_steps<KEYS>(0, 0, 0, a.requests);
     sizes<COLS, KEYS>(a, r, blocks, steps);
     if (target) {
         int64_t work = (int64_t)blocks * steps;
         int all_blocks = blocks;
         for (int b0 = 64; b0 < a.requests; b0 += 64) {
-            sizes<COLS, KEYS>(a, request(a, b0 + lane), blocks, steps);
+            sizes<COLS, KEYS>(a, requests64(a, b0, start), blocks, steps);
             work += (int64_t)blocks * steps;
             all_blocks += blocks;
         }
@@ -102,8 +106,9 @@ __device__ __forceinline__ bool find_item(const Kv4AttnArgs& a, int want, int ta
         m = __builtin_amdgcn_readfirstlane(m);
     }
     int before = 0;
+    start = 0;
     for (int b0 = 0; b0 < a.requests; b0 += 64) {
-        if (a.requests > 64) r = request(a, b0 + lane);
+        if (a.requests > 64) r = requests64(a, b0, start);
         sizes<COLS, KEYS>(a, r, blocks, steps);
         const int splits = request_splits(steps, m), mine = blocks * splits;
         const int upto = before + wave_scan32(mine);
@@ -111,7 +116,6 @@ __device__ __forceinline__ bool find_item(const Kv4AttnArgs& a, int want, int ta
         if (hit) {
             const int at = __builtin_ctzll(hit);
             auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
-            it.b = b0 + at;
             it.r = Request{pick(r.row0), pick(r.rows), pick(r.len)};
             it.b = b0 + at;
             it.chunk = m * KEYS;
@@ -149,18 +153,19 @@ __device__ __forceinline__ void zero_rows(const Kv4AttnArgs& a) {
         for (int64_t i = (int64_t)lo * pieces + threadIdx.x; i < (int64_t)hi * pieces; i += blockDim.x) out[i] = u32x4{0, 0, 0, 0};
         for (int i = lo + (int)threadIdx.x; i < hi; i += (int)blockDim.x) a.records[i] = i32x4{0, 0, 0, 1};
     };
-    const int lane = threadIdx.x & 63;
+    int start = 0, first = 0, end = 0;                   // of all requests' rows
     for (int b0 = 0; b0 < a.requests; b0 += 64) {
-        const Request r = request(a, b0 + lane);
+        const Request r = requests64(a, b0, start);
+        if (b0 == 0) first = __builtin_amdgcn_readlane(r.row0, 0);
+        if (b0 + 64 >= a.requests) end = __builtin_amdgcn_readlane(r.row0 + r.rows, (a.requests - 1) & 63);
         uint64_t none = __ballot(r.len == 0 && r.rows > 0);
         for (; none; none &= none - 1) {
             const int at = __builtin_ctzll(none), row0 = __builtin_amdgcn_readlane(r.row0, at);
             clear(row0, row0 + __builtin_amdgcn_readlane(r.rows, at));
         }
     }
-    const Request first = request(a, 0), last = request(a, a.requests - 1);
-    clear(0, first.row0);
-    clear(last.row0 + last.rows, a.total);
+    clear(0, first);
+    clear(end, a.total);
 }
 
 // ---- pieces of both kernels ---------------------------------------------------------

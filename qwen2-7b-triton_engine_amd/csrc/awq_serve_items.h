@@ -35,8 +35,12 @@ constexpr int kTileItems = 1024, kSplitBelow = 256;
 // 41.0, 448 68 / 57.
 constexpr int kDecodeColumns = 128;
 
-// The rows of a request in a batch of `total`, from its entries of query_start.
-AWQ_ITEMS_FN int first_row(int lo, int total) { return lo < 0 ? 0 : lo < total ? lo : total; }
+// The rows of a request in a batch of `total`, from its entries of query_start: the first,
+// given the largest of the starts before it (0 of none), and the one past the last.  A start below
+// an earlier one counts as that one, so no row is two requests' and all of them have
+// `total` rows at most: the plan below counts on it.
+AWQ_ITEMS_FN int row_in(int start, int total) { return start < 0 ? 0 : start < total ? start : total; }
+AWQ_ITEMS_FN int first_row(int before, int lo, int total) { return before > row_in(lo, total) ? before : row_in(lo, total); }
 AWQ_ITEMS_FN int end_row(int row0, int hi, int total) { return hi < row0 ? row0 : hi < total ? hi : total; }
 
 // Tokens to walk over: one past the table where the length is (that one is not

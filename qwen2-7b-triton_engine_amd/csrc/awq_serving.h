@@ -140,7 +140,18 @@ __device__ __forceinline__ int wave_scan32(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2 and 3
     return v;
 }
-// The same over a workgroup of WAVES waves, and the whole in `all`.  Values of at
+// Largest of a value of 0 or more over the lanes below this one and itself.
+__device__ __forceinline__ int wave_scan_max(int v) {
+    auto step = [&](int o) { v = o > v ? o : v; };
+    step(__builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true));
+    step(__builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true));
+    step(__builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true));
+    step(__builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true));
+    step(__builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+    step(__builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+    return v;
+}
+// The sums over a workgroup of WAVES waves, and the whole in `all`.  Values of at
 // most 2^24 + 1: a wave's sum fits 32 bits, the waves' are added in 64.
 // lds: free for use before the call and after it.
 template <int WAVES>

@@ -18,8 +18,10 @@ Kernel walk(int requests, const int* starts, const int* lens, int total, int max
     int all_blocks = 0, item = 0;
     for (int pass = 0; pass < 2; ++pass) {
         if (pass) item = item_steps<KEYS>(target, work, all_blocks, requests);
+        int row0 = 0;
         for (int b = 0; b < requests; ++b) {
-            const int row0 = first_row(starts[b], total), rows = end_row(row0, starts[b + 1], total) - row0;
+            row0 = first_row(row0, starts[b], total);
+            const int rows = end_row(row0, starts[b + 1], total) - row0;
             const int len = lens[b] < 0 ? 0 : lens[b], n = walked_tokens(width, page_log2, len);
             const int blocks = request_blocks<COLS>(request_columns(rows, max_query, group), limit);
             const int steps = request_steps<KEYS>(n);

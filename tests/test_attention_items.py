@@ -5,6 +5,7 @@ of its launch's grid (less one, which clears rows of no request), and an item th
 several of its request a place for its sums."""
 import ctypes
 import os
+import random
 import subprocess
 from dataclasses import dataclass
 
@@ -65,3 +66,34 @@ def _fits(decode, tiles, places):
 ])
 def test_lengths_up_to_the_limit(walk, requests, group, kvh):
     _fits(*walk(requests, group, kvh, page=256))
+
+
+@pytest.mark.parametrize("starts,lens,total,group,kvh", [
+    ([0, 32] * 32 + [64], [4096] * 64, 64, 4, 8),
+    ([0, 16] * 32 + [16], [4096] * 64, 16, 8, 8),
+    ([0, 400] * 100 + [0], [2000] * 200, 400, 4, 4),           # tiles
+    ([9, 2, 30, -7, 2**31 - 1, 5, -2**31, 40, 12], [300] * 8, 33, 8, 2),
+])
+def test_starts_that_go_down(walk, starts, lens, total, group, kvh):
+    """No row is two requests': a start below an earlier one counts as that one."""
+    requests = list(zip(lens, [0] * len(lens)))
+    max_query = min(total, max(max(0, b - a) for a, b in zip(starts, starts[1:])))
+    _fits(*walk(requests, group, kvh, starts=starts, total=total, max_query=max_query))
+    _fits(*walk(requests, group, kvh, starts=starts, total=total, max_query=1))
+
+
+def test_many_shapes(walk):
+    """Random batches: single tokens, chunks and prompts, empty requests, bounds that are too small."""
+    rng = random.Random(0)
+    for _ in range(300):
+        n = rng.choice([1, 1, 2, 5, 64, 65, 300])
+        longest = rng.choice([1, 100, 5000, 200000])
+        most = rng.choice([1, 4, 60, 700])
+        requests = [(rng.choice([0, rng.randint(1, longest)]), rng.choice([0, 1, 1, rng.randint(1, most)])) for _ in range(n)]
+        total = sum(m for _, m in requests)
+        kw = {"total": max(0, total + rng.choice([0, 0, 9, -3])), "page": rng.choice([16, 64, 256])}
+        if rng.random() < 0.2:
+            kw["max_query"] = rng.randint(1, most)
+        if rng.random() < 0.2:
+            kw["width"] = rng.randint(1, 20)
+        _fits(*walk(requests, rng.choice([1, 4, 7, 8, 64]), rng.choice([1, 4, 8, 40]), **kw))
