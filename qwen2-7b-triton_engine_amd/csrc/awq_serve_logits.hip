@@ -124,13 +124,15 @@ __global__ __launch_bounds__(kThreads) void awq_logits_kernel(LogitsArgs a) {
     const bool history = a.tokens != nullptr, biases = a.bias_start != nullptr;
     int64_t len = history ? a.lengths[row] : 0;
     const int64_t prompt = history ? a.prompt_lens[row] : 0;
-    int bias_lo = biases ? a.bias_start[row] : 0, bias_hi = biases ? a.bias_start[row + 1] : 0;
+    const int bias_from = biases ? a.bias_start[row] : 0, bias_to = biases ? a.bias_start[row + 1] : 0;
     const float rep = history && a.repetition ? a.repetition[row] : 1.0f;
     const float pres = history && a.presence ? a.presence[row] : 0.0f;
     const float freq = history && a.frequency ? a.frequency[row] : 0.0f;
     len = len < a.width ? len : a.width;
-    bias_lo = bias_lo < 0 ? 0 : bias_lo;
-    bias_hi = bias_hi < a.bias_count ? bias_hi : a.bias_count;
+    // Both ends within the entries, and unsigned: with a thread's or a stride's number on top a
+    // start near 2^31 must not come out below the end.
+    const uint32_t bias_hi = bias_to < 0 ? 0 : bias_to < a.bias_count ? bias_to : a.bias_count;
+    const uint32_t bias_lo = bias_from < 0 ? 0 : (uint32_t)bias_from < bias_hi ? bias_from : bias_hi;
     constexpr int kFlight = 8;                      // tokens of a thread in flight
     int64_t t[kFlight];
     const bool wide_ids = a.token_bytes == 8;
@@ -164,10 +166,10 @@ __global__ __launch_bounds__(kThreads) void awq_logits_kernel(LogitsArgs a) {
     }
     __syncthreads();
     if (bias_lo < bias_hi) {
-        for (int i = bias_lo + tid; i < bias_hi; i += kThreads) {
+        for (uint32_t i = bias_lo + tid; i < bias_hi; i += kThreads) {
             const uint32_t at = (uint32_t)((i == bias_lo + tid ? first_bias : a.bias_tokens[i]) - v0);
             if (at >= (uint32_t)n) continue;
-            if (atomicMax(&entry[at], (uint32_t)i + 1u) == 0 && word[at] == 0) list[atomicAdd(&listed, 1)] = (uint16_t)at;
+            if (atomicMax(&entry[at], i + 1u) == 0 && word[at] == 0) list[atomicAdd(&listed, 1)] = (uint16_t)at;
         }
         __syncthreads();
     }

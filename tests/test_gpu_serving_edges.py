@@ -7,6 +7,8 @@ import pytest
 import torch
 from test_gpu_kv4 import _batch, _cache, _close, _i32
 
+from test_gpu_logits import _check
+
 from kernels.kv4 import kv4_attention
 
 pytestmark = pytest.mark.gpu
@@ -30,3 +32,21 @@ def test_starts_that_go_down(gpu, starts, total, rows):
     y = kv4_attention(*args, _i32(starts, gpu), rows)
     _close(y, O.attend(q.double().numpy().reshape(-1, 8, 64), k, v, lengths, meant, table, 16), "fp16", "starts that go down")
     assert torch.equal(y, kv4_attention(*args, _i32(meant, gpu), rows))
+
+
+@pytest.mark.parametrize("start", [
+    [2**31 - 1, 2**31 - 1, 2**31 - 1], [2**31 - 100, 2**31 - 1, 3], [9, 2**31 - 1, 2**31 - 500], [-2**31, -5, 2**31 - 1],
+    [2**31 - 2, -2**31, 5]])
+def test_bias_starts_outside_the_entries(gpu, start):
+    """Only entries that there are count: 0 .. 8."""
+    ids = torch.tensor([5, 5, 4, 99, 7, 5, 2, 9, 5], dtype=torch.int32)
+    _check(gpu, torch.zeros((2, 100)), bias=(torch.tensor(start, dtype=torch.int32), ids, torch.arange(9, dtype=torch.float32) + 1))
+
+
+@pytest.mark.parametrize("n", [511, 512, 513, 2000])
+def test_many_biases_in_a_row(gpu, n):
+    """More entries than a workgroup has threads, most tokens several times: the last one counts."""
+    g = torch.Generator().manual_seed(n)
+    start = torch.tensor([0, n, n + 3], dtype=torch.int32)
+    ids = torch.randint(0, 300, (n + 3,), generator=g, dtype=torch.int32) * 17
+    _check(gpu, torch.randn((2, 5100), generator=g).half(), bias=(start, ids, torch.randn(n + 3, generator=g) * 4))
