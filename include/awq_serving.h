@@ -128,7 +128,7 @@ int awq_serve_kv4_gather(const void* cache, const int32_t* slots, void* k, void*
  * earlier one counts as that one.  out [total, num_heads * head_dim] in q's type.
  * A request of more than table_width * page_size tokens gives NaN.
  * max_query: at least the largest number of rows of a request (it sizes the grid and the
- * workspace; rows past it are not computed).
+ * workspace; rows past it are NaN).
  * q is scaled by a power of two and held in fp16 (exact for fp16, to 2^-30 of the
  * row's largest value for bf16), the probabilities in two fp16 parts, all sums in
  * fp32.  num_heads a multiple of num_kv_heads, at most AWQ_SERVE_MAX_GROUP

@@ -144,13 +144,14 @@ __device__ __forceinline__ void write_records(const Kv4AttnArgs& a, const Item& 
                                          i >= a.max_query || it.splits == 1 ? 1 : blind ? 0 : it.splits};
     }
 }
-// Rows that no item has -- of no request, or of one without tokens -- are zeros.
+// Rows that no item has: those of no request, or of one without tokens, are zeros, those past
+// a max_query that was too small NaN (not what the memory held).
 // Done by the first workgroup past the items; a grid has at least one.
-__device__ __forceinline__ void zero_rows(const Kv4AttnArgs& a) {
+__device__ __forceinline__ void fill_rows(const Kv4AttnArgs& a) {
     const int pieces = a.nh * a.s.hd / 8;                // of 16 bytes
-    auto clear = [&](int lo, int hi) {
+    auto fill = [&](int lo, int hi, uint32_t w) {        // a word of two elements everywhere
         u32x4* out = reinterpret_cast<u32x4*>(a.out);
-        for (int64_t i = (int64_t)lo * pieces + threadIdx.x; i < (int64_t)hi * pieces; i += blockDim.x) out[i] = u32x4{0, 0, 0, 0};
+        for (int64_t i = (int64_t)lo * pieces + threadIdx.x; i < (int64_t)hi * pieces; i += blockDim.x) out[i] = u32x4{w, w, w, w};
         for (int i = lo + (int)threadIdx.x; i < hi; i += (int)blockDim.x) a.records[i] = i32x4{0, 0, 0, 1};
     };
     int start = 0, first = 0, end = 0;                   // of all requests' rows
@@ -158,14 +159,15 @@ __device__ __forceinline__ void zero_rows(const Kv4AttnArgs& a) {
         const Request r = requests64(a, b0, start);
         if (b0 == 0) first = __builtin_amdgcn_readlane(r.row0, 0);
         if (b0 + 64 >= a.requests) end = __builtin_amdgcn_readlane(r.row0 + r.rows, (a.requests - 1) & 63);
-        uint64_t none = __ballot(r.len == 0 && r.rows > 0);
-        for (; none; none &= none - 1) {
-            const int at = __builtin_ctzll(none), row0 = __builtin_amdgcn_readlane(r.row0, at);
-            clear(row0, row0 + __builtin_amdgcn_readlane(r.rows, at));
+        const int done = r.len == 0 ? 0 : a.max_query;   // rows that are an item's
+        for (uint64_t some = __ballot(r.rows > done); some; some &= some - 1) {
+            const int at = __builtin_ctzll(some), row0 = __builtin_amdgcn_readlane(r.row0, at);
+            const int skip = __builtin_amdgcn_readlane(done, at);
+            fill(row0 + skip, row0 + __builtin_amdgcn_readlane(r.rows, at), skip ? 0x7FFF7FFFu : 0u);
         }
     }
-    clear(0, first);
-    clear(end, a.total);
+    fill(0, first, 0);
+    fill(end, a.total, 0);
 }
 
 // ---- pieces of both kernels ---------------------------------------------------------
@@ -336,7 +338,7 @@ __global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs
 
     Item it;
     if (!find_item<kCols, kKeys>(a, blockIdx.x, a.decode_target, it)) {
-        if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) zero_rows(a);   // the grid's last column has no item
+        if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) fill_rows(a);   // the grid's last column has no item
         return;
     }
     write_records(a, it, false);
@@ -636,7 +638,7 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
     Item it;
     const int tid = threadIdx.x, lane = tid & 63;
     if (!find_item<kTileCols, kTileKeys>(a, blockIdx.x, a.tile_target, it)) {
-        if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && a.limit == 0) zero_rows(a);
+        if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && a.limit == 0) fill_rows(a);
         return;
     }
     write_records(a, it, true);

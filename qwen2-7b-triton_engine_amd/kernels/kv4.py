@@ -90,7 +90,7 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_tables: torch.Tensor, 
     ``[requests, width]``, ``seq_lens`` int32 ``[requests]`` the tokens of each request with
     its rows among them, ``query_start`` int32 ``[requests + 1]`` its first row (an entry below
     an earlier one counts as that one), ``max_query``
-    at least the most rows of a request (rows past it are not computed).  The i-th
+    at least the most rows of a request (rows past it are NaN).  The i-th
     of a request's n rows stands at position ``seq_lens - n + i`` and sees the tokens up to
     it; a row before the first token, and a row of no request, gives zeros.
     ``scale``: 1 / sqrt(head_dim) unless given.  A page outside the cache, or a length

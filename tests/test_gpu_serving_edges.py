@@ -5,7 +5,7 @@ import kv4_oracle as O
 import numpy as np
 import pytest
 import torch
-from test_gpu_kv4 import _batch, _cache, _close, _i32
+from test_gpu_kv4 import DT, _batch, _cache, _close, _i32
 
 from test_gpu_logits import _check
 
@@ -50,3 +50,22 @@ def test_many_biases_in_a_row(gpu, n):
     start = torch.tensor([0, n, n + 3], dtype=torch.int32)
     ids = torch.randint(0, 300, (n + 3,), generator=g, dtype=torch.int32) * 17
     _check(gpu, torch.randn((2, 5100), generator=g).half(), bias=(start, ids, torch.randn(n + 3, generator=g) * 4))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("most", [1, 3, 40])
+def test_rows_past_max_query_are_nan(gpu, most, dtype):
+    """A bound that is too small: the rows within it are right, the others say that they are not."""
+    rng = np.random.default_rng(most)
+    requests = [(50, 45), (9, 1), (0, 60), (300, 41)]
+    lengths, starts, table, pages = _batch(rng, requests, 16)
+    cache, k, v = _cache(rng, pages, 16, 2, 64, 64, gpu)
+    q = torch.from_numpy(rng.standard_normal((int(starts[-1]), 4 * 64)).astype(np.float32)).to(DT[dtype])
+    for _ in range(2):                                        # (memory that held a result before)
+        y = kv4_attention(q.to(gpu), cache, _i32(table, gpu), _i32(lengths, gpu), _i32(starts, gpu), most)
+    ref = O.attend(q.double().numpy().reshape(-1, 4, 64), k, v, lengths, starts, table, 16)
+    for b, (n, m) in enumerate(requests):
+        seen = m if n == 0 else min(m, most)                  # (rows of a request without tokens are zeros)
+        lo = int(starts[b])
+        _close(y[lo:lo + seen], ref[lo:lo + seen], dtype, f"request {b}")
+        assert torch.isnan(y[lo + seen:lo + m]).all()
