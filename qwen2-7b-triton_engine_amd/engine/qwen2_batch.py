@@ -48,6 +48,7 @@ class Qwen2BatchDecoder:
         self._data = torch.zeros((s.num_layers, num_pages, s.num_kv_heads,
                                   Kv4Cache.block_bytes(s.head_dim, page_size, group_size)), dtype=torch.uint8, device=self.dev)
         self.caches = [Kv4Cache.of(d, s.head_dim, page_size, group_size) for d in self._data]
+        self.failed = torch.zeros(max_requests, dtype=torch.int32, device=self.dev)   # of the last step
 
     # ---- one pass over a step's rows ---------------------------------------------
     def _attention(self, li: int, qkv: torch.Tensor, step: PagedStep, max_query: int) -> torch.Tensor:
@@ -81,12 +82,19 @@ class Qwen2BatchDecoder:
         ``ids`` int64 the rows of all requests, ``new_tokens`` int32 ``[max_requests]`` how many
         of them each has, ``max_query`` at least the most of one, ``requests`` the first so many
         whose logits are wanted (all).  A request that adds no row has no logits of its own: its row
-        is another request's."""
+        is another request's.
+
+        Nothing here waits for the device, so what it refuses -- a request whose pages or
+        rows do not suffice (``paged_step``) -- is told in ``failed``, int32 ``[max_requests]``, 1
+        where this step refused a request: it keeps its length, nothing of it is stored, and its
+        logits are NaN.  The other requests' tokens count."""
         step = paged_step(self.tables, new_tokens, ids.shape[0])
         h = self._rows(ids, step, max_query)
         self.tables.commit(step)
+        self.failed = step.failed
         ends = (step.query_start[1:].long() - 1).clamp(min=0)[:requests]
-        return self._logits(h.index_select(0, ends))
+        refused = step.failed[:requests].bool().unsqueeze(1)
+        return self._logits(h.index_select(0, ends).masked_fill(refused, float("nan")))
 
     def _check(self, prompts, new_tokens):
         requests, page = len(prompts), self.tables.page_size

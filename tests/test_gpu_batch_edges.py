@@ -1,0 +1,47 @@
+"""The batch engine where a request cannot be served, and calls that meet what earlier
+ones left."""
+import pytest
+import torch
+from test_gpu_batch import SHAPE, _model, _prompts
+
+from engine.qwen2_batch import Qwen2BatchDecoder
+from kernels.paged import paged_release
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(values, dev):
+    return torch.tensor(values, dtype=torch.int32, device=dev)
+
+
+def _step(engine, prompts, dev):
+    """Logits of a step that adds prompts[b] to request b (None: nothing)."""
+    new = [0 if p is None else len(p) for p in prompts]
+    ids = torch.cat([p for p in prompts if p is not None]).to(dev)
+    return engine.step(ids, _i32(new, dev), max(new))
+
+
+def _near(a, b):
+    """The same rows through the same kernels, in a batch of other rows: roundings of fp16 activations."""
+    return ((a.float() - b.float()).norm() / b.float().norm()).item() <= 4 * 2.0**-11
+
+
+def test_refused_requests_are_told_and_have_no_logits(gpu):
+    """Too few pages, for a prompt that is new and for a request that runs."""
+    rng = torch.Generator().manual_seed(11)
+    model, _ = _model(SHAPE, 12, gpu)
+    engine, ample = (Qwen2BatchDecoder(model, 3, num_pages=n, page_size=16) for n in (4, 20))
+    a, b, c = _prompts(rng, SHAPE, [20, 10, 40])
+    got, want = (_step(e, [a, b, c], gpu) for e in (engine, ample))
+    assert engine.failed.tolist() == [0, 0, 1] and ample.failed.tolist() == [0, 0, 0]
+    assert torch.isnan(got[2]).all() and engine.tables.lengths.tolist() == [20, 10, 0]
+    assert _near(got[:2], want[:2])
+    paged_release(ample.tables, _i32([20, 10, 0], gpu))
+    a, b = _prompts(rng, SHAPE, [13, 7])                     # one page is left, and either needs one
+    got, want = _step(engine, [a, b, None], gpu), _step(ample, [a, None, None], gpu)
+    assert engine.failed.tolist() == [0, 1, 0] and engine.tables.lengths.tolist() == [33, 10, 0]
+    assert torch.isnan(got[1]).all() and _near(got[0], want[0])
+    for e in (engine, ample):                                # the first request ends: now the second has its page
+        paged_release(e.tables, _i32([0, 10, 0], gpu))
+    got, want = (_step(e, [None, b, None], gpu) for e in (engine, ample))
+    assert engine.failed.tolist() == [0, 0, 0] and _near(got[1], want[1])
