@@ -51,6 +51,19 @@ class Qwen2BatchDecoder:
         self.failed = torch.zeros(max_requests, dtype=torch.int32, device=self.dev)   # of the last step
 
     # ---- one pass over a step's rows ---------------------------------------------
+    def _place(self, new_tokens: torch.Tensor, total: int) -> PagedStep:
+        """``paged_step`` under the model's ``max_seq_len``, which the tables know as whole pages
+        only.  A request that would pass it inside its last page is shown to the step with
+        a length that the step refuses, and keeps its own."""
+        t, limit = self.tables, self.model.max_seq_len
+        if limit % t.page_size == 0 or new_tokens.shape != t.lengths.shape:
+            return paged_step(t, new_tokens, total)
+        over = t.lengths + new_tokens > limit
+        state = torch.cat((t.lengths.masked_fill(over, -1), t.free_count))
+        step = paged_step(PagedTables.of(t.block_tables, state, t.free_pages, t.page_size), new_tokens, total)
+        step.lengths.copy_(torch.where(over, t.lengths, step.lengths))
+        return step
+
     def _attention(self, li: int, qkv: torch.Tensor, step: PagedStep, max_query: int) -> torch.Tensor:
         m = self.model
         q = kv4_append(qkv, self.caches[li], step.slots, step.positions, m.cos, m.sin, self.s.num_heads)
@@ -85,10 +98,10 @@ class Qwen2BatchDecoder:
         is another request's.
 
         Nothing here waits for the device, so what it refuses -- a request whose pages or
-        rows do not suffice (``paged_step``) -- is told in ``failed``, int32 ``[max_requests]``, 1
+        rows do not suffice (``paged_step``), or whose tokens would pass ``max_seq_len`` -- is told in ``failed``, int32 ``[max_requests]``, 1
         where this step refused a request: it keeps its length, nothing of it is stored, and its
         logits are NaN.  The other requests' tokens count."""
-        step = paged_step(self.tables, new_tokens, ids.shape[0])
+        step = self._place(new_tokens, ids.shape[0])
         h = self._rows(ids, step, max_query)
         self.tables.commit(step)
         self.failed = step.failed

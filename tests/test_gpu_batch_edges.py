@@ -5,6 +5,7 @@ import torch
 from test_gpu_batch import SHAPE, _model, _prompts
 
 from engine.qwen2_batch import Qwen2BatchDecoder
+from engine.qwen2_decode import Qwen2AwqDecoder
 from kernels.paged import paged_release
 
 pytestmark = pytest.mark.gpu
@@ -45,3 +46,25 @@ def test_refused_requests_are_told_and_have_no_logits(gpu):
         paged_release(e.tables, _i32([0, 10, 0], gpu))
     got, want = (_step(e, [None, b, None], gpu) for e in (engine, ample))
     assert engine.failed.tolist() == [0, 0, 0] and _near(got[1], want[1])
+
+
+@pytest.mark.parametrize("limit,lens", [(100, [99, 90]), (130, [127, 128])])
+def test_no_token_past_the_models_positions(gpu, limit, lens):
+    """The last page reaches past max_seq_len; a request that would too is refused like one without pages."""
+    rng = torch.Generator().manual_seed(limit)
+    engine = Qwen2BatchDecoder(Qwen2AwqDecoder(SHAPE, limit, seed=3, device=gpu), 3, page_size=64)
+    pages = lambda n: -(-n // 64)  # noqa: E731
+    assert torch.isfinite(_step(engine, [*_prompts(rng, SHAPE, lens), None], gpu)[:2]).all()
+    for add in ([1, 1], [limit - lens[0], 3], [0, 1], [2**30, 0], [1, limit - lens[1] - 1], [0, 1]):
+        ids = torch.zeros(min(sum(add), 9), dtype=torch.int64, device=gpu)
+        add.append(0)                                       # (behind rows that pass the batch, a request is refused too)
+        fits = [(*lens, 0)[b] + add[b] <= limit and sum(add[:b + 1]) <= 9 for b in range(3)]
+        logits = engine.step(ids, _i32(add, gpu), 9)
+        lens = [n + m if ok else n for n, m, ok in zip(lens, add, fits)]
+        assert engine.failed.tolist() == [0 if ok else 1 for ok in fits]
+        assert engine.tables.lengths.tolist() == [*lens, 0]
+        assert engine.tables.free_count.item() == engine.tables.free_pages.shape[0] - sum(map(pages, lens))
+        for b in range(2):
+            assert torch.isnan(logits[b]).all() if not fits[b] else add[b] == 0 or torch.isfinite(logits[b]).all()
+    with pytest.raises(ValueError):
+        engine.step(ids, _i32([1, 1], gpu), 9)
