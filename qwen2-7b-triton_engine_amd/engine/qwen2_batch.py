@@ -121,6 +121,8 @@ class Qwen2BatchDecoder:
         if sum(-(-n // page) for n in ends) > self.tables.free_pages.shape[0]:
             raise ValueError(f"the requests need {sum(-(-n // page) for n in ends)} pages, the cache has "
                              f"{self.tables.free_pages.shape[0]}")
+        if self.tables.lengths.any():
+            raise RuntimeError("requests of earlier steps are running: release their pages (paged_release) first")
 
     @torch.no_grad()
     def generate(self, prompts: list, new_tokens: int, repetition: float = 1.0, presence: float = 0.0,
@@ -129,7 +131,8 @@ class Qwen2BatchDecoder:
         ``[requests, new_tokens]`` on the host.  Penalties as in ``process_logits``, the same for all
         requests; ``biases`` a dict {token: value} per request; ``mask`` int32
         ``[requests, ceil(vocab / 32)]``, the tokens that a request's grammar allows.  All
-        requests' pages are returned at the end.  Raises if a mask left a request no token."""
+        requests' pages are returned at the end.  Raises if a mask left a request no token, and if
+        requests that a caller of ``step`` began are still running (it has all pages to itself)."""
         self._check(prompts, new_tokens)
         B, slots, dev = len(prompts), self.tables.block_tables.shape[0], self.dev
         lens = [p.shape[0] for p in prompts]
@@ -144,23 +147,23 @@ class Qwen2BatchDecoder:
             counts = [len(d) for d in biases]
             rules["bias"] = (i32([sum(counts[:b]) for b in range(B + 1)]), i32([t for d in biases for t in d]),
                              torch.tensor([float(v) for d in biases for v in d.values()], dtype=torch.float32, device=dev))
-        keep = torch.zeros(slots, dtype=torch.int32, device=dev)
-        paged_release(self.tables, keep)                # whatever an interrupted call left
         new = i32(lens + [0] * (slots - B))
         ids, most = torch.cat([p.to(dev) for p in prompts]), max(lens)
         rows = torch.arange(B, device=dev)
         out = []
-        for i in range(new_tokens):
-            logits = self.step(ids, new, most, B)
-            lengths = prompt_lens + i
-            _, token = process_logits(logits, tokens=history, lengths=lengths, out=logits, **rules)
-            out.append(token)
-            # a token that does not exist (-1) must not reach the embedding; reported below
-            ids, most = token.clamp(min=0), 1
-            history[rows, lengths.long()] = ids
-            if i == 0:
-                new = i32([1] * B + [0] * (slots - B))
-        paged_release(self.tables, keep)
+        try:
+            for i in range(new_tokens):
+                logits = self.step(ids, new, most, B)
+                lengths = prompt_lens + i
+                _, token = process_logits(logits, tokens=history, lengths=lengths, out=logits, **rules)
+                out.append(token)
+                # a token that does not exist (-1) must not reach the embedding; reported below
+                ids, most = token.clamp(min=0), 1
+                history[rows, lengths.long()] = ids
+                if i == 0:
+                    new = i32([1] * B + [0] * (slots - B))
+        finally:                                        # also of a call that fails or is interrupted
+            paged_release(self.tables, torch.zeros(slots, dtype=torch.int32, device=dev))
         tokens = torch.stack(out, 1).cpu()
         if (tokens < 0).any():
             raise RuntimeError("the mask left a request no token to take")

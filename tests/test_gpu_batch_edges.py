@@ -68,3 +68,23 @@ def test_no_token_past_the_models_positions(gpu, limit, lens):
             assert torch.isnan(logits[b]).all() if not fits[b] else add[b] == 0 or torch.isfinite(logits[b]).all()
     with pytest.raises(ValueError):
         engine.step(ids, _i32([1, 1], gpu), 9)
+
+
+def test_generate_leaves_running_requests_alone(gpu):
+    """It refuses while a caller of step has requests, and takes back its own pages when it fails."""
+    rng = torch.Generator().manual_seed(21)
+    model, successor = _model(SHAPE, 22, gpu)
+    engine = Qwen2BatchDecoder(model, 3, page_size=16)
+    a, b = _prompts(rng, SHAPE, [20, 5])
+    want = engine.generate([a, b], 4)
+    _step(engine, [None, a, None], gpu)
+    state = engine.tables.state.clone()
+    with pytest.raises(RuntimeError, match="running"):
+        engine.generate([a, b], 4)
+    assert torch.equal(engine.tables.state, state)
+    assert int(_step(engine, [None, successor[a[-1:]], None], gpu)[1].argmax()) == int(want[0, 1])
+    paged_release(engine.tables, _i32([0, 0, 0], gpu))
+    with pytest.raises(ValueError):                          # a mask of another vocabulary: found in the middle
+        engine.generate([a, b], 4, mask=torch.zeros((2, 3), dtype=torch.int32, device=gpu))
+    assert engine.tables.free_count.item() == engine.tables.free_pages.shape[0]
+    assert torch.equal(engine.generate([a, b], 4), want)
