@@ -141,8 +141,9 @@ class Qwen2BatchDecoder:
         for b, p in enumerate(prompts):
             history[b, :lens[b]] = p.to(dev)
         prompt_lens = i32(lens)
-        rules = {"repetition": torch.full((B,), repetition, device=dev), "presence": torch.full((B,), presence, device=dev),
-                 "frequency": torch.full((B,), frequency, device=dev), "mask": mask, "prompt_lens": prompt_lens}
+        each = lambda v: torch.full((B,), v, dtype=torch.float32, device=dev)  # noqa: E731
+        rules = {"repetition": each(repetition), "presence": each(presence), "frequency": each(frequency), "mask": mask,
+                 "prompt_lens": prompt_lens}
         if biases is not None:
             counts = [len(d) for d in biases]
             rules["bias"] = (i32([sum(counts[:b]) for b in range(B + 1)]), i32([t for d in biases for t in d]),

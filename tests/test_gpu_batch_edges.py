@@ -88,3 +88,13 @@ def test_generate_leaves_running_requests_alone(gpu):
         engine.generate([a, b], 4, mask=torch.zeros((2, 3), dtype=torch.int32, device=gpu))
     assert engine.tables.free_count.item() == engine.tables.free_pages.shape[0]
     assert torch.equal(engine.generate([a, b], 4), want)
+
+
+def test_generate_takes_whole_penalties(gpu):
+    """Penalties given as integers are the same numbers."""
+    rng = torch.Generator().manual_seed(31)
+    model, _ = _model(SHAPE, 32, gpu)
+    engine = Qwen2BatchDecoder(model, 2, page_size=16)
+    prompts = _prompts(rng, SHAPE, [9, 4])
+    rules = {"repetition": 2, "presence": 3, "frequency": 1}
+    assert torch.equal(engine.generate(prompts, 5, **rules), engine.generate(prompts, 5, **{k: float(v) for k, v in rules.items()}))
