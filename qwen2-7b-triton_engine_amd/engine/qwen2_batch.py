@@ -118,9 +118,9 @@ class Qwen2BatchDecoder:
         ends = [p.shape[0] + new_tokens for p in prompts]
         if max(ends) > self.model.max_seq_len:
             raise ValueError(f"prompt + new tokens ({max(ends)}) exceed max_seq_len {self.model.max_seq_len}")
-        if sum(-(-n // page) for n in ends) > self.tables.free_pages.shape[0]:
-            raise ValueError(f"the requests need {sum(-(-n // page) for n in ends)} pages, the cache has "
-                             f"{self.tables.free_pages.shape[0]}")
+        pages = sum(-(-(n - 1) // page) for n in ends)   # the last token is returned and not stored
+        if pages > self.tables.free_pages.shape[0]:
+            raise ValueError(f"the requests need {pages} pages, the cache has {self.tables.free_pages.shape[0]}")
         if self.tables.lengths.any():
             raise RuntimeError("requests of earlier steps are running: release their pages (paged_release) first")
 

@@ -98,3 +98,14 @@ def test_generate_takes_whole_penalties(gpu):
     prompts = _prompts(rng, SHAPE, [9, 4])
     rules = {"repetition": 2, "presence": 3, "frequency": 1}
     assert torch.equal(engine.generate(prompts, 5, **rules), engine.generate(prompts, 5, **{k: float(v) for k, v in rules.items()}))
+
+
+def test_generate_asks_for_no_page_that_it_does_not_use(gpu):
+    """The last token is returned and never stored: 14 + 3 tokens are one page of 16."""
+    rng = torch.Generator().manual_seed(41)
+    model, _ = _model(SHAPE, 42, gpu)
+    prompts = _prompts(rng, SHAPE, [14, 30])
+    want = Qwen2BatchDecoder(model, 2, page_size=16).generate(prompts, 3)
+    assert torch.equal(Qwen2BatchDecoder(model, 2, num_pages=3, page_size=16).generate(prompts, 3), want)
+    with pytest.raises(ValueError, match="need 5 pages, the cache has 3"):
+        Qwen2BatchDecoder(model, 2, num_pages=3, page_size=16).generate(prompts, 4)
