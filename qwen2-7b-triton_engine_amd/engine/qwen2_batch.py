@@ -92,7 +92,7 @@ class Qwen2BatchDecoder:
     @torch.no_grad()
     def step(self, ids: torch.Tensor, new_tokens: torch.Tensor, max_query: int, requests: int | None = None) -> torch.Tensor:
         """Logits fp16 ``[requests, vocab]`` of each request's last row after one pass:
-        ``ids`` int64 the rows of all requests, ``new_tokens`` int32 ``[max_requests]`` how many
+        ``ids`` int64 the rows of all requests (within the vocabulary), ``new_tokens`` int32 ``[max_requests]`` how many
         of them each has, ``max_query`` at least the most of one, ``requests`` the first so many
         whose logits are wanted (all).  A request that adds no row has no logits of its own: its row
         is another request's.
@@ -140,6 +140,9 @@ class Qwen2BatchDecoder:
         history = torch.zeros((B, max(lens) + new_tokens), dtype=torch.int64, device=dev)
         for b, p in enumerate(prompts):
             history[b, :lens[b]] = p.to(dev)
+        ids, most = torch.cat([p.to(dev) for p in prompts]), max(lens)
+        if ((ids < 0) | (ids >= self.s.vocab_size)).any():
+            raise ValueError(f"a prompt has a token outside the vocabulary [0, {self.s.vocab_size})")
         prompt_lens = i32(lens)
         each = lambda v: torch.full((B,), v, dtype=torch.float32, device=dev)  # noqa: E731
         rules = {"repetition": each(repetition), "presence": each(presence), "frequency": each(frequency), "mask": mask,
@@ -149,7 +152,6 @@ class Qwen2BatchDecoder:
             rules["bias"] = (i32([sum(counts[:b]) for b in range(B + 1)]), i32([t for d in biases for t in d]),
                              torch.tensor([float(v) for d in biases for v in d.values()], dtype=torch.float32, device=dev))
         new = i32(lens + [0] * (slots - B))
-        ids, most = torch.cat([p.to(dev) for p in prompts]), max(lens)
         rows = torch.arange(B, device=dev)
         out = []
         try:

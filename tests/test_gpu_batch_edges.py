@@ -109,3 +109,16 @@ def test_generate_asks_for_no_page_that_it_does_not_use(gpu):
     assert torch.equal(Qwen2BatchDecoder(model, 2, num_pages=3, page_size=16).generate(prompts, 3), want)
     with pytest.raises(ValueError, match="need 5 pages, the cache has 3"):
         Qwen2BatchDecoder(model, 2, num_pages=3, page_size=16).generate(prompts, 4)
+
+
+def test_generate_refuses_ids_outside_the_vocabulary(gpu):
+    """The embedding would look them up outside its table."""
+    model, _ = _model(SHAPE, 52, gpu)
+    engine = Qwen2BatchDecoder(model, 2, page_size=16)
+    one = torch.zeros(3, dtype=torch.int64)
+    for id_ in (-1, SHAPE.vocab_size, 2**40):
+        for dev in ("cpu", gpu):
+            bad = torch.tensor([5, id_], device=dev)
+            with pytest.raises(ValueError, match="vocabulary"):
+                engine.generate([one, bad], 2)
+    assert engine.generate([one, torch.tensor([SHAPE.vocab_size - 1])], 2).shape == (2, 2)
