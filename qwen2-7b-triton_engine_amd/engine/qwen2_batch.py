@@ -148,6 +148,8 @@ class Qwen2BatchDecoder:
         rules = {"repetition": each(repetition), "presence": each(presence), "frequency": each(frequency), "mask": mask,
                  "prompt_lens": prompt_lens}
         if biases is not None:
+            if len(biases) != B:
+                raise ValueError(f"biases of {len(biases)} requests for {B} prompts")
             counts = [len(d) for d in biases]
             rules["bias"] = (i32([sum(counts[:b]) for b in range(B + 1)]), i32([t for d in biases for t in d]),
                              torch.tensor([float(v) for d in biases for v in d.values()], dtype=torch.float32, device=dev))

@@ -122,3 +122,13 @@ def test_generate_refuses_ids_outside_the_vocabulary(gpu):
             with pytest.raises(ValueError, match="vocabulary"):
                 engine.generate([one, bad], 2)
     assert engine.generate([one, torch.tensor([SHAPE.vocab_size - 1])], 2).shape == (2, 2)
+
+
+def test_generate_refuses_biases_for_other_requests(gpu):
+    model, _ = _model(SHAPE, 62, gpu)
+    engine = Qwen2BatchDecoder(model, 2, page_size=16)
+    one = torch.zeros(3, dtype=torch.int64)
+    for biases in ([], [{5: 1.0}], [{}, {}, {5: 1.0}]):
+        with pytest.raises(ValueError, match="biases"):
+            engine.generate([one, one], 2, biases=biases)
+    assert engine.generate([one, one], 2, biases=[{}, {}]).shape == (2, 2)
