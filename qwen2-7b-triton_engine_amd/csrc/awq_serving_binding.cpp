@@ -59,7 +59,8 @@ struct Cache {
     int64_t heads() const { return data.size(1); }
 };
 
-// Tables as kernels/paged.py holds them.
+// Tables as kernels/paged.py holds them.  Checked where they are made and in every call: their parts
+// can be set, and the kernels go by them.
 void check_tables(const Tensor& block_tables, const Tensor& state, const Tensor& free_pages, int64_t page_size) {
     TORCH_CHECK_VALUE(block_tables.dim() == 2 && free_pages.dim() == 1, "block_tables must be 2-D and free_pages 1-D");
     const int64_t requests = block_tables.size(0), width = block_tables.size(1), capacity = free_pages.size(0);
@@ -74,7 +75,7 @@ void check_tables(const Tensor& block_tables, const Tensor& state, const Tensor&
                       " requests and at least one page");
     TORCH_CHECK_VALUE(width <= (1 << 30) / page_size && capacity <= (1 << 24), "a request's tokens pass 2^30, or the free pages 2^24");
 }
-// A cache as kernels/kv4.py holds it.
+// A cache as kernels/kv4.py holds it, checked alike.
 void check_cache(const Tensor& data, int64_t head_dim, int64_t page_size, int64_t group_size) {
     TORCH_CHECK_VALUE(head_dim == 64 || head_dim == 128, "head_dim ", head_dim, " must be 64 or 128");
     TORCH_CHECK_VALUE(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128 || page_size == 256, "page_size ",
@@ -95,6 +96,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_step(const Tensor& stat
                                                               int64_t page_size, int64_t total,
                                                               const c10::optional<std::vector<Tensor>>& out) {
     const Plain plain;
+    check_tables(block_tables, state, free_pages, page_size);
     const at::Device device = state.device();
     check_on_gpu(state, "the tables");
     const int64_t requests = block_tables.size(0), width = block_tables.size(1);
@@ -124,6 +126,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_step(const Tensor& stat
 
 Tensor paged_release(const Tensor& state, const Tensor& keep, const Tensor& block_tables, const Tensor& free_pages,
                      int64_t page_size) {
+    check_tables(block_tables, state, free_pages, page_size);
     const at::Device device = state.device();
     check_on_gpu(state, "the tables");
     const int64_t requests = block_tables.size(0);
@@ -141,6 +144,7 @@ Tensor kv4_append(const Tensor& qkv_in, const Tensor& data, int64_t head_dim, in
                   const Tensor& slots, const Tensor& positions, const OptTensor& cos_in, const OptTensor& sin_in,
                   int64_t num_heads) {
     const Plain plain;
+    check_cache(data, head_dim, page_size, group_size);
     const Cache cache{data, head_dim, page_size, group_size};
     const at::Device device = qkv_in.device();
     const int64_t columns = (num_heads + 2 * cache.heads()) * head_dim;
@@ -178,6 +182,7 @@ Tensor kv4_append(const Tensor& qkv_in, const Tensor& data, int64_t head_dim, in
 std::tuple<Tensor, Tensor> kv4_gather(const Tensor& data, int64_t head_dim, int64_t page_size, int64_t group_size,
                                       const Tensor& slots, at::ScalarType dtype) {
     const Plain plain;
+    check_cache(data, head_dim, page_size, group_size);
     const Cache cache{data, head_dim, page_size, group_size};
     TORCH_CHECK_VALUE(dtype == at::kHalf || dtype == at::kBFloat16, "dtype must be float16 or bfloat16, got ", dtype);
     check_on_gpu(data, "the cache");
@@ -197,6 +202,7 @@ Tensor kv4_attention(const Tensor& q_in, const Tensor& data, int64_t head_dim, i
                      const Tensor& block_tables, const Tensor& seq_lens, const Tensor& query_start, int64_t max_query,
                      c10::optional<double> scale_in) {
     const Plain plain;
+    check_cache(data, head_dim, page_size, group_size);
     const Cache cache{data, head_dim, page_size, group_size};
     const at::Device device = q_in.device();
     const int64_t kvh = cache.heads();
