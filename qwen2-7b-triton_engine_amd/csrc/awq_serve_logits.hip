@@ -95,28 +95,31 @@ __device__ __forceinline__ float rounded(float x) {
     return (float)__builtin_bit_cast(half_t, h);
 }
 
-// One workgroup: the stretch blockIdx.x of CH logits of row blockIdx.y.
-template <int DT, int CH>
+// Logits of a workgroup, eight a thread.  Shorter stretches read the history more often, longer
+// ones leave a CU one workgroup (LDS).  1024 / 4096 / 8192 logits, us: one row of 152064 6.97 /
+// 6.93 / 8.05, eight with histories of 4096 12.8 / 8.9 / 9.6, sixty-four 60 / 26 / 37; eight
+// of 50257 with 16000 12.4 / 13.6 / 15.2.
+constexpr int kStretch = 8 * kThreads;
+int stretches(int vocab) { return (vocab + kStretch - 1) / kStretch; }
+
+// One workgroup: the stretch blockIdx.x of row blockIdx.y.
+template <int DT>
 __global__ __launch_bounds__(kThreads) void awq_logits_kernel(LogitsArgs a) {
-    constexpr int kPieces = (CH / 8 + kThreads - 1) / kThreads;   // of a thread
     constexpr int kBytes = Piece<DT>::kBytes;
-    __shared__ __align__(16) uint32_t word[CH];     // counts of the history's tokens, then the new logits
-    __shared__ __align__(16) uint32_t entry[CH];    // 1 + the last bias entry, 0: none
-    __shared__ uint32_t touched[CH / 32];           // bit of each token with a new logit
-    __shared__ uint16_t list[CH];                   // those tokens
+    __shared__ __align__(16) uint32_t word[kStretch];   // counts of the history's tokens, then the new logits
+    __shared__ __align__(16) uint32_t entry[kStretch];  // 1 + the last bias entry, 0: none
+    __shared__ uint32_t touched[kStretch / 32];     // bit of each token with a new logit
+    __shared__ uint16_t list[kStretch];             // those tokens
     __shared__ int listed;
     __shared__ uint64_t best[kWaves];
     const int row = blockIdx.y, tid = threadIdx.x;
-    const int v0 = blockIdx.x * CH;
-    const int n = a.vocab - v0 < CH ? a.vocab - v0 : CH;
+    const int v0 = blockIdx.x * kStretch;
+    const int n = a.vocab - v0 < kStretch ? a.vocab - v0 : kStretch;
     const uint8_t* in = reinterpret_cast<const uint8_t*>(a.logits) + ((int64_t)row * a.ld + v0) * kBytes;
     uint8_t* out = reinterpret_cast<uint8_t*>(a.out) + ((int64_t)row * a.vocab + v0) * kBytes;
-    Piece<DT> x[kPieces];
-#pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-        const int at = 8 * (j * kThreads + tid);
-        if (at + 8 <= n) x[j].load(in + (int64_t)at * kBytes);
-    }
+    const int first = 8 * tid;                      // of the thread's eight
+    Piece<DT> x;
+    if (first + 8 <= n) x.load(in + (int64_t)first * kBytes);
     const uint32_t* mask = a.mask ? a.mask + (int64_t)row * ((a.vocab + 31) / 32) + v0 / 32 : nullptr;
 
     // Everything that hangs on nothing else is loaded at once: a workgroup is a
@@ -147,11 +150,11 @@ __global__ __launch_bounds__(kThreads) void awq_logits_kernel(LogitsArgs a) {
     if (len > 0) fetch(tid);
     const int first_bias = bias_lo + tid < bias_hi ? a.bias_tokens[bias_lo + tid] : -1;
 
-    for (int i = 4 * tid; i < CH; i += 4 * kThreads) {
+    for (int i = 4 * tid; i < kStretch; i += 4 * kThreads) {
         *reinterpret_cast<u32x4*>(&word[i]) = u32x4{0, 0, 0, 0};
         *reinterpret_cast<u32x4*>(&entry[i]) = u32x4{0, 0, 0, 0};
     }
-    for (int i = tid; i < CH / 32; i += kThreads) touched[i] = 0;
+    for (int i = tid; i < kStretch / 32; i += kThreads) touched[i] = 0;
     if (tid == 0) listed = 0;
     __syncthreads();
     for (int64_t i0 = tid; i0 < len; i0 += kFlight * kThreads) {
@@ -187,51 +190,40 @@ __global__ __launch_bounds__(kThreads) void awq_logits_kernel(LogitsArgs a) {
         word[at] = __builtin_bit_cast(uint32_t, rounded<DT>(y));
         atomicOr(&touched[at / 32], 1u << (at % 32));
     }
-    // In place the pieces below overwrite what is read above (and only that).
+    // In place what follows overwrites what is read above (and only that).
     __syncthreads();
 
-    float top = -INFINITY;
     uint64_t top_key = 0;
     auto see = [&](float v, int at) {               // by key: ties, zeros and NaN in order
         const uint64_t key = ((uint64_t)order_of(v) << 32) | (0xFFFFFFFFu - (uint32_t)(v0 + at));
         top_key = key > top_key ? key : top_key;
     };
-#pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-        const int at = 8 * (j * kThreads + tid);
-        if (at >= n) continue;
-        const uint32_t changed = touched[at / 32] >> (at % 32) & 0xFFu;
-        const uint32_t allowed = mask ? mask[at / 32] >> (at % 32) : 0xFFu;
-        if (at + 8 > n) {                           // the vocabulary's last piece, one by one
-            for (int e = 0; at + e < n; ++e) {
-                float y = changed >> e & 1 ? __builtin_bit_cast(float, word[at + e]) : load_one<DT>(in + (int64_t)(at + e) * kBytes);
+    if (first < n) {
+        const uint32_t changed = touched[first / 32] >> (first % 32) & 0xFFu;
+        const uint32_t allowed = mask ? mask[first / 32] >> (first % 32) : 0xFFu;
+        if (first + 8 > n) {                        // the vocabulary's last piece, one by one
+            for (int at = first; at < n; ++at) {
+                const int e = at - first;
+                float y = changed >> e & 1 ? __builtin_bit_cast(float, word[at]) : load_one<DT>(in + (int64_t)at * kBytes);
                 if (!(allowed >> e & 1)) y = -INFINITY;
-                store_one<DT>(out + (int64_t)(at + e) * kBytes, y);
-                see(y, at + e);
+                store_one<DT>(out + (int64_t)at * kBytes, y);
+                see(y, at);
             }
-            continue;
-        }
-        float y[8];
-        x[j].get(y);
-        if (changed) {
+        } else {
+            float y[8];
+            x.get(y);
+            if (changed) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (changed >> e & 1) y[e] = __builtin_bit_cast(float, word[at + e]);
-        }
-        float most = -INFINITY, sum = 0.0f;
+                for (int e = 0; e < 8; ++e)
+                    if (changed >> e & 1) y[e] = __builtin_bit_cast(float, word[first + e]);
+            }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            y[e] = allowed >> e & 1 ? y[e] : -INFINITY;
-            most = fmaxf(most, y[e]);
-            sum += y[e];
-        }
-        x[j].set(y);
-        x[j].store(out + (int64_t)at * kBytes);
-        // Few pieces raise the thread's maximum; a NaN, which it passes over, shows in the sum.
-        if (most > top || !(sum == sum) || top_key == 0) {
-            top = fmaxf(top, most);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) see(y[e], at + e);
+            for (int e = 0; e < 8; ++e) {
+                y[e] = allowed >> e & 1 ? y[e] : -INFINITY;
+                see(y[e], first + e);
+            }
+            x.set(y);
+            x.store(out + (int64_t)first * kBytes);
         }
     }
     top_key = wave_max64(top_key);
@@ -257,21 +249,14 @@ __global__ __launch_bounds__(64) void awq_greedy_kernel(const uint64_t* __restri
         next[blockIdx.x] = (uint32_t)(top >> 32) == kMinusInf ? -1 : (int64_t)(0xFFFFFFFFu - (uint32_t)top);
 }
 
-// Logits of a workgroup.  Shorter stretches read the history more often, longer ones
-// leave a CU one workgroup (LDS).  1024 / 4096 / 8192 logits, us: one row of 152064 6.97 /
-// 6.93 / 8.05, eight with histories of 4096 12.8 / 8.9 / 9.6, sixty-four 60 / 26 / 37; eight
-// of 50257 with 16000 12.4 / 13.6 / 15.2.
-constexpr int kStretch = 4096;
-int stretches(int vocab) { return (vocab + kStretch - 1) / kStretch; }
-
 }  // namespace
 
 size_t logits_workspace(int rows, int vocab) { return (size_t)rows * stretches(vocab) * sizeof(uint64_t); }
 
 hipError_t launch_logits(const LogitsArgs& a, hipStream_t stream) {
-    auto kernel = a.dtype == AWQ_SERVE_FP16   ? awq_logits_kernel<AWQ_SERVE_FP16, kStretch>
-                  : a.dtype == AWQ_SERVE_BF16 ? awq_logits_kernel<AWQ_SERVE_BF16, kStretch>
-                                              : awq_logits_kernel<AWQ_SERVE_FP32, kStretch>;
+    auto kernel = a.dtype == AWQ_SERVE_FP16   ? awq_logits_kernel<AWQ_SERVE_FP16>
+                  : a.dtype == AWQ_SERVE_BF16 ? awq_logits_kernel<AWQ_SERVE_BF16>
+                                              : awq_logits_kernel<AWQ_SERVE_FP32>;
     hipLaunchKernelGGL(kernel, dim3(stretches(a.vocab), a.rows), dim3(kThreads), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
