@@ -22,7 +22,8 @@
  * Lengths, tables, slots and positions are read on the device; the host does
  * not see them.  What lies outside its range never moves an access out of a
  * buffer: a token without a valid slot is not stored, a query whose request
- * refers to a page outside the cache gives NaN.
+ * refers to a page outside the cache gives NaN.  (Bounds that the host gives -- sizes,
+ * strides, max_pos -- have to be true of the buffers.)
  *
  * The cache of one layer: uint8 [num_pages, num_kv_heads, block], block =
  * page_size * (head_dim + 8 * head_dim / group_size) bytes.  A block holds one
@@ -106,7 +107,8 @@ int awq_serve_page_release(const int32_t* state, const int32_t* keep, const int3
  * positions (both NULL: no rotation), q_out [tokens, num_heads * head_dim] in
  * qkv's type, k and v quantised into the cache's slots.  A slot outside the
  * cache: nothing is stored.  A position outside 0 .. max_pos - 1: q_out NaN, nothing
- * stored.  Two rows of one slot: either's values.  dtype fp16 or bf16; qkv, cos, sin, q_out
+ * stored.  Two rows of one slot leave any mixture of theirs (codes of one, scales of the
+ * other) in it.  dtype fp16 or bf16; qkv, cos, sin, q_out
  * 16-byte aligned, qkv_stride a multiple of 8.  One launch. */
 int awq_serve_kv4_append(const void* qkv, int64_t qkv_stride, void* cache, const int32_t* slots,
                          const int32_t* positions, const void* cos, const void* sin, void* q_out, int64_t tokens,
@@ -126,11 +128,11 @@ int awq_serve_kv4_gather(const void* cache, const int32_t* slots, void* k, void*
  * sees the tokens 0 .. position.  A row that sees none (a negative position) and a
  * row of no request give zeros.  No row is two requests': an entry of query_start below an
  * earlier one counts as that one.  out [total, num_heads * head_dim] in q's type.
- * A request of more than table_width * page_size tokens gives NaN.
+ * A row that sees a token past table_width * page_size, or in a page outside the cache, gives NaN.
  * max_query: at least the largest number of rows of a request (it sizes the grid and the
  * workspace; rows past it are NaN).
- * q is scaled by a power of two and held in fp16 (exact for fp16, to 2^-30 of the
- * row's largest value for bf16), the probabilities in two fp16 parts, all sums in
+ * q is scaled by a power of two that brings a row's largest value below 2^8 and held in fp16
+ * (to 2^-32 of that value; exact for fp16 rows that are below 2^8 to begin with), the probabilities in two fp16 parts, all sums in
  * fp32.  num_heads a multiple of num_kv_heads, at most AWQ_SERVE_MAX_GROUP
  * times it; scale positive and finite; head_dim 64 or 128, group_size 32, 64 or 128 and at most head_dim.
  * workspace: at least awq_serve_kv4_attention_workspace bytes of any content. */

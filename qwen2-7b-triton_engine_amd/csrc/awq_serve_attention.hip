@@ -10,8 +10,8 @@
 // The first terms are products of tiles; the second are one more k-step (the
 // zeros against q's sums, held in three fp16 parts) and one more row block (the zeros
 // as further columns of V, with a column of ones that gives the softmax's sum).
-// q is scaled by its row's power of two and held in fp16, which is exact for fp16
-// input; the probabilities are fp32 and enter as two fp16 parts, hi and lo.
+// q is scaled by its row's power of two and held in fp16, to 2^-32 of the row's largest
+// value (fp16 rows below 2^8 exactly); the probabilities are fp32 and enter as two fp16 parts, hi and lo.
 // Outputs are as far from the 64-bit result as plain fp32 torch's (2.1e-4 of their
 // norm in fp16, 1.7e-3 in bf16: the output's own rounding).
 //

@@ -9,8 +9,8 @@ rows of a batch, one token of each request or chunks of prompts, each row seeing
 the tokens up to its own position (``model/qwen2.py:104-163``).  A token takes
 ``head_dim + 8 head_dim / group_size`` bytes for k and v of a head: 144 instead of
 512 for heads of 128 in groups of 64.  Attention adds no rounding to the cache's
-values: scores, softmax and sums are fp32, q and the values exact, the
-probabilities held to 23 bits.
+values: scores, softmax and sums are fp32, the values exact, q held to 2^-32 of its
+row's largest value, the probabilities to 23 bits.
 """
 from __future__ import annotations
 
@@ -68,7 +68,7 @@ def kv4_append(qkv: torch.Tensor, cache: Kv4Cache, slots: torch.Tensor, position
     """q after RoPE, ``[T, num_heads * head_dim]`` in ``qkv``'s type, of the rows ``qkv``
     fp16 or bf16 ``[T, (num_heads + 2 kv heads) * head_dim]`` (any row stride); their k
     (after RoPE) and v go into the cache's ``slots`` (int32 ``[T]``; one outside the cache,
-    -1 say: not stored).  ``cos`` / ``sin`` fp32 ``[max_pos, head_dim]`` at ``positions`` (int32
+    -1 say: not stored; a slot that two rows have holds a mixture of theirs).  ``cos`` / ``sin`` fp32 ``[max_pos, head_dim]`` at ``positions`` (int32
     ``[T]``; one outside: q NaN, nothing stored), both None: no rotation.  A token
     whose k or v of a head is not finite is stored so that every query that sees
     it gives NaN."""
@@ -93,7 +93,7 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, block_tables: torch.Tensor, 
     at least the most rows of a request (rows past it are NaN).  The i-th
     of a request's n rows stands at position ``seq_lens - n + i`` and sees the tokens up to
     it; a row before the first token, and a row of no request, gives zeros.
-    ``scale``: 1 / sqrt(head_dim) unless given.  A page outside the cache, or a length
-    past the table, gives NaN."""
+    ``scale``: 1 / sqrt(head_dim) unless given.  A row that sees a token in a page outside the
+    cache, or past the table, gives NaN."""
     return _native.binding().kv4_attention(q, cache.data, cache.head_dim, cache.page_size, cache.group_size, block_tables,
                                            seq_lens, query_start, max_query, scale)

@@ -69,3 +69,19 @@ def test_rows_past_max_query_are_nan(gpu, most, dtype):
         lo = int(starts[b])
         _close(y[lo:lo + seen], ref[lo:lo + seen], dtype, f"request {b}")
         assert torch.isnan(y[lo + seen:lo + m]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 6, 75])
+def test_only_rows_that_see_past_the_table_are_nan(gpu, rows):
+    """Five pages of 16 tokens under a length of 82: the rows at 80 and 81."""
+    rng = np.random.default_rng(rows)
+    lengths, starts, table, pages = _batch(rng, [(80, rows)], 16, width=5)
+    cache, k, v = _cache(rng, pages, 16, 2, 64, 64, gpu)
+    q = torch.from_numpy(rng.standard_normal((rows, 4 * 64)).astype(np.float32)).half()
+    y = kv4_attention(q.to(gpu), cache, _i32(table, gpu), _i32([82], gpu), _i32(starts, gpu), rows)
+    past = min(rows, 2)
+    assert torch.isnan(y[rows - past:]).all()
+    seen = rows - past                                       # positions up to 79
+    ref = O.attend(q[:seen].double().numpy().reshape(-1, 4, 64), k, v, lengths, [0, seen], table, 16)
+    if seen:
+        _close(y[:seen], ref, "fp16", "rows within the table")
