@@ -273,6 +273,12 @@ __device__ __forceinline__ int load_query(const uint16_t* src, int col, int t, h
     return exp;
 }
 
+// What one of a row's scaled scores counts in powers of two.  Kept finite: bf16 queries near 2^127
+// under a large scale pass fp32 here, and a difference of zero times infinity would be NaN.
+__device__ __forceinline__ float score_unit(float factor, int exp) {
+    return fminf(__builtin_ldexpf(factor, -exp), __FLT_MAX__);
+}
+
 // Tells the scheduler how to mix READS reads of LDS and MFMAS products: FIRST reads, then
 // one after every EACH products.
 template <int READS, int MFMAS, int EACH, int FIRST>
@@ -427,7 +433,7 @@ __global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs
     // exp(scale x) = exp2(x factor); the scores here are 2^exp times as large.
     // Every exponent is a difference of scores first: what they were rounded to
     // on the way must be the same wherever two meet.
-    const float factor = a.scale * 1.4426950408889634f, unit = __builtin_ldexpf(factor, -exp);
+    const float factor = a.scale * 1.4426950408889634f, unit = score_unit(factor, exp);
     const uint32_t base = base16_vgpr();
     // Rows GN .. 15 of the zeros' block: a row of ones at 4, the rest zero.
     const uint32_t z_mask = col < GN ? 0xFFFFFFFFu : 0u, z_fill = col == 4 ? 0x3C003C00u : 0u;
@@ -775,7 +781,7 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
     const int lim = limit_of(cc);
     const int exp = load_query<HD, GN, BF16>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + cc / group) * a.ld +
                                                  (int64_t)(g * group + cc % group) * HD, col, t, q, qz);
-    const float factor = a.scale * 1.4426950408889634f, unit = __builtin_ldexpf(factor, -exp);
+    const float factor = a.scale * 1.4426950408889634f, unit = score_unit(factor, exp);
     const int lim_min = __builtin_amdgcn_readlane(lim, 0), lim_max = __builtin_amdgcn_readlane(lim, 15);
 
     float m = -INFINITY;

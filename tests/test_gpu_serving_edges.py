@@ -9,7 +9,7 @@ from test_gpu_kv4 import DT, _batch, _cache, _close, _i32
 
 from test_gpu_logits import _check
 
-from kernels.kv4 import kv4_attention
+from kernels.kv4 import Kv4Cache, kv4_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,17 @@ def test_only_rows_that_see_past_the_table_are_nan(gpu, rows):
     ref = O.attend(q[:seen].double().numpy().reshape(-1, 4, 64), k, v, lengths, [0, seen], table, 16)
     if seen:
         _close(y[:seen], ref, "fp16", "rows within the table")
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+def test_queries_near_the_largest_bf16_under_a_large_scale(gpu, rows):
+    """Finite scores of 1e37 and more: the largest takes all, none is NaN."""
+    rng = np.random.default_rng(rows + 5)
+    lengths, starts, table, pages = _batch(rng, [(100, rows)], 16)
+    parts = [O.quantise((rng.standard_normal((pages * 16, 1, 64)) * gain).astype(np.float32), 64)[:3] for gain in (1e-4, 1.0)]
+    k, v = (O.values(p, 64) for p in parts)
+    cache = Kv4Cache.of(torch.from_numpy(O.pack(*parts, pages, 16, 64, 64)).to(gpu), 64, 16, 64)
+    q = torch.from_numpy((rng.choice([-1.0, 1.0], (rows, 64)) * rng.uniform(1e38, 3.3e38, (rows, 64))).astype(np.float32)).bfloat16()
+    y = kv4_attention(q.to(gpu), cache, _i32(table, gpu), _i32(lengths, gpu), _i32(starts, gpu), rows, scale=300.0)
+    ref = O.attend(q.double().numpy().reshape(-1, 1, 64), k, v, lengths, starts, table, 16, 300.0)
+    _close(y, ref, "bf16", "queries of 1e38")
