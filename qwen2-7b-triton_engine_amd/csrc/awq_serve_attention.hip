@@ -17,9 +17,10 @@
 //
 // Three launches at most: requests of few columns (decode), requests of many (tiles), and the
 // joining of what was split along the tokens.  28 heads of 128 over 4 kv heads, groups
-// of 64, pages of 64, graph replays, us: one request of 1100 tokens 10.3, 64 of up to
-// 4096 (2150 on average) 34.5, 16 of up to 16000 30.3; prompts of 256, 1024, 1777 and 4096
-// tokens 22, 42, 84 and 278 (433 TFLOP/s of useful work).
+// of 64, pages of 64, graph replays, us: one request of 1100 tokens 10.4, 64 of up to
+// 4096 (2190 on average) 36, 16 of up to 16000 31; prompts of 256, 1024, 1777 and 4096
+// tokens 21, 40, 78 and 277 (434 TFLOP/s of useful work).  Past 64 requests every wave's search for
+// its item takes over: 256 of up to 2048 tokens 73, 1024 of up to 512 139, 4096 of up to 256 1130.
 #include "awq_serve_items.h"
 #include "awq_serving.h"
 
@@ -42,15 +43,24 @@ struct Request {
     int row0, rows, len;               // first row, rows, tokens
 };
 // 64 requests, one a lane, from b0 on.  before: the largest start of those below b0, and
-// afterwards of those below b0 + 64.
-__device__ __forceinline__ Request requests64(const Kv4AttnArgs& a, int b0, int& before) {
+// afterwards of those below b0 + 64.  Starts go up, as good as always: only where they do not is the
+// running maximum formed, and up says whether they did (a walk of all requests that found it true need not
+// look again).  With the maximum in every walk 1024 requests took 162 us instead of 142.
+__device__ __forceinline__ Request requests64(const Kv4AttnArgs& a, int b0, int& before, bool look, bool& up) {
     const int b = b0 + (int)(threadIdx.x & 63);
-    const bool there = b < a.requests;
-    const int lo = there ? a.query_start[b] : 0, hi = there ? a.query_start[b + 1] : 0, len = there ? a.seq_lens[b] : 0;
+    int lo = a.total, hi = a.total, len = 0;
+    if (b < a.requests) {
+        lo = a.query_start[b];
+        hi = a.query_start[b + 1];
+        len = a.seq_lens[b];
+    }
     Request r;
-    r.row0 = first_row(before, lo, a.total);
-    if (a.requests > 1) r.row0 = wave_scan_max(r.row0);
-    r.rows = there ? end_row(r.row0, hi, a.total) - r.row0 : 0;
+    r.row0 = row_in(lo, a.total);
+    if (look && __any(hi < lo || r.row0 < before)) {
+        r.row0 = wave_scan_max(first_row(before, lo, a.total));
+        up = false;
+    }
+    r.rows = end_row(r.row0, hi, a.total) - r.row0;
     r.len = len < 0 ? 0 : len;
     before = __builtin_amdgcn_readlane(r.row0, 63);
     return r;
@@ -80,14 +90,15 @@ struct Item {
 template <int COLS, int KEYS>
 __device__ __forceinline__ bool find_item(const Kv4AttnArgs& a, int want, int target, Item& it) {
     int start = 0;
-    Request r = requests64(a, 0, start);
+    bool up = true;
+    Request r = requests64(a, 0, start, true, up);
     int blocks, steps, m = item_steps<KEYS>(0, 0, 0, a.requests);
     sizes<COLS, KEYS>(a, r, blocks, steps);
     if (target) {
         int64_t work = (int64_t)blocks * steps;
         int all_blocks = blocks;
         for (int b0 = 64; b0 < a.requests; b0 += 64) {
-            sizes<COLS, KEYS>(a, requests64(a, b0, start), blocks, steps);
+            sizes<COLS, KEYS>(a, requests64(a, b0, start, true, up), blocks, steps);
             work += (int64_t)blocks * steps;
             all_blocks += blocks;
         }
@@ -107,8 +118,9 @@ __device__ __forceinline__ bool find_item(const Kv4AttnArgs& a, int want, int ta
     }
     int before = 0;
     start = 0;
+    const bool look = !up || !target;                    // (without a target this is the first walk)
     for (int b0 = 0; b0 < a.requests; b0 += 64) {
-        if (a.requests > 64) r = requests64(a, b0, start);
+        if (a.requests > 64) r = requests64(a, b0, start, look, up);
         sizes<COLS, KEYS>(a, r, blocks, steps);
         const int splits = request_splits(steps, m), mine = blocks * splits;
         const int upto = before + wave_scan32(mine);
@@ -155,8 +167,9 @@ __device__ __forceinline__ void fill_rows(const Kv4AttnArgs& a) {
         for (int i = lo + (int)threadIdx.x; i < hi; i += (int)blockDim.x) a.records[i] = i32x4{0, 0, 0, 1};
     };
     int start = 0, first = 0, end = 0;                   // of all requests' rows
+    bool up = true;
     for (int b0 = 0; b0 < a.requests; b0 += 64) {
-        const Request r = requests64(a, b0, start);
+        const Request r = requests64(a, b0, start, true, up);
         if (b0 == 0) first = __builtin_amdgcn_readlane(r.row0, 0);
         if (b0 + 64 >= a.requests) end = __builtin_amdgcn_readlane(r.row0 + r.rows, (a.requests - 1) & 63);
         const int done = r.len == 0 ? 0 : a.max_query;   // rows that are an item's
@@ -325,13 +338,13 @@ struct Pages64 {
 // likewise: each is in flight under the other half of the pass, without a second
 // set of registers.  The waves' results meet once, at the end.
 //
-// What bounds it: at one request latency -- 7.1 us of launch, item, page, codes and
+// What bounds it: at one request latency -- 7.2 us of launch, item, page, codes and
 // the waves' meeting, one after another; at 64 requests of up to 4096 tokens (85 MB
 // of codes and scales, 30 us) the start and end of a workgroup, 9 us, and the vector
 // unit in between: 300 instructions a wave for 32 tokens, a third of them the
 // multiplying out of 8192 codes, against 28 products.  Three waves a SIMD (146 to 163
-// registers; four spilled 44 to 68 bytes).  A second set of K and V registers and a page number loaded
-// in the pass before were 33 to 36 us.
+// registers; four spilled 44 to 68 bytes).  A second set of K and V registers, and a page number
+// loaded in the pass before, were slower when they were tried.
 template <int HD, int GN, bool BF16>
 __global__ __launch_bounds__(kThreads, 3) void awq_kv4_decode_kernel(Kv4AttnArgs a) {
     constexpr int kSteps = HD / 32;
@@ -628,8 +641,8 @@ __device__ __forceinline__ int v_chunk(int row, int chunk) { return chunk ^ ((ro
 // What bounds it: at 4096 tokens the issue of vector instructions beside the
 // products, some 380 a wave and tile -- sixteen scores a lane with their exponentials
 // and two parts, 130 to multiply the codes out -- against 56 products; LDS is
-// busy 40 % of the time.  At 1777 the longest of the 784 workgroups, 28 tiles where the
-// average is 14.5.  128 columns a workgroup, in two column blocks a wave or in eight
+// busy 40 % of the time.  At 1777 the 780 workgroups, of 1 to 28 tiles, are nearly all resident at
+// once (768 places): the CUs whose three have the most tiles end last.  128 columns a workgroup, in two column blocks a wave or in eight
 // waves, multiply out half as much and were slower (107 and 116 us against 97 and 105): fewer, coarser
 // workgroups, and no registers to read operands ahead.
 // ONE_PAGE: pages of 64 tokens and more, where a tile lies in one of them and its
@@ -893,8 +906,8 @@ __global__ __launch_bounds__(kThreads, GN == 4 ? 2 : 3) void awq_kv4_tile_kernel
 // the overall maximum).  WAVES waves have a row and head: each every WAVES-th item,
 // a lane an item's weight and two columns' sums, eight loads in flight; the
 // waves meet in LDS.  All four where rows and heads are few (and items many), else
-// one: 2 requests of 32768 tokens, 64 rows and heads, 29.0 us with one and 25.6
-// with four; 64 of up to 4096, 1792 rows and heads, 33.8 and 37.5.
+// one: 2 requests of up to 32768 tokens, 64 rows and heads, 27.8 us with one and 24.7
+// with four; 64 of up to 4096, 1792 rows and heads, 35.8 and 38.1.
 template <int HD, int WAVES, bool BF16>
 __global__ __launch_bounds__(kThreads) void awq_kv4_combine_kernel(Kv4AttnArgs a) {
     constexpr int W = HD / 64;                           // columns a lane

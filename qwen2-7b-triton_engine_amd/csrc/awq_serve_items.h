@@ -23,16 +23,18 @@ constexpr int kTileKeys = 64;          // tokens of a tile kernel's step
 constexpr int kTileCols = 64;          // columns of a tile workgroup, 16 a wave
 
 // Items that a launch aims at, all kv heads together.  Decode: three workgroups on each
-// of 256 CUs, one round of them.  512 / 768 / 1024: 64 requests of up to 4096 tokens 46.8 /
-// 37.8 / 41.8 us, 16 of up to 16000 38.5 / 30.5 / 35.8, one of 16000 14.7 / 15.7 / 16.2.
+// of 256 CUs, one round of them.  512 / 768 / 1024: 64 requests of up to 4096 tokens 44.1 /
+// 36.1 / 39.5 us, 16 of up to 16000 37.4 / 30.7 / 34.8, one of 16000 14.7 / 15.0 / 15.8.
 constexpr int kDecodeItems = 768;
 // Tiles, only where the blocks of columns are fewer than CUs: 256 / 512 / 1024 items for
-// 3 chunks of 389 rows behind 4000 tokens 77 / 59 / 51 us.  Prompts with more blocks than that are
-// not split: a prompt of 1024 tokens 46 us whole, 50 to 73 split (partial sums of every row).
+// 3 chunks of up to 389 rows behind up to 4000 tokens, heads of 64, 120 / 61 / 54 us.  Prompts with more
+// blocks than that are not split: one of 1024 tokens 40 us whole and 57 split, 1777 78 and 110, 4096 277 and
+// 309 (partial sums of every row).
 constexpr int kTileItems = 1024, kSplitBelow = 256;
-// A request of more columns goes to the tile kernel.  8 requests behind up to 4000 tokens, all by
-// the decode kernel / by the tile kernel: 56 columns 24.9 / 30.4 us, 112 28.3 / 32.4, 224 42.9 /
-// 41.0, 448 68 / 57.
+// A request of more columns goes to the tile kernel.  8 requests of 4000 tokens each, all by
+// the decode kernel / by the tile kernel: 56 columns 33.0 / 35.1 us, 112 46.8 / 46.3, 224 92 / 66, 448
+// 123 / 123 (there the tiles' blocks are as many as CUs and not split); of 2200 tokens on average 25.8 /
+// 28.7, 38.3 / 32.9, 56 / 49, 92 / 121.
 constexpr int kDecodeColumns = 128;
 
 // The rows of a request in a batch of `total`, from its entries of query_start: the first,
@@ -44,10 +46,10 @@ AWQ_ITEMS_FN int first_row(int before, int lo, int total) { return before > row_
 AWQ_ITEMS_FN int end_row(int row0, int hi, int total) { return hi < row0 ? row0 : hi < total ? hi : total; }
 
 // Tokens to walk over: one past the table where the length is (that one is not
-// there, and gives NaN).  A table holds 2^30 tokens at most.
+// there, and gives NaN).  A table holds 2^30 tokens at most: 32 bits do.
 AWQ_ITEMS_FN int walked_tokens(int width, int page_log2, int len) {
-    const int64_t room = (int64_t)width << page_log2;
-    return len <= room ? len : (int)room + 1;
+    const int past = (width << page_log2) + 1;
+    return len < past ? len : past;
 }
 
 // Columns of a request that are computed, its blocks of them in this kernel (COLS says
@@ -56,10 +58,10 @@ AWQ_ITEMS_FN int request_columns(int rows, int max_query, int group) { return (r
 template <int COLS>
 AWQ_ITEMS_FN int request_blocks(int columns, int limit) {
     const bool mine = (columns <= limit) == (COLS == kCols);
-    return mine ? (columns + COLS - 1) / COLS : 0;
+    return mine ? (int)((uint32_t)(columns + COLS - 1) / COLS) : 0;
 }
 template <int KEYS>
-AWQ_ITEMS_FN int request_steps(int walked) { return (int)(((int64_t)walked + KEYS - 1) / KEYS); }
+AWQ_ITEMS_FN int request_steps(int walked) { return (int)((uint32_t)(walked + KEYS - 1) / KEYS); }
 
 // Steps of an item: as few as `target` items in all allow, from the sums over all
 // requests of blocks times steps and of blocks.  At most target + the blocks come out.

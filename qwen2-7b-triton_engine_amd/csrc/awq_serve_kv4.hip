@@ -8,7 +8,8 @@
 // is exact in fp16, so attention multiplies the matrix cores' operands out
 // without a rounding.  It costs a step that is at most 1/64 coarser.
 //
-// What bounds them: memory, and at a decode step's few tokens latency.  Eight
+// What bounds them: at a decode step's few tokens latency, at a prompt's the start and end of
+// workgroups and the loads, 80 bytes of cos, sin and RoPE partner for 16 of the row.  Eight
 // columns a thread: one 16-byte load of the row, one of its RoPE partner, one
 // 32-bit word of codes out.  k and v of a head go through the same lanes, since
 // a token's head is stored as NaN when either cannot be held.  The arithmetic
@@ -16,8 +17,8 @@
 // decided at the middle between two values, where one more or less rounding
 // moves a value by a whole step.  For the same reason the quotients are true
 // divisions, not products with a reciprocal.
-// Measured, 28 query and 4 kv heads of 128, groups of 64, us: append 4.2 for 64 tokens,
-// 12.7 for 2011 (37 MB: 2.9 TB/s), gather 2.9 and 4.0.
+// Measured in a graph, 28 query and 4 kv heads of 128, groups of 64, us: append 4.3 for 64 tokens,
+// 11.7 for 2011 (9.2 without RoPE; a copy of its rows takes 6.0), gather 2.7 and 3.9.
 #include "awq_serving.h"
 
 #pragma clang fp contract(off)

@@ -2,8 +2,7 @@
 // greedy token (include/awq_serving.h: awq_serve_logits):
 //   x / or * repetition, x - frequency n, x - presence, x + bias, -inf; argmax.
 //
-// What bounds it: memory -- the logits in and out once; for one row the
-// latency of two launches.  The penalties need to know how often each token
+// What it cannot do without is the logits in and out once.  The penalties need to know how often each token
 // occurs in the row's history.  A counter per token in memory would be a
 // second tensor as large as the logits, to be kept from step to step; here a
 // workgroup has a stretch of the vocabulary, counts the history's tokens that
@@ -12,9 +11,10 @@
 // as the largest index.  The listed tokens, few among many, get their new
 // logits by one thread each; then the stretch passes through, its logits loaded
 // before the counting began.  The history is read once per stretch, out of the caches.
-// Both launches, us: one row of 152064 logits 7.4, sixty-four with histories of 4096
-// 29.1 (41 MB in and out: 6.6 at the memory's rate): some 500 vector instructions a wave,
-// half of them the history's tokens, and chains of LDS latencies between barriers.  With a
+// What bounds it, both launches in a graph, us: one row of 152064 logits 7.6, the latency of
+// two launches; sixty-four with histories of 4096 26.5 (41 MB in and out: 6.6 at the memory's
+// rate), some 500 vector instructions a wave, half of them the history's tokens, which each of the
+// row's 38 stretches looks at, and chains of LDS latencies between barriers.  With a
 // counter and a bias entry read for every logit 45.  A fourth workgroup on a CU (4032 logits
 // each) changed nothing; a wave that gathers its tokens of the stretch before it counts them was
 // faster where histories are long (eight rows of 50257 with 16000: 13.5 -> 11.6) and slower for

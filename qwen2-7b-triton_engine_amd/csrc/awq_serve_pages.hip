@@ -8,12 +8,13 @@
 //   taken[b] = need[0] + .. + need[b - 1],   k-th page = F[c - 1 - k]
 // and token p of a request lies in slot page(p / P) * P + p % P.
 //
-// What bounds it: latency -- a few kilobytes pass.  One launch, no atomics and
+// What bounds it: latency -- a few kilobytes pass.  One launch, no atomics in memory and
 // nothing between workgroups: each has the two prefix sums of all requests to
 // itself (16 requests a thread at most) and keeps them in LDS, then places one row
 // a thread by binary search.  The torch form is some forty launches.  Measured: 64
-// requests of a token each 3.0 us, 16384 rows of 256 requests 6.1 (9.7 with
-// 64-bit wave sums).
+// requests of a token each 2.9 us, 16384 rows of 256 requests 6.0 (9.7 with
+// 64-bit wave sums), 4096 requests of a token each 16; a release of every eighth request of 64 or
+// 256 3.1 us, of 4096 26 (every workgroup adds all of them up).
 #include "awq_serving.h"
 
 namespace awq {

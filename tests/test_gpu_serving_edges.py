@@ -19,6 +19,7 @@ pytestmark = pytest.mark.gpu
     ([5, 2, 9, -7, 2**31 - 1, 30, -2**31], 33, 40),
     ([0, 70, 0, 70, 10, 140], 140, 70),                       # tiles
     ([0, 2] * 70 + [150], 150, 20),                           # the largest start so far passes from 64 requests on to the next
+    ([0, 40] * 50 + [1000], 1000, 960),                       # ... also where prompts are not split
 ])
 def test_starts_that_go_down(gpu, starts, total, rows):
     """A start below an earlier one counts as that one."""
