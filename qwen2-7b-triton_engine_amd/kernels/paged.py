@@ -67,7 +67,8 @@ class PagedTables:
         return self.state[-1:]
 
     def commit(self, step: "PagedStep") -> None:
-        """The step's lengths and free pages become the tables' (the tensor itself: no copy)."""
+        """The step's lengths and free pages become the tables' (the tensor itself: no copy).  A step
+        goes with the state that it was made from: not after a release or another step's commit."""
         if step.state.shape != self.state.shape or step.state.device != self.state.device:
             raise ValueError("the step belongs to other tables")
         self.state = step.state

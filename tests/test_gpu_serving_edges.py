@@ -100,3 +100,15 @@ def test_queries_near_the_largest_bf16_under_a_large_scale(gpu, rows):
     y = kv4_attention(q.to(gpu), cache, _i32(table, gpu), _i32(lengths, gpu), _i32(starts, gpu), rows, scale=300.0)
     ref = O.attend(q.double().numpy().reshape(-1, 1, 64), k, v, lengths, starts, table, 16, 300.0)
     _close(y, ref, "bf16", "queries of 1e38")
+
+
+def test_rows_past_max_query_of_one_prompt_are_nan(gpu):
+    """The tile kernel by itself, which then fills them; rows of no request behind them."""
+    rng = np.random.default_rng(17)
+    lengths, starts, table, pages = _batch(rng, [(300, 90)], 16)
+    cache, k, v = _cache(rng, pages, 16, 2, 64, 64, gpu)
+    q = torch.from_numpy(rng.standard_normal((95, 8 * 64)).astype(np.float32)).half()
+    y = kv4_attention(q.to(gpu), cache, _i32(table, gpu), _i32(lengths, gpu), _i32(starts, gpu), 40)
+    ref = O.attend(q.double().numpy().reshape(-1, 8, 64), k, v, lengths, starts, table, 16)
+    _close(y[:40], ref[:40], "fp16", "rows within the bound")
+    assert torch.isnan(y[40:90]).all() and (y[90:] == 0).all()
