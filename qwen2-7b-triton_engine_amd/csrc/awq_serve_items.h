@@ -1,18 +1,12 @@
 // How attention over the paged cache is cut into items (csrc/awq_serve_attention.hip):
 // the arithmetic that its kernels, their grids and the workspace have in common.
-// Plain C++ without the HIP headers, so that tests/test_attention_items.py runs it on the
-// host: every item has to have a workgroup, and every item that is one of several a place
-// for its sums.
+// Plain C++ without the HIP headers (constexpr functions are the device's too), so that
+// tests/test_attention_items.py runs it on the host: every item has to have a
+// workgroup, and every item that is one of several a place for its sums.
 #pragma once
 
 #include <stddef.h>
 #include <stdint.h>
-
-#ifdef __HIPCC__
-#define AWQ_ITEMS_FN __host__ __device__ inline
-#else
-#define AWQ_ITEMS_FN inline
-#endif
 
 namespace awq {
 
@@ -41,27 +35,27 @@ constexpr int kDecodeColumns = 128;
 // given the largest of the starts before it (0 of none), and the one past the last.  A start below
 // an earlier one counts as that one, so no row is two requests' and all of them have
 // `total` rows at most: the plan below counts on it.
-AWQ_ITEMS_FN int row_in(int start, int total) { return start < 0 ? 0 : start < total ? start : total; }
-AWQ_ITEMS_FN int first_row(int before, int lo, int total) { return before > row_in(lo, total) ? before : row_in(lo, total); }
-AWQ_ITEMS_FN int end_row(int row0, int hi, int total) { return hi < row0 ? row0 : hi < total ? hi : total; }
+constexpr int row_in(int start, int total) { return start < 0 ? 0 : start < total ? start : total; }
+constexpr int first_row(int before, int lo, int total) { return before > row_in(lo, total) ? before : row_in(lo, total); }
+constexpr int end_row(int row0, int hi, int total) { return hi < row0 ? row0 : hi < total ? hi : total; }
 
 // Tokens to walk over: one past the table where the length is (that one is not
 // there, and gives NaN).  A table holds 2^30 tokens at most: 32 bits do.
-AWQ_ITEMS_FN int walked_tokens(int width, int page_log2, int len) {
+constexpr int walked_tokens(int width, int page_log2, int len) {
     const int past = (width << page_log2) + 1;
     return len < past ? len : past;
 }
 
 // Columns of a request that are computed, its blocks of them in this kernel (COLS says
 // which), its tokens in steps.  limit: columns up to which a request is the decode kernel's.
-AWQ_ITEMS_FN int request_columns(int rows, int max_query, int group) { return (rows < max_query ? rows : max_query) * group; }
+constexpr int request_columns(int rows, int max_query, int group) { return (rows < max_query ? rows : max_query) * group; }
 template <int COLS>
-AWQ_ITEMS_FN int request_blocks(int columns, int limit) {
+constexpr int request_blocks(int columns, int limit) {
     const bool mine = (columns <= limit) == (COLS == kCols);
     return mine ? (int)((uint32_t)(columns + COLS - 1) / COLS) : 0;
 }
 template <int KEYS>
-AWQ_ITEMS_FN int request_steps(int walked) { return (int)((uint32_t)(walked + KEYS - 1) / KEYS); }
+constexpr int request_steps(int walked) { return (int)((uint32_t)(walked + KEYS - 1) / KEYS); }
 
 // Steps of an item: as few as `target` items in all allow, from the sums over all
 // requests of blocks times steps and of blocks.  At most target + the blocks come out.
@@ -69,7 +63,7 @@ AWQ_ITEMS_FN int request_steps(int walked) { return (int)((uint32_t)(walked + KE
 // an item has all of its request's: the grid has no place for more, and without a target the
 // workspace none for sums.
 template <int KEYS>
-AWQ_ITEMS_FN int item_steps(int target, int64_t work, int all_blocks, int requests) {
+constexpr int item_steps(int target, int64_t work, int all_blocks, int requests) {
     constexpr int kMost = (1 << 30) / KEYS + 1;          // of a request: 2^30 tokens, and one past the table
     if (!target) return kMost;
     // Each block ends in a shorter item, half of one too many on average: with as many
@@ -81,9 +75,9 @@ AWQ_ITEMS_FN int item_steps(int target, int64_t work, int all_blocks, int reques
     return few ? (few < (uint32_t)kMost ? (int)few : kMost)
                : work == 0 ? 1 : work < most ? (int)((work + target - 1) / target) : kMost;
 }
-AWQ_ITEMS_FN int request_splits(int steps, int item) { return (int)((uint32_t)(steps + item - 1) / (uint32_t)item); }
+constexpr int request_splits(int steps, int item) { return (int)((uint32_t)(steps + item - 1) / (uint32_t)item); }
 // Where an item ends that begins at `start`, of a block that sees `limit` tokens.
-AWQ_ITEMS_FN int item_end(int start, int chunk, int limit) {
+constexpr int item_end(int start, int chunk, int limit) {
     return limit - start < chunk ? limit : start + chunk;   // start + chunk may pass 32 bits where limit does not
 }
 
