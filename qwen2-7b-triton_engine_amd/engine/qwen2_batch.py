@@ -56,8 +56,8 @@ class Qwen2BatchDecoder:
         only.  A request that would pass it inside its last page is shown to the step with
         a length that the step refuses, and keeps its own."""
         t, limit = self.tables, self.model.max_seq_len
-        if limit % t.page_size == 0 or new_tokens.shape != t.lengths.shape:
-            return paged_step(t, new_tokens, total)
+        if limit % t.page_size == 0 or new_tokens.shape != t.lengths.shape or new_tokens.device != t.state.device:
+            return paged_step(t, new_tokens, total)      # (which refuses what is no int32 tensor of the tables')
         over = t.lengths + new_tokens > limit
         state = torch.cat((t.lengths.masked_fill(over, -1), t.free_count))
         step = paged_step(PagedTables.of(t.block_tables, state, t.free_pages, t.page_size), new_tokens, total)

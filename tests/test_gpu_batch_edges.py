@@ -66,8 +66,9 @@ def test_no_token_past_the_models_positions(gpu, limit, lens):
         assert engine.tables.free_count.item() == engine.tables.free_pages.shape[0] - sum(map(pages, lens))
         for b in range(2):
             assert torch.isnan(logits[b]).all() if not fits[b] else add[b] == 0 or torch.isfinite(logits[b]).all()
-    with pytest.raises(ValueError):
-        engine.step(ids, _i32([1, 1], gpu), 9)
+    for bad in (_i32([1, 1], gpu), _i32([1, 1, 0], "cpu"), _i32([1, 1, 0], gpu).long()):
+        with pytest.raises(ValueError):
+            engine.step(ids, bad, 9)
 
 
 def test_generate_leaves_running_requests_alone(gpu):
