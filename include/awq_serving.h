@@ -1,12 +1,14 @@
 /*
  * awq_serving.h -- C ABI of the serving operators in the W4A16 AWQ library:
- * many requests that share one paged KV cache held in 4 bits.
+ * many requests that share one paged KV cache, held in 4 bits or as it comes in 16.
  *
  *   awq_serve_page_step       block tables, slots and positions of a step's tokens
  *   awq_serve_page_release    pages of requests that end or shrink go back
  *   awq_serve_kv4_append      RoPE of q and k; k and v quantised and stored
  *   awq_serve_kv4_gather      the values that the cache holds
  *   awq_serve_kv4_attention   attention over the cache
+ *   awq_serve_kv16_append     RoPE of q and k; k and v stored as they are
+ *   awq_serve_kv16_attention  attention over that cache: windows, documents, prefixes, capped scores, distances
  *   awq_serve_logits          penalties, biases, a grammar's mask, greedy token
  *
  * The reference has one static fp16 cache and one sequence
@@ -25,7 +27,7 @@
  * refers to a page outside the cache gives NaN.  (Bounds that the host gives -- sizes,
  * strides, max_pos -- have to be true of the buffers.)
  *
- * The cache of one layer: uint8 [num_pages, num_kv_heads, block], block =
+ * The 4-bit cache of one layer: uint8 [num_pages, num_kv_heads, block], block =
  * page_size * (head_dim + 8 * head_dim / group_size) bytes.  A block holds one
  * page of one kv head:
  *
@@ -145,6 +147,44 @@ int awq_serve_kv4_attention(const void* q, int64_t q_stride, const void* cache, 
                             int64_t head_dim, int64_t table_width, int64_t num_pages, int64_t page_size,
                             int64_t group_size, float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
                             void* stream);
+
+/* The 16-bit cache of one layer: fp16 or bf16 [num_pages, num_kv_heads, 2, page_size, head_dim], K
+ * and V of a page and head.
+ *
+ * q, k and v of `tokens` rows of a fused projection as awq_serve_kv4_append takes them: RoPE in fp32, rounded
+ * once to dtype (a value that fp16 cannot hold becomes an infinity); k and v into the cache's slots. */
+int awq_serve_kv16_append(const void* qkv, int64_t qkv_stride, void* cache, const int32_t* slots,
+                          const int32_t* positions, const void* cos, const void* sin, void* q_out, int64_t tokens,
+                          int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t num_pages,
+                          int64_t page_size, int64_t max_pos, int32_t dtype, void* stream);
+
+/* softmax(score) V over a 16-bit paged cache, requests, rows and tables as in awq_serve_kv4_attention.  The
+ * score of row i (at position p_i, see there) and token j, in this order:
+ *   x = scale * q_i . k_j
+ *   softcap > 0:      x = softcap * tanh(x / softcap)
+ *   slopes != NULL:   x = x - slopes[head] * |p_i - j|          fp32 [num_heads]
+ * and row i sees token j where all of these hold:
+ *   j <= p_i, or prefix != NULL and j < prefix[b]               int32 [requests]; j < seq_lens[b] always
+ *   window > 0:       j > p_i - window
+ *   first != NULL:    j >= first[i]                             int32 [total], by rows of the batch
+ * A row that sees nothing (a negative position, first[i] past it) and a row of no request give zeros; rows past
+ * max_query, and rows that see a token past the table or in a page outside the cache, NaN.  What a row does
+ * not see may hold anything.  A row that sees a key or value that is not finite is not finite: in the columns
+ * that the arithmetic says, or in all of them.
+ * Scores, softmax and sums are fp32; the probabilities enter the product with V in dtype where a request
+ * has many rows (an error of half a step of dtype each, as the output's own), in two parts of dtype
+ * otherwise.  bf16 queries are scaled by a power of two first.  scale positive and finite, softcap 0 or
+ * at least 2^-100 and finite; head_dim 64 or 128; cache 16-byte aligned.
+ * workspace: at least awq_serve_kv16_attention_workspace bytes of any content. */
+size_t awq_serve_kv16_attention_workspace(int64_t requests, int64_t total, int64_t max_query, int64_t num_heads,
+                                          int64_t num_kv_heads, int64_t head_dim, int64_t table_width,
+                                          int64_t page_size);
+int awq_serve_kv16_attention(const void* q, int64_t q_stride, const void* cache, const int32_t* block_tables,
+                             const int32_t* seq_lens, const int32_t* query_start, const float* slopes,
+                             const int32_t* prefix, const int32_t* first, void* out, int64_t requests, int64_t total,
+                             int64_t max_query, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                             int64_t table_width, int64_t num_pages, int64_t page_size, int64_t window, float scale,
+                             float softcap, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* One step's logits [rows, vocab] (row_stride elements from row to row) after, in this
  * order and in fp32:

@@ -1,0 +1,717 @@
+// Attention over the 16-bit paged cache (include/awq_serving.h:
+// awq_serve_kv16_attention): o = softmax(score(q K^T)) V for the rows of many
+// requests, each over its own pages, GQA heads; the score is scale x, capped by
+// c tanh(x / c), less slope |i - j|, and a row sees tokens lo .. hi - 1 of a window,
+// a document or a prefix.
+//
+// Both kernels form S^T = K Q^T: an MFMA column is a (row, head) pair, so that the
+// running maximum and sum of a column live in the lanes that hold its scores, and
+// the probabilities are already the B operand of O^T = V^T P^T (the k order of that
+// product, tokens, is V's as it is read).  Rows and the heads that share a kv head are
+// one axis of columns: K and V of a token are read once for all of them.
+#include "awq_serve_walk.h"
+
+namespace awq {
+namespace {
+
+constexpr int k16Cols = Kv16AttnArgs::kTileCols;
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// ---- 16-bit operands of either type, eight in four words ---------------------------
+
+template <bool BF16>
+__device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return mfma16x16x32(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c);
+}
+template <bool BF16>
+__device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+// Two values rounded to nearest.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    if constexpr (BF16)
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x, y}, bf16x2));
+    else
+        return as_u32(__builtin_convertvector(f2{x, y}, half2_t));
+}
+template <bool BF16>
+__device__ __forceinline__ float low16(uint32_t w) {
+    if constexpr (BF16) return __builtin_bit_cast(float, w << 16);
+    else return (float)as_h2(w).x;
+}
+template <bool BF16>
+__device__ __forceinline__ float high16(uint32_t w) {
+    if constexpr (BF16) return __builtin_bit_cast(float, w & 0xFFFF0000u);
+    else return (float)as_h2(w).y;
+}
+template <bool BF16>
+constexpr uint32_t kOnes = BF16 ? 0x3F803F80u : 0x3C003C00u;
+template <bool BF16>
+constexpr uint32_t kExponents = BF16 ? 0x7F807F80u : 0x7C007C00u;
+
+// Largest exponent field of each half: all ones where a value is not finite.
+template <bool BF16>
+__device__ __forceinline__ uint32_t exponents(uint32_t most, uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most),
+                                                                  __builtin_bit_cast(u16x2, w & kExponents<BF16>)));
+}
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(uint32_t most) {
+    constexpr uint32_t kLow = kExponents<BF16> & 0xFFFFu;
+    return (most & 0xFFFFu) == kLow || (most >> 16) == kLow;
+}
+// The same words with 0 in the place of values that are not finite.
+template <bool BF16>
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) {
+    constexpr uint32_t kLow = kExponents<BF16> & 0xFFFFu, kHigh = kExponents<BF16> & 0xFFFF0000u;
+    return ((w & kLow) == kLow ? 0u : w & 0xFFFFu) | ((w & kHigh) == kHigh ? 0u : w & 0xFFFF0000u);
+}
+
+// The probabilities' scale: fp16's smallest values would lose bits, 2^14 times as large
+// they keep 11 down to 2^-28.
+template <bool BF16>
+constexpr float kPScale = BF16 ? 0.0f : 14.0f;
+// The running maximum is raised only where a score passes it by more than this (in
+// powers of two): probabilities of up to 2^1.5 still fit fp16 when scaled, and most
+// tiles do without the cross-lane maximum and the rescaling.
+constexpr float kSlack16 = 1.5f;
+
+// bf16 queries are brought to at most 2^8 by a power of two, so that a sum of products
+// stays inside fp32 for keys of ordinary size; fp16's are inside it as they are.  Returns the power's exponent.
+// mx: largest value of the row.
+__device__ __forceinline__ int query_exp(float mx) {
+    const int exp = 8 - __builtin_amdgcn_frexp_expf(mx);
+    return exp < 100 ? exp : 100;
+}
+__device__ __forceinline__ u32x4 scaled_bf16(u32x4 w, float up) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack2<true>(low16<true>(w[i]) * up, high16<true>(w[i]) * up);
+    return w;
+}
+// What multiplies a product of the scaled query: kept finite (2^127 under a large scale passes fp32 here).
+__device__ __forceinline__ float unit_of(float factor, int exp) { return fminf(__builtin_ldexpf(factor, -exp), __FLT_MAX__); }
+
+// c tanh(x / c).  Below 1/4 the series, to 1e-8 of the value; above, 1 - 2 / (1 + e^2u), whose cancellation costs
+// 5e-7 of it there at most.
+__device__ __forceinline__ float capped(float x, float c, float inv) {
+    const float u = x * inv, u2 = u * u;
+    const float e = __builtin_amdgcn_exp2f(u * 2.8853900817779268f);
+    const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+    const float near = u * fmaf(u2, fmaf(u2, fmaf(u2, fmaf(u2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    return c * (fabsf(u) < 0.25f ? near : far);
+}
+
+// ---- few columns: decode ---------------------------------------------------------------
+
+// One workgroup: an item's tokens of one kv head for up to 16 columns, 32 tokens per
+// wave and pass.  Lane (i, t) of K holds token i, columns 32 s + 8 t ..; of V the columns
+// VC i .. VC i + VC - 1 of tokens 4 t .. 4 t + 3 of both halves, turned into the A operands of VC products
+// by byte permutations: V's row order in the result is free.  K's registers are loaded
+// again as soon as its products are made, V's likewise.  The waves meet once, at the end.
+// The probabilities enter in two 16-bit parts: the products wait for memory anyway.
+template <int HD, bool BF16, bool SHAPED>
+__global__ __launch_bounds__(kThreads, 2) void awq_kv16_decode_kernel(Kv16AttnArgs a) {
+    constexpr int kSteps = HD / 32;
+    constexpr int VC = HD / 16;            // V columns per lane
+    constexpr int VW = VC / 2;             // words of them
+    constexpr int kStride = HD + 4;        // floats per column of the reduction buffer
+    typedef uint32_t vwords __attribute__((ext_vector_type(VW)));
+    __shared__ float m_lds[kWaves][kCols], l_lds[kWaves][kCols];
+    __shared__ int seen_lds[kCols];
+    __shared__ __align__(16) float o_lds[kWaves][kCols][kStride];
+
+    Item it;
+    const int kvh = a.s.kvh, g = blockIdx.x % kvh, item = blockIdx.x / kvh;
+    if (!find_item<kCols, kKeys>(a, item, a.decode_target, it)) {
+        if (blockIdx.x == gridDim.x - 1) fill_rows(a);   // the grid's last workgroup has no item
+        return;
+    }
+    if (g == 0) write_records(a, it, false);
+    const int group = a.nh / kvh;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, t = lane >> 4;
+    const int block = it.rel % it.blocks, split = it.rel / it.blocks;
+    const int all_cols = columns(a, it.r.rows), c0 = block * kCols;
+    const int cols = all_cols - c0 < kCols ? all_cols - c0 : kCols;
+    const int n = walked(a, it.r.len);
+
+    // This lane's column: row c / group of the request, head c % group; the tokens it sees, and
+    // those that all columns and that any column sees (columns that see none do not count).
+    const int c = c0 + (col < cols ? col : 0);
+    const int row = c / group, head = g * group + c % group;
+    const auto sees = a.range(it.b, it.r.row0, it.r.rows, it.r.len, row);
+    const bool blind = sees.hi == 0;
+    int lo_min = blind ? n : sees.lo, lo_max = blind ? 0 : sees.lo, hi_min = blind ? n : sees.hi, hi_max = sees.hi;
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+        lo_min = min(lo_min, __shfl_xor(lo_min, d));
+        lo_max = max(lo_max, __shfl_xor(lo_max, d));
+        hi_min = min(hi_min, __shfl_xor(hi_min, d));
+        hi_max = max(hi_max, __shfl_xor(hi_max, d));
+    }
+    lo_min = __builtin_amdgcn_readfirstlane(lo_min);
+    lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+    hi_min = __builtin_amdgcn_readfirstlane(hi_min);
+    hi_max = __builtin_amdgcn_readfirstlane(hi_max);
+    int start = it.first + split * it.chunk;
+    const int end = item_end(start, it.chunk, hi_max);
+    if (start < lo_min) start = lo_min / kWaveKeys * kWaveKeys;
+
+    struct Place {                         // of 16 tokens
+        const uint16_t* at;
+        bool there;
+    };
+    auto place = [&](int page, int key) {
+        Place p;
+        p.there = page >= 0 && page < a.s.num_pages;
+        p.at = a.cache + ((int64_t)(p.there ? page : 0) * kvh + g) * a.s.block() + (key & (a.s.page() - 1)) * HD;
+        return p;
+    };
+    u32x4 kw[2][kSteps];                   // token col, columns 32 s + 8 t .. of K
+    vwords vw[2][4];                       // tokens 4 t + r, columns VC col .. of V
+    const uint32_t k_ofs = col * HD + 8 * t, v_ofs = (HD << a.s.page_log2) + 4 * t * HD + VC * col;
+    auto load_k = [&](const Place (&p)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) kw[h][s] = *reinterpret_cast<const u32x4*>(p[h].at + k_ofs + 32 * s);
+    };
+    auto load_v = [&](const Place (&p)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) vw[h][r] = *reinterpret_cast<const vwords*>(p[h].at + v_ofs + r * HD);
+    };
+
+    int key0 = start + kWaveKeys * wave;
+    Pages64 pages = {a.tables + (int64_t)it.b * a.width, 0, 0};
+    pages.fetch(a, key0, n);
+    Place now[2];
+    now[0] = place(pages.page(a, key0, n), key0);
+    now[1] = place(pages.page(a, key0 + 16, n), key0 + 16);
+    if (key0 < end) {
+        load_k(now);
+        load_v(now);
+    }
+
+    u32x4 q[kSteps];
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + row) * a.ld + (int64_t)head * HD + 8 * t;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+    int exp = 0;
+    if constexpr (BF16) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(low16<true>(q[s][i])), fabsf(high16<true>(q[s][i]))));
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)));
+        const float up = __builtin_ldexpf(1.0f, exp);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) q[s] = scaled_bf16(q[s], up);
+    }
+    // Shaped scores are in their own unit, plain ones products of the scaled query:
+    // every exponent is a difference of scores first, so that what they were rounded to on the way is
+    // the same wherever two meet.
+    const float factor = a.factor(), unit = SHAPED ? factor : unit_of(factor, exp);
+    const float natural = unit_of(a.scale, exp), inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const float slope = SHAPED && a.slopes ? a.slopes[head] : 0.0f;
+    const int pos = it.r.len - it.r.rows + row;          // of a row that sees a token: 0 or more
+
+    float m = -INFINITY, l = 0.0f;
+    floatx4 acc[VC];
+#pragma unroll
+    for (int v = 0; v < VC; ++v) acc[v] = floatx4{0.f, 0.f, 0.f, 0.f};
+    while (key0 < end) {
+        const bool more = key0 + kKeys < end;
+        Place next[2];
+        const int key1 = more ? key0 + kKeys : key0;
+        next[0] = place(pages.page(a, key1, n), key1);
+        next[1] = place(pages.page(a, key1 + 16, n), key1 + 16);
+
+        floatx4 s[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            s[h] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) s[h] = mfma16<BF16>(kw[h][st], q[st], s[h]);
+        }
+        if (more) load_k(next);
+        if constexpr (SHAPED) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = s[h][r] * natural;
+                    if (a.softcap > 0.0f) x = capped(x, a.softcap, inv_cap);
+                    s[h][r] = fmaf(-slope, fabsf((float)(pos - (key0 + 16 * h + 4 * t + r))), x);
+                }
+        }
+        const bool gone = !now[0].there || !now[1].there;
+        if (gone || key0 < lo_max || key0 + kWaveKeys > hi_min) {
+            // Some column does not see all of these tokens.  A page outside the cache, or a value that is
+            // not finite: NaN for the rows that see its token, and no product of it for the others.
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int key = key0 + 16 * h + 4 * t + r;
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) most = exponents<BF16>(most, vw[h][r][w]);
+                    const bool odd = !now[h].there || (__ballot(not_finite<BF16>(most)) >> (16 * t) & 0xFFFFu) != 0;
+                    s[h][r] = key < sees.lo || key >= sees.hi ? -INFINITY : odd ? NAN : s[h][r];
+                    if (odd) vw[h][r] = vwords{};
+                }
+        }
+        float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int r = 1; r < 4; ++r) mx = fmaxf(mx, fmaxf(s[0][r], s[1][r]));
+        if (__any((mx - m) * unit > kSlack16)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
+            const float alpha = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : (m - mn) * unit);
+            l *= alpha;
+#pragma unroll
+            for (int v = 0; v < VC; ++v) acc[v] *= alpha;
+            m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;     // nothing yet: every exponential is 0
+        float p[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[4 * h + r] = __builtin_amdgcn_exp2f(fmaf(s[h][r] - ref, unit, kPScale<BF16>));
+                l += p[4 * h + r];
+            }
+        u32x4 phi, plo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            phi[i] = pack2<BF16>(p[2 * i], p[2 * i + 1]);
+            plo[i] = pack2<BF16>(p[2 * i] - low16<BF16>(phi[i]), p[2 * i + 1] - high16<BF16>(phi[i]));
+        }
+#pragma unroll
+        for (int v = 0; v < VC; ++v) {
+            constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;
+            u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                w[i] = __builtin_amdgcn_perm(vw[i >> 1][2 * (i & 1) + 1][v / 2], vw[i >> 1][2 * (i & 1)][v / 2], v & 1 ? kHigh : kLow);
+            acc[v] = mfma16<BF16>(w, plo, acc[v]);
+            acc[v] = mfma16<BF16>(w, phi, acc[v]);
+        }
+        if (more) load_v(next);
+        now[0] = next[0];
+        now[1] = next[1];
+        key0 += kKeys;
+    }
+
+    // This lane: rows 4 t + r of each product, i.e. columns VC (4 t + r) + v of column `col`.
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (t == 0) {
+        m_lds[wave][col] = SHAPED ? m : __builtin_ldexpf(m, -exp);   // of the scores themselves
+        l_lds[wave][col] = l;
+        if (wave == 0) seen_lds[col] = sees.hi;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int v = 0; v < VC; v += 4)
+            *reinterpret_cast<floatx4*>(&o_lds[wave][col][VC * (4 * t + r) + v]) =
+                floatx4{acc[v][r], acc[v + 1][r], acc[v + 2][r], acc[v + 3][r]};
+    __syncthreads();
+    for (int i = threadIdx.x; i < cols * HD; i += kThreads) {
+        const int k = i / HD, d = i - k * HD;
+        float mx = m_lds[0][k];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) mx = fmaxf(mx, m_lds[w][k]);
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        float sum = 0.0f, ls = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float al = __builtin_amdgcn_exp2f((m_lds[w][k] - ref) * factor);
+            sum = fmaf(al, o_lds[w][k][d], sum);
+            ls = fmaf(al, l_lds[w][k], ls);
+        }
+        if (it.splits == 1) {
+            const int cc = c0 + k, r = cc / group, h = g * group + cc % group;
+            const float y = seen_lds[k] == 0 ? 0.0f : sum / ls;
+            reinterpret_cast<uint16_t*>(a.out)[((int64_t)(it.r.row0 + r) * a.nh + h) * HD + d] = to16<BF16>(y);
+        } else {
+            float* dst = a.part + (((int64_t)item * kvh + g) * kCols + k) * (HD + 2);
+            dst[d] = sum;
+            if (d == 0) {
+                dst[HD] = mx;
+                dst[HD + 1] = ls;
+            }
+        }
+    }
+}
+
+// ---- many columns: tiles ---------------------------------------------------------------
+
+// The 16-byte chunks of a token's row in LDS are swizzled by this.  An operand of K is
+// one chunk of 32 tokens, a transposing read of V four neighbouring chunks of four
+// tokens each: both touch every bank once.
+template <int HD>
+__device__ __forceinline__ constexpr int swizzle(int token) {
+    return HD == 128 ? (token & 3) << 2 | (token >> 2 & 3) : (token >> 1 & 1) << 2 | (token >> 2 & 3);
+}
+
+// One workgroup: 128 columns of one kv head, 32 a wave, over an item's tokens in tiles of
+// 64.  K and V go from memory to LDS without passing registers, the next tile's under
+// this one's products: two buffers and one barrier a tile.  V is transposed as it is
+// read (ds_read_b64_tr_b16).
+template <int HD, bool BF16, bool SHAPED>
+__global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs a) {
+    constexpr int kKS = HD / 16;                         // k-steps of S
+    constexpr int kDb = HD / 32;                         // blocks of V's columns
+    constexpr int kChunks = HD / 8;
+    constexpr int kLoads = 16 * HD * 2 / 1024;           // of a wave: 16 tokens of K or V
+    constexpr int kHalf = kTileKeys * HD;                // elements of K or V in a buffer
+    __shared__ __align__(1024) uint16_t buf[2][2 * kHalf];
+    __shared__ __align__(8) uint16_t odd_lds[2][kWaves];
+
+    Item it;
+    const int kvh = a.s.kvh, g = blockIdx.x % kvh, item = blockIdx.x / kvh;
+    if (!find_item<k16Cols, kTileKeys>(a, item, a.tile_target, it)) {
+        if (blockIdx.x == gridDim.x - 1 && a.limit == 0) fill_rows(a);
+        return;
+    }
+    if (g == 0) write_records(a, it, true);
+    const int group = a.nh / kvh;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    // The last blocks, which see the most tokens, start first.
+    const int block = it.blocks - 1 - it.rel % it.blocks, split = it.rel / it.blocks;
+    const int all_cols = columns(a, it.r.rows), c0 = block * k16Cols;
+    const int n = walked(a, it.r.len);
+
+    // Every wave looks at all columns of the workgroup, two a lane: their first and last tokens.
+    int wg_lo = n, wg_lo_max = 0, wg_hi = 0, wg_hi_min = n;
+#pragma unroll
+    for (int i = 0; i < k16Cols; i += 64) {
+        const int c = c0 + i + lane;
+        if (c < all_cols) {
+            const auto r = a.range(it.b, it.r.row0, it.r.rows, it.r.len, c / group);
+            wg_lo = r.hi ? min(wg_lo, r.lo) : wg_lo;
+            wg_lo_max = max(wg_lo_max, r.lo);
+            wg_hi_min = r.hi ? min(wg_hi_min, r.hi) : wg_hi_min;
+            wg_hi = max(wg_hi, r.hi);
+        }
+    }
+    const int local = 32 * wave + col, c = c0 + local, cc = c < all_cols ? c : all_cols - 1;
+    const int row = cc / group, head = g * group + cc % group;
+    const auto sees = a.range(it.b, it.r.row0, it.r.rows, it.r.len, row);
+    const bool blind = sees.hi == 0;
+    int lo_min = blind ? n : sees.lo, lo_max = blind ? 0 : sees.lo, hi_min = blind ? n : sees.hi, hi_max = sees.hi;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        wg_lo = min(wg_lo, __shfl_xor(wg_lo, d));
+        wg_lo_max = max(wg_lo_max, __shfl_xor(wg_lo_max, d));
+        wg_hi_min = min(wg_hi_min, __shfl_xor(wg_hi_min, d));
+        wg_hi = max(wg_hi, __shfl_xor(wg_hi, d));
+        lo_min = min(lo_min, __shfl_xor(lo_min, d));
+        lo_max = max(lo_max, __shfl_xor(lo_max, d));
+        hi_min = min(hi_min, __shfl_xor(hi_min, d));
+        hi_max = max(hi_max, __shfl_xor(hi_max, d));
+    }
+    wg_lo = __builtin_amdgcn_readfirstlane(wg_lo);
+    wg_lo_max = __builtin_amdgcn_readfirstlane(wg_lo_max);
+    wg_hi_min = __builtin_amdgcn_readfirstlane(wg_hi_min);
+    wg_hi = __builtin_amdgcn_readfirstlane(wg_hi);
+    lo_min = __builtin_amdgcn_readfirstlane(lo_min);
+    lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+    hi_min = __builtin_amdgcn_readfirstlane(hi_min);
+    hi_max = __builtin_amdgcn_readfirstlane(hi_max);
+    int start = it.first + split * it.chunk;
+    const int end = item_end(start, it.chunk, wg_hi);
+    if (start < wg_lo) start = wg_lo / kTileKeys * kTileKeys;
+    const int tiles = end > start ? (end - start + kTileKeys - 1) / kTileKeys : 0;
+
+    // Loads: wave w brings tokens 16 w .. of the tile.  A place past the
+    // last token, or in a page outside the cache, lies past its resource's end and reads as zeros.
+    Pages64 window = {a.tables + (int64_t)it.b * a.width, 0, 0};
+    window.fetch(a, start, n);
+    const int r0 = lane / kChunks;                       // a load's rows begin with this lane's token
+    const uint32_t l_ofs = r0 * (HD * 2) + ((lane % kChunks) ^ swizzle<HD>(r0)) * 16;
+    const uint32_t lds0 = lds_addr(&buf[0][0]) + wave * (16 * HD * 2);
+    // Which of a tile's blocks of 16 tokens lie in pages outside the cache: a bit each.
+    auto issue = [&](int key0, int stage) {
+        uint32_t gone = 0;
+        int mine = -1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int page = window.page(a, key0 + 16 * j, n);
+            const bool there = page >= 0 && page < a.s.num_pages;
+            if (!there) gone |= 1u << j;
+            if (j == wave) mine = there ? page : -1;
+        }
+        const int key = key0 + 16 * wave, left = n - key;
+        const uint32_t bytes = mine < 0 || left <= 0 ? 0u : (uint32_t)(left < 16 ? left : 16) * (HD * 2);
+        const uint16_t* at = a.cache + ((int64_t)(mine < 0 ? 0 : mine) * kvh + g) * a.s.block() + (key & (a.s.page() - 1)) * HD;
+        const u32x4 rk = raw_rsrc(at, bytes), rv = raw_rsrc(at + (HD << a.s.page_log2), bytes);
+        const uint32_t to = lds0 + stage * (4 * kHalf);
+        constexpr uint32_t kFlip = HD == 128 ? 16 : 32;  // the swizzle of the tokens of a load after
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) buffer_load_lds_x4(rk, (l_ofs ^ (kFlip * i)) + 1024 * i, 0, to + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) buffer_load_lds_x4(rv, (l_ofs ^ (kFlip * i)) + 1024 * i, 0, to + 2 * kHalf + 1024 * i);
+        return gone;
+    };
+    uint32_t gone_next = tiles > 0 ? issue(start, 0) : 0;
+
+    // This lane's query: columns 16 s + 8 half .. of the head.
+    u32x4 q[kKS];
+    int exp = 0;
+    {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + row) * a.ld + (int64_t)head * HD + 8 * half;
+#pragma unroll
+        for (int s = 0; s < kKS; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s);
+        if constexpr (BF16) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kKS; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(low16<true>(q[s][i])), fabsf(high16<true>(q[s][i]))));
+            exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)));
+            const float up = __builtin_ldexpf(1.0f, exp);
+#pragma unroll
+            for (int s = 0; s < kKS; ++s) q[s] = scaled_bf16(q[s], up);
+        }
+    }
+    const float factor = a.factor(), unit = SHAPED ? factor : unit_of(factor, exp);
+    const float natural = unit_of(a.scale, exp), inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const float slope = SHAPED && a.slopes ? a.slopes[head] : 0.0f;
+    const int pos = it.r.len - it.r.rows + row;
+
+    // Operand addresses in bytes: token col (+ 32) and chunk 2 s + half of K; of V, lane 4 m + j of
+    // 16 supplies four columns of token 4 half + m, and its group's other half of the 32 columns.
+    const uint32_t k_at = col * (HD * 2) + (half ^ swizzle<HD>(col)) * 16;
+    const int vm = 4 * half + (lane >> 2 & 3), vj = lane & 3;
+    const uint32_t v_at = 2 * kHalf + vm * (HD * 2) + ((2 * (lane >> 4 & 1) + (vj >> 1)) ^ swizzle<HD>(vm)) * 16 + (vj & 1) * 8;
+
+    float m = -INFINITY, l = 0.0f;
+    floatx16 acc[kDb];
+#pragma unroll
+    for (int d = 0; d < kDb; ++d) acc[d] = floatx16{};
+    for (int tile = 0; tile < tiles; ++tile) {
+        const int key0 = start + tile * kTileKeys;
+        const uint32_t gone = gone_next;
+        char* base = reinterpret_cast<char*>(&buf[tile & 1][0]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // Where some column does not see all of the tile's tokens, a value of V that is not finite must
+        // not meet its probability of zero: each wave takes such values out of the tokens it
+        // brought, and the rows that see them get NaN by their scores.
+        const bool edge = key0 < wg_lo_max || key0 + kTileKeys > wg_hi_min;
+        if (edge) {
+            constexpr int kRows = 1024 / (HD * 2);       // tokens of a read
+            uint32_t odd = 0;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                u32x4* at = reinterpret_cast<u32x4*>(base + 2 * kHalf + wave * (16 * HD * 2) + 1024 * i + 16 * lane);
+                u32x4 w = *at;
+                uint32_t most = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) most = exponents<BF16>(most, w[j]);
+                const uint64_t hit = __ballot(not_finite<BF16>(most));
+                if (hit) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = finite_part<BF16>(w[j]);
+                    *at = w;
+#pragma unroll
+                    for (int j = 0; j < kRows; ++j)
+                        if (hit >> (kChunks * j) & ((1u << kChunks) - 1)) odd |= 1u << (kRows * i + j);
+                }
+            }
+            if (lane == 0) odd_lds[tile & 1][wave] = (uint16_t)odd;
+        }
+        lds_barrier();                                   // the tile is there, and the other buffer read by all
+        if (tile + 1 < tiles) gone_next = issue(key0 + kTileKeys, (tile + 1) & 1);
+        if (key0 >= hi_max || key0 + kTileKeys <= lo_min) continue;   // nothing for this wave
+        uint64_t bad = 0;                                // tokens that give NaN, a bit each
+        if (edge) {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(&odd_lds[tile & 1][0]);
+            bad = (uint64_t)__builtin_amdgcn_readfirstlane(w.y) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane(w.x);
+        }
+        if (gone) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (gone >> j & 1) bad |= 0xFFFFull << (16 * j);
+        }
+
+        floatx16 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            s[b] = floatx16{};
+#pragma unroll
+            for (int st = 0; st < kKS; ++st)
+                s[b] = mfma32<BF16>(*reinterpret_cast<const u32x4*>(base + (k_at ^ (32 * st)) + b * (32 * HD * 2)), q[st], s[b]);
+        }
+        if constexpr (SHAPED) {
+            const float far = (float)(pos - key0 - 4 * half);
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float x = s[b][i] * natural;
+                    if (a.softcap > 0.0f) x = capped(x, a.softcap, inv_cap);
+                    s[b][i] = fmaf(-slope, fabsf(far - (float)(32 * b + 8 * (i / 4) + i % 4)), x);
+                    if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // few at a time: registers
+                }
+        }
+        if (bad || key0 < lo_max || key0 + kTileKeys > hi_min) {
+            const uint64_t mine = bad >> (4 * half);
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int in = 32 * b + 8 * (i / 4) + i % 4, key = key0 + in + 4 * half;
+                    s[b][i] = key < sees.lo || key >= sees.hi ? -INFINITY : mine >> in & 1 ? NAN : s[b][i];
+                }
+        }
+        float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+        if (__any((mx - m) * unit > kSlack16)) {
+            const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
+            const float alpha = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : (m - mn) * unit);
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < kDb; ++d) acc[d] *= alpha;
+            m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;     // nothing yet: every exponential is 0
+        u32x4 p[4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i] - ref, unit, kPScale<BF16>));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1] - ref, unit, kPScale<BF16>));
+                l += x;
+                l += y;
+                p[2 * b + i / 8][i % 8 / 2] = pack2<BF16>(x, y);
+            }
+        typedef __attribute__((address_space(3))) s16x4* lds4;
+#pragma unroll
+        for (int d = 0; d < kDb; ++d)
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                char* at = base + 16 * st * (HD * 2);
+                const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + (v_at ^ (64 * d)))));
+                const u32x2 y = __builtin_bit_cast(
+                    u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + (v_at ^ (64 * d) ^ 32) + 8 * (HD * 2))));
+                acc[d] = mfma32<BF16>(u32x4{x.x, x.y, y.x, y.y}, p[st], acc[d]);
+            }
+    }
+
+    l += __shfl_xor(l, 32);
+    if (c >= all_cols) return;
+    // This lane: columns 32 d + 8 j + 4 half + r of the head.
+    if (it.splits == 1) {
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + ((int64_t)(it.r.row0 + row) * a.nh + head) * HD + 4 * half;
+#pragma unroll
+        for (int d = 0; d < kDb; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float y[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = blind ? 0.0f : acc[d][4 * j + r] / l;
+                *reinterpret_cast<u32x2*>(dst + 32 * d + 8 * j) = u32x2{pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3])};
+            }
+    } else {
+        float* dst = a.tile_part + (((int64_t)item * kvh + g) * k16Cols + local) * (HD + 2);
+#pragma unroll
+        for (int d = 0; d < kDb; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2)
+                    *reinterpret_cast<float2*>(dst + 32 * d + 8 * j + 4 * half + r) = float2{acc[d][4 * j + r], acc[d][4 * j + r + 1]};
+        if (half == 0) {
+            dst[HD] = SHAPED ? m : __builtin_ldexpf(m, -exp);
+            dst[HD + 1] = l;
+        }
+    }
+}
+
+// ---- joining the items of a row -----------------------------------------------------
+
+template <int HD, int WAVES, bool BF16>
+__global__ __launch_bounds__(kThreads) void awq_kv16_combine_kernel(Kv16AttnArgs a) {
+    combine_items<HD, WAVES, BF16>(a);
+}
+
+// ---- launches ----------------------------------------------------------------------------
+
+template <int HD, bool BF16, bool SHAPED>
+hipError_t launch(Kv16AttnArgs a, hipStream_t stream) {
+    const AttentionPlan p = attention_plan<k16Cols>(a.requests, a.total, a.max_query, a.nh / a.s.kvh, a.s.kvh);
+    a.limit = p.limit;
+    a.decode_target = p.decode_target;
+    a.tile_target = p.tile_target;
+    a.records = reinterpret_cast<i32x4*>(a.part);
+    a.part += (size_t)a.total * (sizeof(i32x4) / sizeof(float));
+    a.tile_part = a.part + p.decode_items * a.s.kvh * kCols * (HD + 2);
+    if (p.decode) {
+        hipLaunchKernelGGL((awq_kv16_decode_kernel<HD, BF16, SHAPED>), dim3((unsigned)(p.decode_items * a.s.kvh)), dim3(kThreads), 0,
+                           stream, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (p.tile) {
+        hipLaunchKernelGGL((awq_kv16_tile_kernel<HD, BF16, SHAPED>), dim3((unsigned)(p.tile_items * a.s.kvh)), dim3(kThreads), 0, stream,
+                           a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (p.combine) {
+        const int64_t all = (int64_t)a.total * a.nh, groups = all <= kFewUnits ? all : (all + 3) / 4;
+        auto kernel = all <= kFewUnits ? awq_kv16_combine_kernel<HD, 4, BF16> : awq_kv16_combine_kernel<HD, 1, BF16>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < kCombineGroups ? groups : kCombineGroups)), dim3(kThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    return hipSuccess;
+}
+
+}  // namespace
+
+// A launch holds 2^32 threads.
+bool kv16_attn_fits(int requests, int total, int max_query, int nh, int kvh) {
+    const AttentionPlan p = attention_plan<k16Cols>(requests, total, max_query, nh / kvh, kvh);
+    return (p.decode_items > p.tile_items ? p.decode_items : p.tile_items) * kvh < ((int64_t)1 << 32) / kThreads;
+}
+
+size_t kv16_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd) {
+    return part_bytes(attention_plan<k16Cols>(requests, total, max_query, nh / kvh, kvh), total, kvh, hd);
+}
+
+hipError_t launch_kv16_attention(const Kv16AttnArgs& a, bool bf16, hipStream_t stream) {
+    auto typed = [&](auto hd, auto type) {
+        return a.shaped() ? launch<hd(), type(), true>(a, stream) : launch<hd(), type(), false>(a, stream);
+    };
+    constexpr std::integral_constant<int, 64> c64;
+    constexpr std::integral_constant<int, 128> c128;
+    if (a.s.hd == 64) return bf16 ? typed(c64, std::true_type{}) : typed(c64, std::false_type{});
+    return bf16 ? typed(c128, std::true_type{}) : typed(c128, std::false_type{});
+}
+
+}  // namespace awq

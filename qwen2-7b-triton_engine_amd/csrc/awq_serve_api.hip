@@ -43,6 +43,15 @@ int check_cache(int64_t kvh, int64_t hd, int64_t num_pages, int64_t page_size, i
     return AWQ_OK;
 }
 
+int check_cache16(int64_t kvh, int64_t hd, int64_t num_pages, int64_t page_size, int32_t dtype, Kv16Shape* s) {
+    if (kvh <= 0 || num_pages <= 0) return AWQ_ERR_BAD_DIMS;
+    if ((hd != 64 && hd != 128) || log2_page(page_size) < 0 || (dtype != AWQ_SERVE_FP16 && dtype != AWQ_SERVE_BF16))
+        return AWQ_ERR_PATH;
+    if (kvh > 4096 || num_pages > kIndexLimit / page_size) return AWQ_ERR_TOO_LARGE;
+    *s = Kv16Shape{(int)kvh, (int)hd, log2_page(page_size), (int)num_pages};
+    return AWQ_OK;
+}
+
 int check_step(const PageStepArgs& a, int64_t requests, int64_t width, int64_t capacity, int64_t page_size) {
     const int st = check_pages(requests, width, capacity, page_size);
     if (st != AWQ_OK) return st;
@@ -208,6 +217,91 @@ int awq_serve_kv4_attention(const void* q, int64_t q_stride, const void* cache, 
     a.width = (int)table_width;
     a.scale = scale;
     return done(launch_kv4_attention(a, dtype == AWQ_SERVE_BF16, static_cast<hipStream_t>(stream)));
+}
+
+int awq_serve_kv16_append(const void* qkv, int64_t qkv_stride, void* cache, const int32_t* slots,
+                          const int32_t* positions, const void* cos, const void* sin, void* q_out, int64_t tokens,
+                          int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t num_pages,
+                          int64_t page_size, int64_t max_pos, int32_t dtype, void* stream) {
+    Kv16AppendArgs a;
+    const int st = check_cache16(num_kv_heads, head_dim, num_pages, page_size, dtype, &a.s);
+    if (st != AWQ_OK) return st;
+    if (tokens < 0 || num_heads <= 0 || max_pos <= 0 || qkv_stride < (num_heads + 2 * num_kv_heads) * head_dim)
+        return AWQ_ERR_BAD_DIMS;
+    if (num_heads > 4096 || max_pos > kIndexLimit || tokens > kIndexLimit / ((num_heads + 2 * num_kv_heads) * 16))
+        return AWQ_ERR_TOO_LARGE;
+    if (tokens == 0) return AWQ_OK;
+    if (!qkv || !cache || !slots || !positions || !q_out || !cos != !sin) return AWQ_ERR_NULL_POINTER;
+    if (!aligned(qkv, 16) || qkv_stride % 8 != 0 || !aligned(cache, 16) || !aligned(slots, 4) ||
+        !aligned(positions, 4) || !aligned(cos, 16) || !aligned(sin, 16) || !aligned(q_out, 16))
+        return AWQ_ERR_MISALIGNED;
+    a.qkv = qkv;
+    a.ld = qkv_stride;
+    a.cache = static_cast<uint16_t*>(cache);
+    a.slots = slots;
+    a.positions = positions;
+    a.cos = static_cast<const float*>(cos);
+    a.sin = static_cast<const float*>(sin);
+    a.q = q_out;
+    a.tokens = (int)tokens;
+    a.nh = (int)num_heads;
+    a.max_pos = (int)max_pos;
+    return done(launch_kv16_append(a, dtype == AWQ_SERVE_BF16, static_cast<hipStream_t>(stream)));
+}
+
+size_t awq_serve_kv16_attention_workspace(int64_t requests, int64_t total, int64_t max_query, int64_t num_heads,
+                                          int64_t num_kv_heads, int64_t head_dim, int64_t table_width,
+                                          int64_t page_size) {
+    if (check_attention(requests, total, max_query, num_heads, num_kv_heads, head_dim, table_width, page_size) != AWQ_OK)
+        return 0;
+    if (!kv16_attn_fits((int)requests, (int)total, (int)max_query, (int)num_heads, (int)num_kv_heads)) return 0;
+    return kv16_attn_workspace((int)requests, (int)total, (int)max_query, (int)num_heads, (int)num_kv_heads, (int)head_dim);
+}
+
+int awq_serve_kv16_attention(const void* q, int64_t q_stride, const void* cache, const int32_t* block_tables,
+                             const int32_t* seq_lens, const int32_t* query_start, const float* slopes,
+                             const int32_t* prefix, const int32_t* first, void* out, int64_t requests, int64_t total,
+                             int64_t max_query, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                             int64_t table_width, int64_t num_pages, int64_t page_size, int64_t window, float scale,
+                             float softcap, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    Kv16AttnArgs a = {};
+    int st = check_cache16(num_kv_heads, head_dim, num_pages, page_size, dtype, &a.s);
+    if (st != AWQ_OK) return st;
+    st = check_attention(requests, total, max_query, num_heads, num_kv_heads, head_dim, table_width, page_size);
+    if (st != AWQ_OK) return st;
+    if (q_stride < num_heads * head_dim || !(scale > 0.0f) || !(scale < HUGE_VALF) || window < 0 ||
+        !(softcap == 0.0f || (softcap >= 0x1p-100f && softcap < HUGE_VALF)))
+        return AWQ_ERR_BAD_DIMS;
+    if (!kv16_attn_fits((int)requests, (int)total, (int)max_query, (int)num_heads, (int)num_kv_heads)) return AWQ_ERR_TOO_LARGE;
+    if (total == 0) return AWQ_OK;
+    if (!q || !cache || !block_tables || !seq_lens || !query_start || !out) return AWQ_ERR_NULL_POINTER;
+    if (!aligned(q, 16) || q_stride % 8 != 0 || !aligned(cache, 16) || !aligned(block_tables, 4) ||
+        !aligned(seq_lens, 4) || !aligned(query_start, 4) || !aligned(slopes, 4) || !aligned(prefix, 4) ||
+        !aligned(first, 4) || !aligned(out, 16) || !aligned(workspace, 16))
+        return AWQ_ERR_MISALIGNED;
+    if (!workspace || workspace_bytes < kv16_attn_workspace((int)requests, (int)total, (int)max_query, (int)num_heads,
+                                                            (int)num_kv_heads, (int)head_dim))
+        return AWQ_ERR_WORKSPACE;
+    a.q = q;
+    a.ld = q_stride;
+    a.cache = static_cast<const uint16_t*>(cache);
+    a.tables = block_tables;
+    a.seq_lens = seq_lens;
+    a.query_start = query_start;
+    a.slopes = slopes;
+    a.prefix = prefix;
+    a.first = first;
+    a.part = static_cast<float*>(workspace);
+    a.out = out;
+    a.requests = (int)requests;
+    a.total = (int)total;
+    a.max_query = (int)max_query;
+    a.nh = (int)num_heads;
+    a.width = (int)table_width;
+    a.window = window < kIndexLimit ? (int)window : 0;   // more than any position: none
+    a.scale = scale;
+    a.softcap = softcap;
+    return done(launch_kv16_attention(a, dtype == AWQ_SERVE_BF16, static_cast<hipStream_t>(stream)));
 }
 
 size_t awq_serve_logits_workspace(int64_t rows, int64_t vocab) {

@@ -83,14 +83,16 @@ constexpr int item_end(int start, int chunk, int limit) {
 
 struct AttentionPlan {
     bool decode, tile, combine;
-    int limit, decode_target, tile_target;
+    int limit, decode_target, tile_target, tile_cols;
     int64_t decode_items, tile_items;  // at most, of one kv head
     size_t part_floats(int kvh, int hd) const {          // the items' sums
-        return (size_t)(decode_items * kCols + (tile_target ? tile_items * kTileCols : 0)) * kvh * (hd + 2);
+        return (size_t)(decode_items * kCols + (tile_target ? tile_items * tile_cols : 0)) * kvh * (hd + 2);
     }
 };
-inline AttentionPlan attention_plan(int requests, int total, int max_query, int group, int kvh) {
+template <int TILE_COLS = kTileCols>
+AttentionPlan attention_plan(int requests, int total, int max_query, int group, int kvh) {
     AttentionPlan p = {};
+    p.tile_cols = TILE_COLS;
     const int64_t rows = (int64_t)requests * max_query < total ? (int64_t)requests * max_query : total;
     p.tile = (int64_t)max_query * group > kDecodeColumns;
     p.decode = !p.tile || requests > 1;
@@ -102,7 +104,7 @@ inline AttentionPlan attention_plan(int requests, int total, int max_query, int 
         p.decode_items = p.decode_target + (p.tile && most < blocks ? most : blocks) + 1;
     }
     if (p.tile) {
-        const int64_t blocks = requests + rows * group / kTileCols;
+        const int64_t blocks = requests + rows * group / TILE_COLS;
         p.tile_target = blocks * kvh < kSplitBelow ? (kvh < kTileItems ? kTileItems / kvh : 1) : 0;
         p.tile_items = blocks + p.tile_target + 1;
     }

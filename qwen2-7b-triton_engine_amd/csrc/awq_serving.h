@@ -4,6 +4,7 @@
 
 #include "../../include/awq_serving.h"
 #include "awq_kernels.h"
+#include "awq_serve_items.h"
 
 namespace awq {
 
@@ -64,9 +65,91 @@ struct Kv4AttnArgs {
     i32x4* records;             // [total]: what the combining launch has to know of a row
     int limit;                  // columns up to which a request is the decode kernel's
     int decode_target, tile_target;   // items of one kv head that the kernels aim at
+    // what awq_serve_walk.h asks for
+    static constexpr int kTileCols = 64;
+    __device__ __forceinline__ int first_key(int, int) const { return 0; }
+    __device__ __forceinline__ bool sees_none(int, int, int rows, int len, int i) const { return (int64_t)len - rows + i < 0; }
+    __device__ __forceinline__ float factor() const { return scale * 1.4426950408889634f; }
 };
 size_t kv4_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd);
 hipError_t launch_kv4_attention(const Kv4AttnArgs& a, bool bf16, hipStream_t stream);
+
+// One layer's 16-bit cache: [num_pages][kvh][K, V][page][hd].
+struct Kv16Shape {
+    int kvh, hd, page_log2, num_pages;
+    __host__ __device__ int page() const { return 1 << page_log2; }
+    __host__ __device__ int64_t block() const { return (int64_t)(hd * 2) << page_log2; }   // elements of a page and head
+};
+
+struct Kv16AppendArgs {
+    const void* qkv;            // [tokens, ...], ld elements from row to row
+    int64_t ld;
+    uint16_t* cache;
+    const int32_t *slots, *positions;
+    const float *cos, *sin;     // [max_pos, hd], or null: no rotation
+    void* q;                    // [tokens, nh * hd]
+    int tokens, nh, max_pos;
+    Kv16Shape s;
+};
+hipError_t launch_kv16_append(const Kv16AppendArgs& a, bool bf16, hipStream_t stream);
+
+struct Kv16AttnArgs {
+    const void* q;              // [total, nh * hd], ld elements from row to row
+    int64_t ld;
+    const uint16_t* cache;
+    const int32_t *tables, *seq_lens, *query_start;
+    const float* slopes;        // [nh], or null
+    const int32_t* prefix;      // [requests], or null
+    const int32_t* first;       // [total], or null
+    float* part;
+    void* out;                  // [total, nh * hd]
+    int requests, total, max_query, nh, width;
+    int window;                 // tokens that a row sees back from itself, 0: all
+    float scale, softcap;       // softcap 0: none
+    Kv16Shape s;
+    // set by the launch
+    float* tile_part;
+    i32x4* records;             // [total]
+    int limit, decode_target, tile_target;
+    // what awq_serve_walk.h asks for
+    static constexpr int kTileCols = 128;
+    __device__ __forceinline__ int first_key(int rows, int len) const {
+        if (window == 0) return 0;
+        const int64_t lo = (int64_t)len - rows - window + 1;
+        const int n = walked_tokens(width, s.page_log2, len);
+        return lo <= 0 || n == 0 ? 0 : lo < n ? (int)lo : n - 1;
+    }
+    // Tokens lo .. hi - 1 that the i-th row of request b sees; none: 0 and 0.  Of a table
+    // that is too short its first missing token is the last one: it gives NaN.
+    struct Range {
+        int lo, hi;
+    };
+    __device__ __forceinline__ Range range(int b, int row0, int rows, int len, int i) const {
+        const int64_t pos = (int64_t)len - rows + i;
+        int64_t lo = window ? pos - window + 1 : 0, hi = pos + 1;
+        if (prefix) {
+            const int p = prefix[b];
+            hi = hi > p ? hi : p < len ? p : len;
+        }
+        if (first) {
+            const int f = first[row0 + i];
+            lo = lo > f ? lo : f;
+        }
+        lo = lo > 0 ? lo : 0;
+        if (pos < 0 || lo >= hi) return Range{0, 0};
+        const int n = walked_tokens(width, s.page_log2, len);
+        return Range{lo < n ? (int)lo : n - 1, hi < n ? (int)hi : n};
+    }
+    __device__ __forceinline__ bool sees_none(int b, int row0, int rows, int len, int i) const {
+        return range(b, row0, rows, len, i).hi == 0;
+    }
+    // Scores that are capped or carry a bias are scaled before, plain ones after their differences.
+    __host__ __device__ bool shaped() const { return softcap > 0.0f || slopes; }
+    __device__ __forceinline__ float factor() const { return (shaped() ? 1.0f : scale) * 1.4426950408889634f; }
+};
+bool kv16_attn_fits(int requests, int total, int max_query, int nh, int kvh);
+size_t kv16_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd);
+hipError_t launch_kv16_attention(const Kv16AttnArgs& a, bool bf16, hipStream_t stream);
 
 struct LogitsArgs {
     const void* logits;

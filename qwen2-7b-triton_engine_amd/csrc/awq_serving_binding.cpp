@@ -140,6 +140,21 @@ Tensor paged_release(const Tensor& state, const Tensor& keep, const Tensor& bloc
     return out;
 }
 
+// RoPE's tables, both or neither, aligned; their positions (no table: any).
+int64_t check_rope(const OptTensor& cos_in, const OptTensor& sin_in, int64_t head_dim, const at::Device& device, Tensor& cos,
+                   Tensor& sin) {
+    TORCH_CHECK_VALUE(cos_in.has_value() == sin_in.has_value(), "cos and sin come together");
+    if (!cos_in.has_value()) return kIntMax;
+    const int64_t max_pos = cos_in->dim() == 2 ? cos_in->size(0) : 0;
+    for (const Tensor* t : {&*cos_in, &*sin_in})
+        TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == max_pos && max_pos > 0 &&
+                              t->size(1) == head_dim && t->is_contiguous() && t->device() == device,
+                          "cos and sin must be contiguous float32 tensors [max_pos, ", head_dim, "] on ", device);
+    cos = aligned16(*cos_in);
+    sin = aligned16(*sin_in);
+    return max_pos;
+}
+
 Tensor kv4_append(const Tensor& qkv_in, const Tensor& data, int64_t head_dim, int64_t page_size, int64_t group_size,
                   const Tensor& slots, const Tensor& positions, const OptTensor& cos_in, const OptTensor& sin_in,
                   int64_t num_heads) {
@@ -156,19 +171,9 @@ Tensor kv4_append(const Tensor& qkv_in, const Tensor& data, int64_t head_dim, in
     const int64_t T = qkv_in.size(0);
     check_i32(slots, "slots", {T}, device);
     check_i32(positions, "positions", {T}, device);
-    TORCH_CHECK_VALUE(cos_in.has_value() == sin_in.has_value(), "cos and sin come together");
     const at::DeviceGuard guard(device);
     Tensor cos, sin;
-    int64_t max_pos = kIntMax;
-    if (cos_in.has_value()) {
-        max_pos = cos_in->dim() == 2 ? cos_in->size(0) : 0;
-        for (const Tensor* t : {&*cos_in, &*sin_in})
-            TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == max_pos && max_pos > 0 &&
-                                  t->size(1) == head_dim && t->is_contiguous() && t->device() == device,
-                              "cos and sin must be contiguous float32 tensors [max_pos, ", head_dim, "] on ", device);
-        cos = aligned16(*cos_in);
-        sin = aligned16(*sin_in);
-    }
+    const int64_t max_pos = check_rope(cos_in, sin_in, head_dim, device, cos, sin);
     const Tensor qkv = rows16(qkv_in);
     Tensor q = at::empty({T, num_heads * head_dim}, qkv.options());
     check_status(awq_serve_kv4_append(qkv.data_ptr(), row_stride(qkv), data.data_ptr(), i32(slots), i32(positions),
@@ -198,15 +203,16 @@ std::tuple<Tensor, Tensor> kv4_gather(const Tensor& data, int64_t head_dim, int6
     return {k, v};
 }
 
-Tensor kv4_attention(const Tensor& q_in, const Tensor& data, int64_t head_dim, int64_t page_size, int64_t group_size,
-                     const Tensor& block_tables, const Tensor& seq_lens, const Tensor& query_start, int64_t max_query,
-                     c10::optional<double> scale_in) {
-    const Plain plain;
-    check_cache(data, head_dim, page_size, group_size);
-    const Cache cache{data, head_dim, page_size, group_size};
+// What the attention calls have in common: sizes, checked.
+struct AttentionCall {
+    at::Device device;
+    int64_t heads, requests, width, rows, most;
+    float scale;
+};
+AttentionCall check_attention(const Tensor& q_in, const Tensor& data, int64_t kvh, int64_t head_dim, int64_t page_size,
+                              const Tensor& block_tables, const Tensor& seq_lens, const Tensor& query_start, int64_t max_query,
+                              c10::optional<double> scale_in) {
     const at::Device device = q_in.device();
-    const int64_t kvh = cache.heads();
-    const int dtype = type16(q_in, "q");
     TORCH_CHECK_VALUE(q_in.dim() == 2 && q_in.size(1) > 0 && q_in.size(1) % (head_dim * kvh) == 0, "q must be a tensor [T, heads * ",
                       head_dim, "] with heads a multiple of ", kvh, ", got ", q_in.sizes());
     const int64_t heads = q_in.size(1) / head_dim;
@@ -229,6 +235,21 @@ Tensor kv4_attention(const Tensor& q_in, const Tensor& data, int64_t head_dim, i
                       " must be positive and finite");
     const int64_t T = q_in.size(0);
     const int64_t most = std::min(max_query, std::max<int64_t>(T, 1));
+    return {device, heads, requests, width, T, most, (float)scale};
+}
+
+Tensor kv4_attention(const Tensor& q_in, const Tensor& data, int64_t head_dim, int64_t page_size, int64_t group_size,
+                     const Tensor& block_tables, const Tensor& seq_lens, const Tensor& query_start, int64_t max_query,
+                     c10::optional<double> scale_in) {
+    const Plain plain;
+    check_cache(data, head_dim, page_size, group_size);
+    const Cache cache{data, head_dim, page_size, group_size};
+    const at::Device device = q_in.device();
+    const int64_t kvh = cache.heads();
+    const int dtype = type16(q_in, "q");
+    const AttentionCall c =
+        check_attention(q_in, data, kvh, head_dim, page_size, block_tables, seq_lens, query_start, max_query, scale_in);
+    const int64_t heads = c.heads, requests = c.requests, width = c.width, T = c.rows, most = c.most;
     const at::DeviceGuard guard(device);
     const Tensor q = rows16(q_in);
     Tensor out = at::empty({T, heads * head_dim}, q.options());
@@ -237,9 +258,100 @@ Tensor kv4_attention(const Tensor& q_in, const Tensor& data, int64_t head_dim, i
     const Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
     check_status(awq_serve_kv4_attention(q.data_ptr(), row_stride(q), data.data_ptr(), i32(block_tables), i32(seq_lens),
                                          i32(query_start), out.data_ptr(), requests, T, most, heads, kvh, head_dim, width,
-                                         cache.pages(), page_size, group_size, (float)scale, dtype, ws.data_ptr(), bytes,
+                                         cache.pages(), page_size, group_size, c.scale, dtype, ws.data_ptr(), bytes,
                                          stream_of(device)),
                  "awq_serve_kv4_attention");
+    return out;
+}
+
+// A 16-bit cache as kernels/kv16.py holds it.
+void check_cache16(const Tensor& data) {
+    TORCH_CHECK_VALUE((data.scalar_type() == at::kHalf || data.scalar_type() == at::kBFloat16) && data.dim() == 5 && data.size(2) == 2 &&
+                          data.is_contiguous(),
+                      "data must be a contiguous fp16 or bf16 tensor [pages, kv heads, 2, page_size, head_dim], got ",
+                      data.scalar_type(), " ", data.sizes());
+    const int64_t page_size = data.size(3), head_dim = data.size(4);
+    TORCH_CHECK_VALUE(head_dim == 64 || head_dim == 128, "head_dim ", head_dim, " must be 64 or 128");
+    TORCH_CHECK_VALUE(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128 || page_size == 256, "page_size ",
+                      page_size, " must be 16, 32, 64, 128 or 256");
+    TORCH_CHECK_VALUE(data.size(0) >= 1 && data.size(1) >= 1 && (reinterpret_cast<uintptr_t>(data.data_ptr()) & 15u) == 0,
+                      "data must hold a page and a head and start on 16 bytes");
+    TORCH_CHECK_VALUE(data.size(0) <= kIntMax / page_size, "slot numbers pass 32 bits");
+}
+
+Tensor kv16_append(const Tensor& qkv_in, const Tensor& data, const Tensor& slots, const Tensor& positions,
+                   const OptTensor& cos_in, const OptTensor& sin_in, int64_t num_heads) {
+    const Plain plain;
+    check_cache16(data);
+    const at::Device device = qkv_in.device();
+    const int64_t kvh = data.size(1), head_dim = data.size(4), columns = (num_heads + 2 * kvh) * head_dim;
+    const int dtype = type16(qkv_in, "qkv");
+    TORCH_CHECK_VALUE(qkv_in.scalar_type() == data.scalar_type(), "qkv and the cache must be of one type, got ",
+                      qkv_in.scalar_type(), " and ", data.scalar_type());
+    TORCH_CHECK_VALUE(qkv_in.dim() == 2 && qkv_in.size(1) == columns && num_heads >= 1, "qkv must be a tensor [T, ", columns,
+                      "], got ", qkv_in.sizes());
+    check_on_gpu(qkv_in, "qkv");
+    TORCH_CHECK_VALUE(data.device() == device, "qkv and the cache must be on one device, got ", device, " and ", data.device());
+    const int64_t T = qkv_in.size(0);
+    check_i32(slots, "slots", {T}, device);
+    check_i32(positions, "positions", {T}, device);
+    const at::DeviceGuard guard(device);
+    Tensor cos, sin;
+    const int64_t max_pos = check_rope(cos_in, sin_in, head_dim, device, cos, sin);
+    const Tensor qkv = rows16(qkv_in);
+    Tensor q = at::empty({T, num_heads * head_dim}, qkv.options());
+    check_status(awq_serve_kv16_append(qkv.data_ptr(), row_stride(qkv), data.data_ptr(), i32(slots), i32(positions),
+                                       cos.defined() ? cos.data_ptr() : nullptr, sin.defined() ? sin.data_ptr() : nullptr,
+                                       q.data_ptr(), T, num_heads, kvh, head_dim, data.size(0), data.size(3), max_pos, dtype,
+                                       stream_of(device)),
+                 "awq_serve_kv16_append");
+    return q;
+}
+
+Tensor kv16_attention(const Tensor& q_in, const Tensor& data, const Tensor& block_tables, const Tensor& seq_lens,
+                      const Tensor& query_start, int64_t max_query, c10::optional<double> scale_in,
+                      c10::optional<double> softcap_in, const OptTensor& slopes, c10::optional<int64_t> window_in,
+                      const OptTensor& prefix, const OptTensor& first) {
+    const Plain plain;
+    check_cache16(data);
+    const int64_t head_dim = data.size(4), page_size = data.size(3);
+    TORCH_CHECK_VALUE(q_in.scalar_type() == data.scalar_type(), "q and the cache must be of one type, got ", q_in.scalar_type(),
+                      " and ", data.scalar_type());
+    const AttentionCall c = check_attention(q_in, data, data.size(1), head_dim, page_size, block_tables, seq_lens, query_start,
+                                            max_query, scale_in);
+    double softcap = 0.0;
+    if (softcap_in.has_value()) {
+        softcap = *softcap_in;
+        TORCH_CHECK_VALUE(softcap >= 0x1p-100 && std::isfinite((float)softcap), "softcap ", softcap, " must be positive and finite");
+    }
+    int64_t window = 0;
+    if (window_in.has_value()) {
+        window = *window_in;
+        TORCH_CHECK_VALUE(window >= 1, "window ", window, " must be positive");
+    }
+    const float* slope = nullptr;
+    if (slopes.has_value()) {
+        TORCH_CHECK_VALUE(slopes->scalar_type() == at::kFloat && slopes->sizes() == at::IntArrayRef({c.heads}) &&
+                              slopes->is_contiguous() && slopes->device() == c.device,
+                          "slopes must be a contiguous float32 tensor [", c.heads, "] on ", c.device);
+        slope = slopes->data_ptr<float>();
+    }
+    if (prefix.has_value()) check_i32(*prefix, "prefix", {c.requests}, c.device);
+    if (first.has_value()) check_i32(*first, "first", {c.rows}, c.device);
+    const at::DeviceGuard guard(c.device);
+    const Tensor q = rows16(q_in);
+    Tensor out = at::empty({c.rows, c.heads * head_dim}, q.options());
+    if (c.rows == 0) return out;
+    const size_t bytes =
+        awq_serve_kv16_attention_workspace(c.requests, c.rows, c.most, c.heads, data.size(1), head_dim, c.width, page_size);
+    const Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    check_status(awq_serve_kv16_attention(q.data_ptr(), row_stride(q), data.data_ptr(), i32(block_tables), i32(seq_lens),
+                                          i32(query_start), slope, prefix.has_value() ? i32(*prefix) : nullptr,
+                                          first.has_value() ? i32(*first) : nullptr, out.data_ptr(), c.requests, c.rows, c.most,
+                                          c.heads, data.size(1), head_dim, c.width, data.size(0), page_size, window, c.scale,
+                                          (float)softcap, q.scalar_type() == at::kHalf ? AWQ_SERVE_FP16 : AWQ_SERVE_BF16,
+                                          ws.data_ptr(), bytes, stream_of(c.device)),
+                 "awq_serve_kv16_attention");
     return out;
 }
 
@@ -339,6 +451,9 @@ void define_serving(py::module_& m) {
     m.def("kv4_append", &kv4_append);
     m.def("kv4_gather", &kv4_gather);
     m.def("kv4_attention", &kv4_attention);
+    m.def("check_cache16", &check_cache16);
+    m.def("kv16_append", &kv16_append);
+    m.def("kv16_attention", &kv16_attention);
     m.def("process_logits", &process_logits);
 }
 

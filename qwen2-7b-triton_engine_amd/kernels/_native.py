@@ -116,6 +116,10 @@ SERVING_SIGNATURES = {
     "awq_serve_kv4_gather": (ctypes.c_int, [_VP] * 4 + [_I64] * 6 + [_I32, _VP]),
     "awq_serve_kv4_attention_workspace": (_SZ, [_I64] * 8),
     "awq_serve_kv4_attention": (ctypes.c_int, [_VP, _I64] + [_VP] * 5 + [_I64] * 10 + [ctypes.c_float, _I32, _VP, _SZ, _VP]),
+    "awq_serve_kv16_append": (ctypes.c_int, [_VP, _I64] + [_VP] * 6 + [_I64] * 7 + [_I32, _VP]),
+    "awq_serve_kv16_attention_workspace": (_SZ, [_I64] * 8),
+    "awq_serve_kv16_attention": (ctypes.c_int, [_VP, _I64] + [_VP] * 8 + [_I64] * 10 + [ctypes.c_float] * 2 +
+                                 [_I32, _VP, _SZ, _VP]),
     "awq_serve_logits_workspace": (_SZ, [_I64] * 2),
     "awq_serve_logits": (ctypes.c_int, [_VP, _I64, _VP, _VP, _I64, _I64, _I32, _VP, _I32, _I64] + [_VP] * 8 +
                          [_I64, _VP, _VP, _SZ, _VP]),
