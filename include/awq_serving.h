@@ -9,6 +9,7 @@
  *   awq_serve_kv4_attention   attention over the cache
  *   awq_serve_kv16_append     RoPE of q and k; k and v stored as they are
  *   awq_serve_kv16_attention  attention over that cache: windows, documents, prefixes, capped scores, distances
+ *   awq_serve_logprobs        log-probabilities of given tokens, without the logits
  *   awq_serve_logits          penalties, biases, a grammar's mask, greedy token
  *
  * The reference has one static fp16 cache and one sequence
@@ -185,6 +186,19 @@ int awq_serve_kv16_attention(const void* q, int64_t q_stride, const void* cache,
                              int64_t max_query, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                              int64_t table_width, int64_t num_pages, int64_t page_size, int64_t window, float scale,
                              float softcap, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* With z = weight h of a token's hidden state h, hidden [tokens, k] (hidden_stride elements from row to row)
+ * and weight [vocab, k] in dtype (fp16 or bf16), both fp32 [tokens]:
+ *   lse = log sum exp z,  logprobs = z[target] - lse.
+ * targets int64 [tokens] (int32 with target_bytes 4); a negative target: logprobs 0, one of vocab or more: NaN.
+ * Products are exact and summed in fp32; the logits are not stored.  A logit of +infinity makes lse infinite,
+ * a NaN among a token's logits its results NaN.  k a multiple of 64, at most 2^20; hidden and weight 16-byte
+ * aligned, hidden_stride a multiple of 8 and at most 2^22; vocab and tokens at most 2^24.
+ * workspace: awq_serve_logprobs_workspace bytes of any content, 8-byte aligned.  Two launches. */
+size_t awq_serve_logprobs_workspace(int64_t tokens, int64_t vocab);
+int awq_serve_logprobs(const void* hidden, int64_t hidden_stride, const void* weight, const void* targets,
+                       int32_t target_bytes, float* logprobs, float* lse, int64_t tokens, int64_t vocab, int64_t k,
+                       int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* One step's logits [rows, vocab] (row_stride elements from row to row) after, in this
  * order and in fp32:

@@ -304,6 +304,40 @@ int awq_serve_kv16_attention(const void* q, int64_t q_stride, const void* cache,
     return done(launch_kv16_attention(a, dtype == AWQ_SERVE_BF16, static_cast<hipStream_t>(stream)));
 }
 
+size_t awq_serve_logprobs_workspace(int64_t tokens, int64_t vocab) {
+    if (tokens <= 0 || vocab <= 0 || tokens > kMostRows || vocab > kMostRows) return 0;
+    return logprobs_workspace((int)tokens, (int)vocab);
+}
+
+int awq_serve_logprobs(const void* hidden, int64_t hidden_stride, const void* weight, const void* targets,
+                       int32_t target_bytes, float* logprobs, float* lse, int64_t tokens, int64_t vocab, int64_t k,
+                       int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (tokens < 0 || vocab <= 0 || k <= 0 || k % 64 != 0 || hidden_stride < k) return AWQ_ERR_BAD_DIMS;
+    if ((dtype != AWQ_SERVE_FP16 && dtype != AWQ_SERVE_BF16) || (target_bytes != 4 && target_bytes != 8)) return AWQ_ERR_PATH;
+    if (tokens > kMostRows || vocab > kMostRows || k > (1 << 20) || hidden_stride > (1 << 22)) return AWQ_ERR_TOO_LARGE;
+    if (tokens == 0) return AWQ_OK;
+    const size_t need = logprobs_workspace((int)tokens, (int)vocab);
+    if (need == 0) return AWQ_ERR_TOO_LARGE;
+    if (!hidden || !weight || !targets || !logprobs || !lse) return AWQ_ERR_NULL_POINTER;
+    if (!aligned(hidden, 16) || hidden_stride % 8 != 0 || !aligned(weight, 16) || !aligned(targets, target_bytes) ||
+        !aligned(logprobs, 4) || !aligned(lse, 4) || !aligned(workspace, 8))
+        return AWQ_ERR_MISALIGNED;
+    if (!workspace || workspace_bytes < need) return AWQ_ERR_WORKSPACE;
+    LogprobsArgs a = {};
+    a.hidden = hidden;
+    a.ld = hidden_stride;
+    a.weight = weight;
+    a.targets = targets;
+    a.token_bytes = target_bytes;
+    a.logprobs = logprobs;
+    a.lse = lse;
+    a.part = static_cast<float*>(workspace);
+    a.tokens = (int)tokens;
+    a.vocab = (int)vocab;
+    a.k = (int)k;
+    return done(launch_logprobs(a, dtype == AWQ_SERVE_BF16, static_cast<hipStream_t>(stream)));
+}
+
 size_t awq_serve_logits_workspace(int64_t rows, int64_t vocab) {
     if (rows <= 0 || vocab <= 0 || rows > 65535 || vocab > kIndexLimit / 2) return 0;
     return logits_workspace((int)rows, (int)vocab);

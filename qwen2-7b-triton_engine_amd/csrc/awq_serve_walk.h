@@ -176,13 +176,6 @@ __device__ __forceinline__ void fill_rows(const Args& a) {
 
 // ---- pieces of the kernels ----------------------------------------------------------
 
-// A barrier for LDS alone: loads from memory stay in flight across it.
-__device__ __forceinline__ void lds_barrier() {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 // A request's pages from the one that holds `key` on: lane i has the i-th of 64, -1 past
 // the length or the table.  One load for 64 pages: a page's number then costs a lane
 // read and no wait for memory (a load of it would be waited for behind the codes'

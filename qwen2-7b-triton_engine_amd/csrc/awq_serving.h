@@ -151,6 +151,20 @@ bool kv16_attn_fits(int requests, int total, int max_query, int nh, int kvh);
 size_t kv16_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd);
 hipError_t launch_kv16_attention(const Kv16AttnArgs& a, bool bf16, hipStream_t stream);
 
+struct LogprobsArgs {
+    const void* hidden;         // [tokens, k], ld elements from row to row
+    int64_t ld;
+    const void* weight;         // [vocab, k]
+    const void* targets;        // [tokens] of token_bytes
+    int token_bytes;
+    float *logprobs, *lse;      // [tokens]
+    float* part;                // [vocabulary tiles][tokens] (maximum, sum)
+    int tokens, vocab, k;
+    float* chosen;              // set by the launch: [tokens], the targets' logits
+};
+size_t logprobs_workspace(int tokens, int vocab);
+hipError_t launch_logprobs(LogprobsArgs a, bool bf16, hipStream_t stream);
+
 struct LogitsArgs {
     const void* logits;
     int64_t ld;
@@ -202,6 +216,13 @@ __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = (uint32_t)to16<BF16>(x[2 * e]) | ((uint32_t)to16<BF16>(x[2 * e + 1]) << 16);
     *reinterpret_cast<u32x4*>(p) = w;
+}
+
+// A barrier for LDS alone: loads from memory stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 // Sum of a 64-bit value over the lanes below this one and itself.

@@ -355,6 +355,41 @@ Tensor kv16_attention(const Tensor& q_in, const Tensor& data, const Tensor& bloc
     return out;
 }
 
+std::tuple<Tensor, Tensor> token_logprobs(const Tensor& hidden_in, const Tensor& weight_in, const Tensor& targets) {
+    const Plain plain;
+    const int dtype = type16(hidden_in, "hidden");
+    TORCH_CHECK_VALUE(weight_in.scalar_type() == hidden_in.scalar_type(), "hidden and weight must be of one type, got ",
+                      hidden_in.scalar_type(), " and ", weight_in.scalar_type());
+    TORCH_CHECK_VALUE(hidden_in.dim() == 2 && weight_in.dim() == 2 && hidden_in.size(1) == weight_in.size(1) && weight_in.size(0) > 0,
+                      "hidden must be [T, K] and weight [V, K], got ", hidden_in.sizes(), " and ", weight_in.sizes());
+    const int64_t T = hidden_in.size(0), K = hidden_in.size(1), V = weight_in.size(0);
+    TORCH_CHECK_VALUE(K > 0 && K % 64 == 0, "K = ", K, " must be a multiple of 64");
+    TORCH_CHECK_VALUE(K <= (1 << 20) && V <= (1 << 24) && T <= (1 << 24), "hidden ", hidden_in.sizes(), " and weight ",
+                      weight_in.sizes(), ": at most 2^24 tokens, as many vocabulary rows and K = 2^20 are served");
+    check_on_gpu(hidden_in, "hidden");
+    const at::Device device = hidden_in.device();
+    TORCH_CHECK_VALUE(weight_in.device() == device, "hidden and weight must be on one device, got ", device, " and ",
+                      weight_in.device());
+    TORCH_CHECK_VALUE((targets.scalar_type() == at::kLong || targets.scalar_type() == at::kInt) && targets.dim() == 1 &&
+                          targets.size(0) == T && targets.is_contiguous() && targets.device() == device,
+                      "targets must be a contiguous int64 or int32 tensor [", T, "] on ", device);
+    const at::DeviceGuard guard(device);
+    Tensor hidden = rows16(hidden_in);
+    if (row_stride(hidden) > (1 << 22)) hidden = hidden.contiguous();
+    const Tensor weight = aligned16(weight_in.contiguous());
+    Tensor out = at::empty({2, T}, hidden.options().dtype(at::kFloat));
+    const std::vector<Tensor> parts = out.unbind(0);
+    if (T == 0) return {parts[0], parts[1]};
+    const size_t bytes = awq_serve_logprobs_workspace(T, V);
+    TORCH_CHECK_VALUE(bytes > 0, T, " tokens of ", V, " are more than one launch serves: give fewer at a time");
+    const Tensor ws = at::empty({(int64_t)bytes}, hidden.options().dtype(at::kByte));
+    check_status(awq_serve_logprobs(hidden.data_ptr(), row_stride(hidden), weight.data_ptr(), targets.data_ptr(),
+                                    (int32_t)targets.element_size(), parts[0].data_ptr<float>(), parts[1].data_ptr<float>(), T, V,
+                                    K, dtype, ws.data_ptr(), bytes, stream_of(device)),
+                 "awq_serve_logprobs");
+    return {parts[0], parts[1]};
+}
+
 std::tuple<Tensor, Tensor> process_logits(const Tensor& logits_in, const OptTensor& tokens, const OptTensor& lengths,
                                           const OptTensor& prompt_lens, const OptTensor& repetition,
                                           const OptTensor& presence, const OptTensor& frequency,
@@ -454,6 +489,7 @@ void define_serving(py::module_& m) {
     m.def("check_cache16", &check_cache16);
     m.def("kv16_append", &kv16_append);
     m.def("kv16_attention", &kv16_attention);
+    m.def("token_logprobs", &token_logprobs);
     m.def("process_logits", &process_logits);
 }
 

@@ -120,6 +120,8 @@ SERVING_SIGNATURES = {
     "awq_serve_kv16_attention_workspace": (_SZ, [_I64] * 8),
     "awq_serve_kv16_attention": (ctypes.c_int, [_VP, _I64] + [_VP] * 8 + [_I64] * 10 + [ctypes.c_float] * 2 +
                                  [_I32, _VP, _SZ, _VP]),
+    "awq_serve_logprobs_workspace": (_SZ, [_I64] * 2),
+    "awq_serve_logprobs": (ctypes.c_int, [_VP, _I64, _VP, _VP, _I32, _VP, _VP] + [_I64] * 3 + [_I32, _VP, _SZ, _VP]),
     "awq_serve_logits_workspace": (_SZ, [_I64] * 2),
     "awq_serve_logits": (ctypes.c_int, [_VP, _I64, _VP, _VP, _I64, _I64, _I32, _VP, _I32, _I64] + [_VP] * 8 +
                          [_I64, _VP, _VP, _SZ, _VP]),
