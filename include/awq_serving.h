@@ -170,8 +170,8 @@ int awq_serve_kv16_append(const void* qkv, int64_t qkv_stride, void* cache, cons
  *   first != NULL:    j >= first[i]                             int32 [total], by rows of the batch
  * A row that sees nothing (a negative position, first[i] past it) and a row of no request give zeros; rows past
  * max_query, and rows that see a token past the table or in a page outside the cache, NaN.  What a row does
- * not see may hold anything.  A row that sees a key or value that is not finite is not finite: in the columns
- * that the arithmetic says, or in all of them.
+ * not see may hold anything.  A row that sees a key of NaN, or a value that is not finite, is not finite: in the
+ * columns that the arithmetic says, or in all of them.
  * Scores, softmax and sums are fp32; the probabilities enter the product with V in dtype where a request
  * has many rows (an error of half a step of dtype each, as the output's own), in two parts of dtype
  * otherwise.  bf16 queries are scaled by a power of two first.  scale positive and finite, softcap 0 or
@@ -192,7 +192,7 @@ int awq_serve_kv16_attention(const void* q, int64_t q_stride, const void* cache,
  *   lse = log sum exp z,  logprobs = z[target] - lse.
  * targets int64 [tokens] (int32 with target_bytes 4); a negative target: logprobs 0, one of vocab or more: NaN.
  * Products are exact and summed in fp32; the logits are not stored.  A logit of +infinity makes lse infinite,
- * a NaN among a token's logits its results NaN.  k a multiple of 64, at most 2^20; hidden and weight 16-byte
+ * a NaN among a token's logits otherwise its results NaN.  k a multiple of 64, at most 2^20; hidden and weight 16-byte
  * aligned, hidden_stride a multiple of 8 and at most 2^22; vocab and tokens at most 2^24.
  * workspace: awq_serve_logprobs_workspace bytes of any content, 8-byte aligned.  Two launches. */
 size_t awq_serve_logprobs_workspace(int64_t tokens, int64_t vocab);

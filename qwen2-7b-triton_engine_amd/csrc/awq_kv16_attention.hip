@@ -15,6 +15,7 @@ namespace awq {
 namespace {
 
 constexpr int k16Cols = Kv16AttnArgs::kTileCols;
+constexpr float kLog2e = 1.4426950408889634f;
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_decode_kernel(Kv16AttnAr
     constexpr int VW = VC / 2;             // words of them
     constexpr int kStride = HD + 4;        // floats per column of the reduction buffer
     typedef uint32_t vwords __attribute__((ext_vector_type(VW)));
-    __shared__ float m_lds[kWaves][kCols], l_lds[kWaves][kCols];
+    __shared__ float m_lds[kWaves][kCols], l_lds[kWaves][kCols], unit_lds[kCols];
     __shared__ int seen_lds[kCols];
     __shared__ __align__(16) float o_lds[kWaves][kCols][kStride];
 
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_decode_kernel(Kv16AttnAr
     // Shaped scores are in their own unit, plain ones products of the scaled query:
     // every exponent is a difference of scores first, so that what they were rounded to on the way is
     // the same wherever two meet.
-    const float factor = a.factor(), unit = SHAPED ? factor : unit_of(factor, exp);
+    const float unit = SHAPED ? kLog2e : unit_of(a.scale * kLog2e, exp);
     const float natural = unit_of(a.scale, exp), inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
     const float slope = SHAPED && a.slopes ? a.slopes[head] : 0.0f;
     const int pos = it.r.len - it.r.rows + row;          // of a row that sees a token: 0 or more
@@ -325,9 +326,12 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_decode_kernel(Kv16AttnAr
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (t == 0) {
-        m_lds[wave][col] = SHAPED ? m : __builtin_ldexpf(m, -exp);   // of the scores themselves
+        m_lds[wave][col] = m;
         l_lds[wave][col] = l;
-        if (wave == 0) seen_lds[col] = sees.hi;
+        if (wave == 0) {
+            seen_lds[col] = sees.hi;
+            unit_lds[col] = unit;
+        }
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -345,7 +349,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_decode_kernel(Kv16AttnAr
         float sum = 0.0f, ls = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float al = __builtin_amdgcn_exp2f((m_lds[w][k] - ref) * factor);
+            const float al = __builtin_amdgcn_exp2f((m_lds[w][k] - ref) * unit_lds[k]);
             sum = fmaf(al, o_lds[w][k][d], sum);
             ls = fmaf(al, l_lds[w][k], ls);
         }
@@ -354,11 +358,12 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_decode_kernel(Kv16AttnAr
             const float y = seen_lds[k] == 0 ? 0.0f : sum / ls;
             reinterpret_cast<uint16_t*>(a.out)[((int64_t)(it.r.row0 + r) * a.nh + h) * HD + d] = to16<BF16>(y);
         } else {
-            float* dst = a.part + (((int64_t)item * kvh + g) * kCols + k) * (HD + 2);
+            float* dst = a.part + (((int64_t)item * kvh + g) * kCols + k) * (HD + a.kExtra);
             dst[d] = sum;
             if (d == 0) {
                 dst[HD] = mx;
                 dst[HD + 1] = ls;
+                dst[HD + 2] = unit_lds[k];
             }
         }
     }
@@ -497,7 +502,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
             for (int s = 0; s < kKS; ++s) q[s] = scaled_bf16(q[s], up);
         }
     }
-    const float factor = a.factor(), unit = SHAPED ? factor : unit_of(factor, exp);
+    const float unit = SHAPED ? kLog2e : unit_of(a.scale * kLog2e, exp);
     const float natural = unit_of(a.scale, exp), inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
     const float slope = SHAPED && a.slopes ? a.slopes[head] : 0.0f;
     const int pos = it.r.len - it.r.rows + row;
@@ -638,18 +643,14 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
                 *reinterpret_cast<u32x2*>(dst + 32 * d + 8 * j) = u32x2{pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3])};
             }
     } else {
-        float* dst = a.tile_part + (((int64_t)item * kvh + g) * k16Cols + local) * (HD + 2);
+        float* dst = a.tile_part + (((int64_t)item * kvh + g) * k16Cols + local) * (HD + a.kExtra);
 #pragma unroll
         for (int d = 0; d < kDb; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; r += 2)
-                    *reinterpret_cast<float2*>(dst + 32 * d + 8 * j + 4 * half + r) = float2{acc[d][4 * j + r], acc[d][4 * j + r + 1]};
-        if (half == 0) {
-            dst[HD] = SHAPED ? m : __builtin_ldexpf(m, -exp);
-            dst[HD + 1] = l;
-        }
+                *reinterpret_cast<floatx4*>(dst + 32 * d + 8 * j + 4 * half) =
+                    floatx4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+        if (half == 0) *reinterpret_cast<floatx4*>(dst + HD) = floatx4{m, l, unit, 0.0f};
     }
 }
 
@@ -670,7 +671,7 @@ hipError_t launch(Kv16AttnArgs a, hipStream_t stream) {
     a.tile_target = p.tile_target;
     a.records = reinterpret_cast<i32x4*>(a.part);
     a.part += (size_t)a.total * (sizeof(i32x4) / sizeof(float));
-    a.tile_part = a.part + p.decode_items * a.s.kvh * kCols * (HD + 2);
+    a.tile_part = a.part + p.decode_items * a.s.kvh * kCols * (HD + a.kExtra);
     if (p.decode) {
         hipLaunchKernelGGL((awq_kv16_decode_kernel<HD, BF16, SHAPED>), dim3((unsigned)(p.decode_items * a.s.kvh)), dim3(kThreads), 0,
                            stream, a);
@@ -701,7 +702,7 @@ bool kv16_attn_fits(int requests, int total, int max_query, int nh, int kvh) {
 }
 
 size_t kv16_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd) {
-    return part_bytes(attention_plan<k16Cols>(requests, total, max_query, nh / kvh, kvh), total, kvh, hd);
+    return part_bytes(attention_plan<k16Cols>(requests, total, max_query, nh / kvh, kvh), total, kvh, hd + Kv16AttnArgs::kExtra);
 }
 
 hipError_t launch_kv16_attention(const Kv16AttnArgs& a, bool bf16, hipStream_t stream) {

@@ -203,8 +203,8 @@ __global__ __launch_bounds__(256) void awq_logprobs_join_kernel(LogprobsArgs a, 
     const int64_t want = a.token_bytes == 8 ? reinterpret_cast<const int64_t*>(a.targets)[token]
                                             : reinterpret_cast<const int32_t*>(a.targets)[token];
     // An infinite logit is all of the sum (its tile's sum is NaN: infinity less itself).
-    const float log_s = logf(s);
-    a.lse[token] = m == INFINITY || m == -INFINITY ? (m == -INFINITY && s != s ? NAN : m) : m + log_s;
+    const float log_s = m == INFINITY ? 0.0f : logf(s);
+    a.lse[token] = m == -INFINITY && s == 0.0f ? m : m + log_s;
     // (z - m) - log s: closer than z - lse where the target is likely
     a.logprobs[token] = want < 0 ? 0.0f : want >= a.vocab ? NAN : (a.chosen[token] - m) - log_s;
 }

@@ -763,7 +763,7 @@ hipError_t launch(Kv4AttnArgs a, hipStream_t stream) {
 }  // namespace
 
 size_t kv4_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd) {
-    return part_bytes(attention_plan(requests, total, max_query, nh / kvh, kvh), total, kvh, hd);
+    return part_bytes(attention_plan(requests, total, max_query, nh / kvh, kvh), total, kvh, hd + Kv4AttnArgs::kExtra);
 }
 
 hipError_t launch_kv4_attention(const Kv4AttnArgs& a, bool bf16, hipStream_t stream) {

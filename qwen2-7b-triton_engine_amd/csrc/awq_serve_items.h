@@ -46,6 +46,13 @@ constexpr int walked_tokens(int width, int page_log2, int len) {
     return len < past ? len : past;
 }
 
+// The first token that any of a request's rows may see under a sliding window (0: none), of `walked` tokens.
+// Where the window lies past the table that is the missing token there.
+constexpr int first_token(int window, int rows, int len, int walked) {
+    const int64_t lo = (int64_t)len - rows - window + 1;
+    return window == 0 || lo <= 0 || walked == 0 ? 0 : lo < walked ? (int)lo : walked - 1;
+}
+
 // Columns of a request that are computed, its blocks of them in this kernel (COLS says
 // which), its tokens in steps.  limit: columns up to which a request is the decode kernel's.
 constexpr int request_columns(int rows, int max_query, int group) { return (rows < max_query ? rows : max_query) * group; }
@@ -85,8 +92,8 @@ struct AttentionPlan {
     bool decode, tile, combine;
     int limit, decode_target, tile_target, tile_cols;
     int64_t decode_items, tile_items;  // at most, of one kv head
-    size_t part_floats(int kvh, int hd) const {          // the items' sums
-        return (size_t)(decode_items * kCols + (tile_target ? tile_items * tile_cols : 0)) * kvh * (hd + 2);
+    size_t part_floats(int kvh, int floats) const {      // the items' sums, so many floats of a column
+        return (size_t)(decode_items * kCols + (tile_target ? tile_items * tile_cols : 0)) * kvh * floats;
     }
 };
 template <int TILE_COLS = kTileCols>

@@ -6,7 +6,8 @@
 //   kTileCols                       columns of a tile workgroup
 //   first_key(rows, len)            the first token that a row of a request may see
 //   sees_none(b, row0, rows, len, i)   whether the i-th row of request b sees no token
-//   factor()                        what one of the maxima in `part` counts in powers of two
+//   kExtra                          floats of a column in `part` past its sums: its maximum, the sum of its exponentials, ..
+//   factor(column)                  what one of that maximum's counts in powers of two
 #pragma once
 
 #include "awq_serve_items.h"
@@ -214,7 +215,6 @@ __device__ __forceinline__ void combine_items(const Args& a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int first = WAVES == 1 ? 0 : wave;
     const int64_t all = (int64_t)a.total * a.nh;
-    const float factor = a.factor();
     constexpr int kUnits = kWaves / WAVES;               // of a workgroup
     for (int64_t unit = (int64_t)blockIdx.x * kUnits + (WAVES == 1 ? wave : 0); unit < all;
          unit += (int64_t)gridDim.x * kUnits) {
@@ -231,8 +231,9 @@ __device__ __forceinline__ void combine_items(const Args& a) {
         const bool tile = rec[1] < 0;
         const int c = rec[0] * group + head % group, cols = tile ? Args::kTileCols : kCols, block = c / cols, splits = rec[3];
         const int item = tile ? ~rec[1] + rec[2] - 1 - block : rec[1] + block;
-        const int64_t step = (int64_t)rec[2] * a.s.kvh * cols * (HD + 2);
-        const float* base = (tile ? a.tile_part : a.part) + (((int64_t)item * a.s.kvh + g) * cols + c % cols) * (HD + 2);
+        const int64_t step = (int64_t)rec[2] * a.s.kvh * cols * (HD + Args::kExtra);
+        const float* base = (tile ? a.tile_part : a.part) + (((int64_t)item * a.s.kvh + g) * cols + c % cols) * (HD + Args::kExtra);
+        const float factor = a.factor(base + HD);
 
         float mx = -INFINITY, l = 0.0f, sum[W] = {};
         for (int s0 = 0; s0 < splits; s0 += 64 * WAVES) {
@@ -306,8 +307,8 @@ __device__ __forceinline__ void combine_items(const Args& a) {
 constexpr int kCombineGroups = 8192;   // workgroups of the combining launch at most
 constexpr int kFewUnits = 512;         // rows times heads that get four waves each there
 
-inline size_t part_bytes(const AttentionPlan& p, int total, int kvh, int hd) {   // row records, then the items' sums
-    return (size_t)total * sizeof(i32x4) + p.part_floats(kvh, hd) * sizeof(float);
+inline size_t part_bytes(const AttentionPlan& p, int total, int kvh, int floats) {   // row records, then the items' sums
+    return (size_t)total * sizeof(i32x4) + p.part_floats(kvh, floats) * sizeof(float);
 }
 
 }  // namespace

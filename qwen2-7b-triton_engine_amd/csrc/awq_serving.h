@@ -66,10 +66,10 @@ struct Kv4AttnArgs {
     int limit;                  // columns up to which a request is the decode kernel's
     int decode_target, tile_target;   // items of one kv head that the kernels aim at
     // what awq_serve_walk.h asks for
-    static constexpr int kTileCols = 64;
+    static constexpr int kTileCols = 64, kExtra = 2;
     __device__ __forceinline__ int first_key(int, int) const { return 0; }
     __device__ __forceinline__ bool sees_none(int, int, int rows, int len, int i) const { return (int64_t)len - rows + i < 0; }
-    __device__ __forceinline__ float factor() const { return scale * 1.4426950408889634f; }
+    __device__ __forceinline__ float factor(const float*) const { return scale * 1.4426950408889634f; }
 };
 size_t kv4_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd);
 hipError_t launch_kv4_attention(const Kv4AttnArgs& a, bool bf16, hipStream_t stream);
@@ -112,12 +112,9 @@ struct Kv16AttnArgs {
     i32x4* records;             // [total]
     int limit, decode_target, tile_target;
     // what awq_serve_walk.h asks for
-    static constexpr int kTileCols = 128;
+    static constexpr int kTileCols = 128, kExtra = 4;   // maximum, sum, unit, nothing
     __device__ __forceinline__ int first_key(int rows, int len) const {
-        if (window == 0) return 0;
-        const int64_t lo = (int64_t)len - rows - window + 1;
-        const int n = walked_tokens(width, s.page_log2, len);
-        return lo <= 0 || n == 0 ? 0 : lo < n ? (int)lo : n - 1;
+        return first_token(window, rows, len, walked_tokens(width, s.page_log2, len));
     }
     // Tokens lo .. hi - 1 that the i-th row of request b sees; none: 0 and 0.  Of a table
     // that is too short its first missing token is the last one: it gives NaN.
@@ -145,7 +142,7 @@ struct Kv16AttnArgs {
     }
     // Scores that are capped or carry a bias are scaled before, plain ones after their differences.
     __host__ __device__ bool shaped() const { return softcap > 0.0f || slopes; }
-    __device__ __forceinline__ float factor() const { return (shaped() ? 1.0f : scale) * 1.4426950408889634f; }
+    __device__ __forceinline__ float factor(const float* extra) const { return extra[2]; }
 };
 bool kv16_attn_fits(int requests, int total, int max_query, int nh, int kvh);
 size_t kv16_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd);
