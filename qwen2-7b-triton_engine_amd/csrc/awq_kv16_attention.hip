@@ -80,14 +80,14 @@ __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
     return ((w & kLow) == kLow ? 0u : w & 0xFFFFu) | ((w & kHigh) == kHigh ? 0u : w & 0xFFFF0000u);
 }
 
-// The probabilities' scale: fp16's smallest values would lose bits, 2^14 times as large
-// they keep 11 down to 2^-28.
+// The probabilities' scale in powers of two, and how far above it a score may lie before the running maximum is
+// raised: of 32 columns one or another passes its maximum in many tiles, and each time the sums are rescaled.
+// fp16 holds values up to 2^16 and 11 bits down to 2^-14: 2^8 leaves both room for 2^7.5 above and
+// all bits down to 2^-22 of the maximum; bf16 has the range of fp32.
 template <bool BF16>
-constexpr float kPScale = BF16 ? 0.0f : 14.0f;
-// The running maximum is raised only where a score passes it by more than this (in
-// powers of two): probabilities of up to 2^1.5 still fit fp16 when scaled, and most
-// tiles do without the cross-lane maximum and the rescaling.
-constexpr float kSlack16 = 1.5f;
+constexpr float kPScale = BF16 ? 0.0f : 8.0f;
+template <bool BF16>
+constexpr float kSlack16 = BF16 ? 16.0f : 7.5f;
 
 // bf16 queries are brought to at most 2^8 by a power of two, so that a sum of products
 // stays inside fp32 for keys of ordinary size; fp16's are inside it as they are.  Returns the power's exponent.
@@ -104,14 +104,25 @@ __device__ __forceinline__ u32x4 scaled_bf16(u32x4 w, float up) {
 // What multiplies a product of the scaled query: kept finite (2^127 under a large scale passes fp32 here).
 __device__ __forceinline__ float unit_of(float factor, int exp) { return fminf(__builtin_ldexpf(factor, -exp), __FLT_MAX__); }
 
-// c tanh(x / c).  Below 1/4 the series, to 1e-8 of the value; above, 1 - 2 / (1 + e^2u), whose cancellation costs
-// 5e-7 of it there at most.
+// c tanh(x / c) as c - 2 c / (1 + e^(2 x / c)): in absolute terms it errs by a few 2^-24 c, nothing beside the
+// probabilities' rounding while c is below 2^9; above, where small scores matter beside a large cap, the series
+// to 1e-8 of the value below c / 4.
+constexpr float kPlainCap = 512.0f;
 __device__ __forceinline__ float capped(float x, float c, float inv) {
     const float u = x * inv, u2 = u * u;
     const float e = __builtin_amdgcn_exp2f(u * 2.8853900817779268f);
     const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+    if (c <= kPlainCap) return c * far;
     const float near = u * fmaf(u2, fmaf(u2, fmaf(u2, fmaf(u2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
     return c * (fabsf(u) < 0.25f ? near : far);
+}
+// A sum of rounded probabilities, two a word.
+template <bool BF16>
+__device__ __forceinline__ float add2(uint32_t p, float sum) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, kOnes<true>), sum, false);
+    else
+        return __builtin_amdgcn_fdot2(as_h2(p), as_h2(kOnes<false>), sum, false);
 }
 
 // ---- few columns: decode ---------------------------------------------------------------
@@ -282,7 +293,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_decode_kernel(Kv16AttnAr
         float mx = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
         for (int r = 1; r < 4; ++r) mx = fmaxf(mx, fmaxf(s[0][r], s[1][r]));
-        if (__any((mx - m) * unit > kSlack16)) {
+        if (__any((mx - m) * unit > kSlack16<BF16>)) {
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
             const float alpha = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : (m - mn) * unit);
@@ -390,7 +401,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
     constexpr int kChunks = HD / 8;
     constexpr int kLoads = 16 * HD * 2 / 1024;           // of a wave: 16 tokens of K or V
     constexpr int kHalf = kTileKeys * HD;                // elements of K or V in a buffer
-    __shared__ __align__(1024) uint16_t buf[2][2 * kHalf];
+    __shared__ __align__(1024) uint16_t k_lds[2][kHalf], v_lds[2][kHalf];
     __shared__ __align__(8) uint16_t odd_lds[2][kWaves];
 
     Item it;
@@ -453,35 +464,64 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
 
     // Loads: wave w brings tokens 16 w .. of the tile.  A place past the
     // last token, or in a page outside the cache, lies past its resource's end and reads as zeros.
-    Pages64 window = {a.tables + (int64_t)it.b * a.width, 0, 0};
-    window.fetch(a, start, n);
+    // The table's entries from a tile's first page on are a lane's each, 64 of them; `lost` has a bit for
+    // those of the request's tokens that are no page of the cache.
+    const int32_t* table = a.tables + (int64_t)it.b * a.width;
+    const int log2 = a.s.page_log2;
+    int first = 0, entry = 0;
+    uint64_t lost = 0;
+    auto fetch = [&](int key0) {
+        first = __builtin_amdgcn_readfirstlane(key0 >> log2);
+        const int index = first + lane;
+        const bool tokens = (int64_t)index << log2 < n;
+        entry = index < a.width && tokens ? table[index] : -1;
+        const bool there = entry >= 0 && entry < a.s.num_pages;
+        lost = __ballot(tokens && !there);
+        entry = there ? entry : 0;
+    };
+    fetch(start);
+    const uint64_t cache_g = reinterpret_cast<uint64_t>(a.cache) + 2 * g * a.s.block();
+    const uint32_t page_bytes = (uint32_t)(2 * kvh * a.s.block());      // of all heads: 2^29 at most
     const int r0 = lane / kChunks;                       // a load's rows begin with this lane's token
     const uint32_t l_ofs = r0 * (HD * 2) + ((lane % kChunks) ^ swizzle<HD>(r0)) * 16;
-    const uint32_t lds0 = lds_addr(&buf[0][0]) + wave * (16 * HD * 2);
-    // Which of a tile's blocks of 16 tokens lie in pages outside the cache: a bit each.
-    auto issue = [&](int key0, int stage) {
-        uint32_t gone = 0;
-        int mine = -1;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int page = window.page(a, key0 + 16 * j, n);
-            const bool there = page >= 0 && page < a.s.num_pages;
-            if (!there) gone |= 1u << j;
-            if (j == wave) mine = there ? page : -1;
-        }
+    const uint32_t k_to = lds_addr(&k_lds[0][0]) + wave * (16 * HD * 2), v_to = lds_addr(&v_lds[0][0]) + wave * (16 * HD * 2);
+    struct Place {                                       // of this wave's tokens of a tile
+        uint64_t at;
+        int tokens;
+        uint32_t gone;                                   // the tile's blocks of 16 tokens in pages outside the cache, a bit each
+    };
+    auto locate = [&](int key0) {
+        if (((key0 + kTileKeys - 1) >> log2) - first >= 64) fetch(key0);
         const int key = key0 + 16 * wave, left = n - key;
-        const uint32_t bytes = mine < 0 || left <= 0 ? 0u : (uint32_t)(left < 16 ? left : 16) * (HD * 2);
-        const uint16_t* at = a.cache + ((int64_t)(mine < 0 ? 0 : mine) * kvh + g) * a.s.block() + (key & (a.s.page() - 1)) * HD;
-        const u32x4 rk = raw_rsrc(at, bytes), rv = raw_rsrc(at + (HD << a.s.page_log2), bytes);
-        const uint32_t to = lds0 + stage * (4 * kHalf);
+        Place p = {0, left < 16 ? (left > 0 ? left : 0) : 16, 0};
+        if (lost) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p.gone |= (uint32_t)(lost >> (((key0 + 16 * j) >> log2) - first) & 1) << j;
+            p.tokens = p.gone >> wave & 1 ? 0 : p.tokens;
+        }
+        p.tokens = __builtin_amdgcn_readfirstlane(p.tokens);
+        const uint32_t page = (uint32_t)__builtin_amdgcn_readlane(entry, (key >> log2) - first);
+        p.at = cache_g + (uint64_t)page * page_bytes + (uint32_t)((key & (a.s.page() - 1)) * (HD * 2));
+        return p;
+    };
+    auto load = [&](uint64_t at, int tokens, uint32_t to) {
+        const u32x4 r = raw_rsrc(reinterpret_cast<const void*>(at), tokens * (HD * 2));
         constexpr uint32_t kFlip = HD == 128 ? 16 : 32;  // the swizzle of the tokens of a load after
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) buffer_load_lds_x4(rk, (l_ofs ^ (kFlip * i)) + 1024 * i, 0, to + 1024 * i);
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) buffer_load_lds_x4(rv, (l_ofs ^ (kFlip * i)) + 1024 * i, 0, to + 2 * kHalf + 1024 * i);
-        return gone;
+        for (int i = 0; i < kLoads; ++i) buffer_load_lds_x4(r, (l_ofs ^ (kFlip * i)) + 1024 * i, 0, to + 1024 * i);
     };
-    uint32_t gone_next = tiles > 0 ? issue(start, 0) : 0;
+    auto load_k = [&](const Place& p, int stage) { load(p.at, p.tokens, k_to + stage * (2 * kHalf)); };
+    auto load_v = [&](const Place& p, int stage) { load(p.at + ((HD * 2) << log2), p.tokens, v_to + stage * (2 * kHalf)); };
+    Place now = {}, next = {};                           // of this tile and the next
+    if (tiles > 0) {
+        now = locate(start);
+        load_k(now, 0);
+        load_v(now, 0);
+    }
+    if (tiles > 1) {
+        next = locate(start + kTileKeys);
+        load_k(next, 1);
+    }
 
     // This lane's query: columns 16 s + 8 half .. of the head.
     u32x4 q[kKS];
@@ -502,26 +542,66 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
             for (int s = 0; s < kKS; ++s) q[s] = scaled_bf16(q[s], up);
         }
     }
-    const float unit = SHAPED ? kLog2e : unit_of(a.scale * kLog2e, exp);
+    // Shaped scores are formed in powers of two, plain ones are products of the scaled query.
+    const float unit = SHAPED ? 1.0f : unit_of(a.scale * kLog2e, exp);
     const float natural = unit_of(a.scale, exp), inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
-    const float slope = SHAPED && a.slopes ? a.slopes[head] : 0.0f;
+    const float cap2 = a.softcap * kLog2e, cap_in = unit_of(a.scale, exp) * inv_cap * 2.8853900817779268f;
+    const float slope = SHAPED && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
     const int pos = it.r.len - it.r.rows + row;
+    wait_vm_stores();                                    // the query, here: in the loop its wait would be one for the next tiles
+    lds_barrier();
 
-    // Operand addresses in bytes: token col (+ 32) and chunk 2 s + half of K; of V, lane 4 m + j of
+    // Operand addresses: token col (+ 32) and chunk 2 s + half of K; of V, lane 4 m + j of
     // 16 supplies four columns of token 4 half + m, and its group's other half of the 32 columns.
-    const uint32_t k_at = col * (HD * 2) + (half ^ swizzle<HD>(col)) * 16;
+    const uint32_t k_at = lds_addr(&k_lds[0][0]) + col * (HD * 2) + (half ^ swizzle<HD>(col)) * 16;
     const int vm = 4 * half + (lane >> 2 & 3), vj = lane & 3;
-    const uint32_t v_at = 2 * kHalf + vm * (HD * 2) + ((2 * (lane >> 4 & 1) + (vj >> 1)) ^ swizzle<HD>(vm)) * 16 + (vj & 1) * 8;
+    const uint32_t v_at = lds_addr(&v_lds[0][0]) + vm * (HD * 2) + ((2 * (lane >> 4 & 1) + (vj >> 1)) ^ swizzle<HD>(vm)) * 16 + (vj & 1) * 8;
 
-    float m = -INFINITY, l = 0.0f;
+    // A score s counts 2^(s unit + ref), scaled by kPScale: the sum is one fused step, rounded once.  Where ref is
+    // large (`big`, for the whole wave) its own rounding would show; there it is (s - m) unit.
+    constexpr float kBig = 256.0f, kMost = kPScale<BF16> + kSlack16<BF16>;
+    float ref = 0.0f, m = 0.0f, l = 0.0f;
+    bool some = false, big = false;                      // some: the column has met a score
     floatx16 acc[kDb];
 #pragma unroll
     for (int d = 0; d < kDb; ++d) acc[d] = floatx16{};
+    floatx16 s[2];
+    // Operands are read two steps ahead of their products, and fences keep it so: the scheduler by itself reads
+    // each right before its product and waits for LDS every time.
+    u32x4 kf[2][2];
+    // Addresses of a stage are formed from one opaque register each tile: sixteen of them, hoisted, would be too many.
+    typedef const __attribute__((address_space(3))) u32x4* lds16;
+    auto in_stage = [&](uint32_t at, int stage) {
+        at += stage * (2 * kHalf);
+        asm volatile("" : "+v"(at));
+        return at;
+    };
+    auto read_k = [&](uint32_t at, int st) {             // of one k-step, both blocks of 32 tokens
+#pragma unroll
+        for (int b = 0; b < 2; ++b) kf[st % 2][b] = *(lds16)(uintptr_t)((at ^ (32 * st)) + b * (32 * HD * 2));
+    };
+    auto score = [&](uint32_t at, int st) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[b] = mfma32<BF16>(kf[st % 2][b], q[st], st ? s[b] : floatx16{});
+        if (st + 2 < kKS) read_k(at, st + 2);
+    };
+    auto all_scores = [&](int stage) {
+        const uint32_t at = in_stage(k_at, stage);
+        read_k(at, 0);
+        read_k(at, 1);
+#pragma unroll
+        for (int st = 0; st < kKS; ++st) {
+            score(at, st);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    if (tiles > 0) all_scores(0);
     for (int tile = 0; tile < tiles; ++tile) {
         const int key0 = start + tile * kTileKeys;
-        const uint32_t gone = gone_next;
-        char* base = reinterpret_cast<char*>(&buf[tile & 1][0]);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        char* v_base = reinterpret_cast<char*>(&v_lds[tile & 1][0]);
+        Place after = {};
+        if (tile + 2 < tiles) after = locate(key0 + 2 * kTileKeys);
+asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         // Where some column does not see all of the tile's tokens, a value of V that is not finite must
         // not meet its probability of zero: each wave takes such values out of the tokens it
         // brought, and the rows that see them get NaN by their scores.
@@ -531,7 +611,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
             uint32_t odd = 0;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                u32x4* at = reinterpret_cast<u32x4*>(base + 2 * kHalf + wave * (16 * HD * 2) + 1024 * i + 16 * lane);
+                u32x4* at = reinterpret_cast<u32x4*>(v_base + wave * (16 * HD * 2) + 1024 * i + 16 * lane);
                 u32x4 w = *at;
                 uint32_t most = 0;
 #pragma unroll
@@ -548,9 +628,19 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
             }
             if (lane == 0) odd_lds[tile & 1][wave] = (uint16_t)odd;
         }
-        lds_barrier();                                   // the tile is there, and the other buffer read by all
-        if (tile + 1 < tiles) gone_next = issue(key0 + kTileKeys, (tile + 1) & 1);
-        if (key0 >= hi_max || key0 + kTileKeys <= lo_min) continue;   // nothing for this wave
+        lds_barrier();
+                                           // the next tile's K and this one's V are there, the others read by all
+        const bool more = tile + 1 < tiles;
+        const int stage = (tile + 1) & 1;
+        if (tile + 2 < tiles) load_k(after, tile & 1);
+        if (more) load_v(next, stage);
+        const uint32_t gone = now.gone;
+        now = next;
+        next = after;
+        if (key0 >= hi_max || key0 + kTileKeys <= lo_min) {   // nothing for this wave
+            if (more) all_scores(stage);
+            continue;
+        }
         uint64_t bad = 0;                                // tokens that give NaN, a bit each
         if (edge) {
             const u32x2 w = *reinterpret_cast<const u32x2*>(&odd_lds[tile & 1][0]);
@@ -561,71 +651,152 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
             for (int j = 0; j < 4; ++j)
                 if (gone >> j & 1) bad |= 0xFFFFull << (16 * j);
         }
-
-        floatx16 s[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            s[b] = floatx16{};
-#pragma unroll
-            for (int st = 0; st < kKS; ++st)
-                s[b] = mfma32<BF16>(*reinterpret_cast<const u32x4*>(base + (k_at ^ (32 * st)) + b * (32 * HD * 2)), q[st], s[b]);
-        }
         if constexpr (SHAPED) {
-            const float far = (float)(pos - key0 - 4 * half);
+            if (a.softcap == 0.0f) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+                for (int i = 0; i < 32; ++i) s[i / 16][i % 16] *= natural * kLog2e;
+            } else if (a.softcap <= kPlainCap) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float x = s[b][i] * natural;
-                    if (a.softcap > 0.0f) x = capped(x, a.softcap, inv_cap);
-                    s[b][i] = fmaf(-slope, fabsf(far - (float)(32 * b + 8 * (i / 4) + i % 4)), x);
+                for (int i = 0; i < 32; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(s[i / 16][i % 16] * cap_in);
+                    s[i / 16][i % 16] = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(e + 1.0f), cap2);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    s[i / 16][i % 16] = capped(s[i / 16][i % 16] * natural, a.softcap, inv_cap) * kLog2e;
                     if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // few at a time: registers
                 }
+            }
+            if (a.slopes) {
+                const float far = (float)(pos - key0 - 4 * half);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    s[i / 16][i % 16] = fmaf(-slope, fabsf(far - (float)(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4)), s[i / 16][i % 16]);
+            }
         }
-        if (bad || key0 < lo_max || key0 + kTileKeys > hi_min) {
+        if (key0 + kTileKeys > hi_min) {
+            const int end = sees.hi - key0 - 4 * half;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                s[i / 16][i % 16] = 32 * (i / 16) + 8 * (i % 16 / 4) + i % 4 < end ? s[i / 16][i % 16] : -INFINITY;
+        }
+        if (key0 < lo_max) {
+            const int begin = sees.lo - key0 - 4 * half;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                s[i / 16][i % 16] = 32 * (i / 16) + 8 * (i % 16 / 4) + i % 4 >= begin ? s[i / 16][i % 16] : -INFINITY;
+        }
+        if (bad) {
             const uint64_t mine = bad >> (4 * half);
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int in = 32 * b + 8 * (i / 4) + i % 4, key = key0 + in + 4 * half;
-                    s[b][i] = key < sees.lo || key >= sees.hi ? -INFINITY : mine >> in & 1 ? NAN : s[b][i];
-                }
+            for (int i = 0; i < 32; ++i) {
+                const int in = 32 * (i / 16) + 8 * (i % 16 / 4) + i % 4, key = key0 + in + 4 * half;
+                if (mine >> in & 1 && key >= sees.lo && key < sees.hi) s[i / 16][i % 16] = NAN;
+            }
         }
-        float mx = fmaxf(s[0][0], s[1][0]);
+        if (__any(!some)) {
+            float mx = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
-        if (__any((mx - m) * unit > kSlack16)) {
-            const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
-            const float alpha = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.0f : (m - mn) * unit);
+            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            if (!some && mx != -INFINITY) {
+                m = mx;
+                ref = kPScale<BF16> - mx * unit;
+                some = true;
+            }
+            big = big || __any(fabsf(ref) > kBig);
+        }
+        float y[32];
+        if (!big) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = SHAPED ? s[i / 16][i % 16] + ref : fmaf(s[i / 16][i % 16], unit, ref);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = fmaf(s[i / 16][i % 16] - m, unit, kPScale<BF16>);
+        }
+        // (here, where the scores' registers are free)
+        const uint32_t k_now = in_stage(k_at, stage), v_now = in_stage(v_at, tile & 1);
+        if (more) {
+            read_k(k_now, 0);
+            if (!SHAPED) read_k(k_now, 1);               // (shaped scores have more else in registers)
+        }
+        float top = fmaxf(y[0], y[1]);
+#pragma unroll
+        for (int i = 2; i < 32; i += 2) top = fmaxf(top, fmaxf(y[i], y[i + 1]));
+        if (__any(top > kMost)) {
+            top = fmaxf(top, __shfl_xor(top, 32));
+            float up = top > kPScale<BF16> ? top - kPScale<BF16> : 0.0f;
+            if (big) {
+                const float mn = m + up / unit;
+                up = (mn - m) * unit;
+                m = mn;
+            } else {
+                const float cn = ref - up;
+                up = ref - cn;
+                ref = cn;
+                if (__any(fabsf(ref) > kBig)) {
+                    m = (kPScale<BF16> - ref) / unit;
+                    big = true;
+                }
+            }
+            const float alpha = __builtin_amdgcn_exp2f(-up);
             l *= alpha;
 #pragma unroll
-            for (int d = 0; d < kDb; ++d) acc[d] *= alpha;
-            m = mn;
+            for (int i = 0; i < 32; ++i) y[i] -= up;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < kDb; ++d) {
+                acc[d] *= alpha;
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        const float ref = m == -INFINITY ? 0.0f : m;     // nothing yet: every exponential is 0
+        // V's operands: product j is of k-step j / kDb and column block j % kDb.
+        constexpr int kProducts = 4 * kDb, kAhead = 4;
+        u32x4 vf[kAhead];
+        auto read_v = [&](int j) {
+            typedef __attribute__((address_space(3))) s16x4* lds4;
+            const uint32_t at = 16 * (j / kDb) * (HD * 2), flip = 64 * (j % kDb);
+            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)((v_now ^ flip) + at)));
+            const u32x2 z = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)((v_now ^ flip ^ 32) + at + 8 * (HD * 2))));
+            vf[j % kAhead] = u32x4{x.x, x.y, z.x, z.y};
+        };
+        // The exponentials under the next tile's scores, then the sums.
         u32x4 p[4];
+        auto weigh = [&](int i) {
+            const uint32_t w = pack2<BF16>(__builtin_amdgcn_exp2f(y[i]), __builtin_amdgcn_exp2f(y[i + 1]));
+            l = add2<BF16>(w, l);
+            p[i / 8][i % 8 / 2] = w;
+        };
+        constexpr int kEach = 32 / kKS;                  // probabilities of a k-step
+        if (more) {
+            if (SHAPED) read_k(k_now, 1);
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+            for (int st = 0; st < kKS; ++st) {
+                score(k_now, st);
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i] - ref, unit, kPScale<BF16>));
-                const float y = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1] - ref, unit, kPScale<BF16>));
-                l += x;
-                l += y;
-                p[2 * b + i / 8][i % 8 / 2] = pack2<BF16>(x, y);
+                for (int i = 0; i < kEach; i += 2) weigh(kEach * st + i);
+                if (st >= kKS - 2)
+#pragma unroll
+                    for (int j = 0; j < kAhead / 2; ++j) read_v(kAhead / 2 * (st - kKS + 2) + j);
+                __builtin_amdgcn_sched_barrier(0);
             }
-        typedef __attribute__((address_space(3))) s16x4* lds4;
+        } else {
+            // Opaque: what both branches have in common must not be moved before them, away from the products.
 #pragma unroll
-        for (int d = 0; d < kDb; ++d)
+            for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(y[i]));
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                char* at = base + 16 * st * (HD * 2);
-                const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + (v_at ^ (64 * d)))));
-                const u32x2 y = __builtin_bit_cast(
-                    u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + (v_at ^ (64 * d) ^ 32) + 8 * (HD * 2))));
-                acc[d] = mfma32<BF16>(u32x4{x.x, x.y, y.x, y.y}, p[st], acc[d]);
-            }
+            for (int i = 0; i < 32; i += 2) weigh(i);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) read_v(j);
+        }
+#pragma unroll
+        for (int j = 0; j < kProducts; ++j) {
+            acc[j % kDb] = mfma32<BF16>(vf[j % kAhead], p[j / kDb], acc[j % kDb]);
+            if (j + kAhead < kProducts) read_v(j + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 
     l += __shfl_xor(l, 32);
@@ -650,7 +821,8 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
             for (int j = 0; j < 4; ++j)
                 *reinterpret_cast<floatx4*>(dst + 32 * d + 8 * j + 4 * half) =
                     floatx4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
-        if (half == 0) *reinterpret_cast<floatx4*>(dst + HD) = floatx4{m, l, unit, 0.0f};
+        const float most = !some ? -INFINITY : big ? m : (kPScale<BF16> - ref) / unit;
+        if (half == 0) *reinterpret_cast<floatx4*>(dst + HD) = floatx4{most, l, unit, 0.0f};
     }
 }
 

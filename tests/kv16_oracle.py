@@ -10,10 +10,11 @@ def attention(q, data, tables, lens, starts, *, scale=None, softcap=None, slopes
 
     The bound of an element, u the half step of the type (eps / 2), p the probabilities:
       u |y|                             the result's own rounding;
-      u sum p |v|                       the probabilities' rounding before the product with V;
+      u (sum p |v| + |y|)               the probabilities' rounding before the product with V and before their sum;
       sum p E (|v| + |y|)               an error E of a score moves its probability by E.  E: the products' sum,
-                                        (hd + 8) 2^-24 of sum |q k| scale; the cap's tanh 2^-20 of the score (1.2e-7 of the
-                                        denominator over 0.245, twice); the distance's product and sum 2^-23 of it; three roundings of
+                                        (hd + 8) 2^-24 of sum |q k| scale; the cap's tanh 2^-20 of the score, and where
+                                        it is c - 2 c / (1 + e) of c up to 512, 2^-22 c (half the exponential's and the
+                                        reciprocal's last bits); the distance's product and sum 2^-23 of it; three roundings of
                                         the exponent, 2^-22 of its size;
       (n + 64) 2^-23 (sum p |v| + |y|)  fp32 sums of n terms, the exponential's last bit, the quotient;
       2^-24                             fp16's smallest step.
@@ -47,7 +48,7 @@ def attention(q, data, tables, lens, starts, *, scale=None, softcap=None, slopes
             x = rows[:, h] @ k.t().contiguous() * scale
             err = (rows[:, h].abs() @ k.abs().t().contiguous()) * scale * (hd + 8) * 2.0**-24
             if softcap is not None:
-                err = err + x.abs() * 2.0**-20
+                err = err + x.abs() * 2.0**-20 + (softcap * 2.0**-22 if softcap <= 512 else 0.0)
                 x = softcap * torch.tanh(x / softcap)
             if slopes is not None:
                 bias = slopes[h].double() * (i - j).abs()
@@ -62,7 +63,7 @@ def attention(q, data, tables, lens, starts, *, scale=None, softcap=None, slopes
             a = p @ v0.abs()
             pe = torch.where(p > 0, p * err, 0.0)
             y[lo:hi, h] = o
-            bound[lo:hi, h] = (u * (o.abs() + a) * 1.01 + pe @ v0.abs() + pe.sum(1, keepdim=True) * o.abs()
+            bound[lo:hi, h] = (u * (2 * o.abs() + a) * 1.01 + pe @ v0.abs() + pe.sum(1, keepdim=True) * o.abs()
                                + (n + 64) * 2.0**-23 * (a + o.abs()) + 2.0**-24)
     return y, bound
 
