@@ -382,6 +382,31 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_decode_kernel(Kv16AttnAr
 
 // ---- many columns: tiles ---------------------------------------------------------------
 
+// Two and four direct loads to neighbouring kilobytes of LDS, from as many of memory: the instruction's offset counts in
+// both, and M0 is written once (awq_device.h, buffer_load_lds_x4).
+__device__ __forceinline__ void buffer_load_lds_2x4(u32x4 rsrc, uint32_t v0, uint32_t v1, uint32_t lds_base) {
+    asm volatile(
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %0, %2, 0 offen lds\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen offset:1024 lds"
+        :
+        : "v"(v0), "v"(v1), "s"(rsrc), "s"(lds_base)
+        : "memory", "m0");
+}
+__device__ __forceinline__ void buffer_load_lds_4x4(u32x4 rsrc, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3,
+                                                    uint32_t lds_base) {
+    asm volatile(
+        "s_mov_b32 m0, %5\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %0, %4, 0 offen lds\n\t"
+        "buffer_load_dwordx4 %1, %4, 0 offen offset:1024 lds\n\t"
+        "buffer_load_dwordx4 %2, %4, 0 offen offset:2048 lds\n\t"
+        "buffer_load_dwordx4 %3, %4, 0 offen offset:3072 lds"
+        :
+        : "v"(v0), "v"(v1), "v"(v2), "v"(v3), "s"(rsrc), "s"(lds_base)
+        : "memory", "m0");
+}
 // The 16-byte chunks of a token's row in LDS are swizzled by this.  An operand of K is
 // one chunk of 32 tokens, a transposing read of V four neighbouring chunks of four
 // tokens each: both touch every bank once.
@@ -393,16 +418,30 @@ __device__ __forceinline__ constexpr int swizzle(int token) {
 // One workgroup: 128 columns of one kv head, 32 a wave, over an item's tokens in tiles of
 // 64.  K and V go from memory to LDS without passing registers, the next tile's under
 // this one's products: two buffers and one barrier a tile.  V is transposed as it is
-// read (ds_read_b64_tr_b16).
-template <int HD, bool BF16, bool SHAPED>
-__global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs a) {
+// read (ds_read_b64_tr_b16).  Of a tile the scores' maximum comes first; then each exponential is taken under a
+// product of the next tile's scores, which need the matrix unit and not these registers.  Products of 32 columns
+// because a wave then reads each operand of K and V once for 32 columns: with 16, LDS would give them at
+// twice the rate it has.
+//
+// What bounds it: instructions.  The 64 x 32 exponentials and the steps around them take a wave as long as its
+// products, and two waves of a SIMD overlap the two only in part.  A prompt of 6001 rows, 28 heads of 128 over 4,
+// is 258 GFLOP in 306 us, 844 TFLOP/s, where a large product of a library reaches 1152; of zeros, at the clock that less power
+// allows, it took 252.  Behind them each workgroup costs 6 us of finding its item, pages, query and first tile,
+// so with few tiles the time is that: 256 rows take 16.5 us, 1024 36.
+//
+// PARTS = 2: two groups of four waves take every other tile and meet through LDS, where whole workgroups of
+// four would be one round and leave CUs half empty (attention_plan16).  Prompts of 1200 / 1777 / 2300 rows: 31.5 / 48 / 63 us
+// against 36 / 55 / 69; with 6001, 349 against 311, for eight waves meet at each barrier.
+template <int HD, bool BF16, bool SHAPED, int PARTS>
+__global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnArgs a) {
     constexpr int kKS = HD / 16;                         // k-steps of S
     constexpr int kDb = HD / 32;                         // blocks of V's columns
     constexpr int kChunks = HD / 8;
     constexpr int kLoads = 16 * HD * 2 / 1024;           // of a wave: 16 tokens of K or V
     constexpr int kHalf = kTileKeys * HD;                // elements of K or V in a buffer
-    __shared__ __align__(1024) uint16_t k_lds[2][kHalf], v_lds[2][kHalf];
-    __shared__ __align__(8) uint16_t odd_lds[2][kWaves];
+    // [group of waves][stage]; at the end the second group's sums
+    __shared__ __align__(1024) uint16_t kv_lds[PARTS][2][2 * kHalf];
+    __shared__ __align__(8) uint16_t odd_lds[PARTS][2][4];
 
     Item it;
     const int kvh = a.s.kvh, g = blockIdx.x % kvh, item = blockIdx.x / kvh;
@@ -413,7 +452,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
     if (g == 0) write_records(a, it, true);
     const int group = a.nh / kvh;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6 & 3), part = PARTS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int col = lane & 31, half = lane >> 5;
     // The last blocks, which see the most tokens, start first.
     const int block = it.blocks - 1 - it.rel % it.blocks, split = it.rel / it.blocks;
@@ -460,7 +499,11 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
     int start = it.first + split * it.chunk;
     const int end = item_end(start, it.chunk, wg_hi);
     if (start < wg_lo) start = wg_lo / kTileKeys * kTileKeys;
-    const int tiles = end > start ? (end - start + kTileKeys - 1) / kTileKeys : 0;
+    const int all_tiles = end > start ? (end - start + kTileKeys - 1) / kTileKeys : 0;
+    // Tile `tile` of this group is the (PARTS tile + part)-th.
+    const int steps = (all_tiles + PARTS - 1) / PARTS, tiles = (all_tiles + PARTS - 1 - part) / PARTS;
+    start += part * kTileKeys;
+    constexpr int kStep = PARTS * kTileKeys;
 
     // Loads: wave w brings tokens 16 w .. of the tile.  A place past the
     // last token, or in a page outside the cache, lies past its resource's end and reads as zeros.
@@ -484,7 +527,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
     const uint32_t page_bytes = (uint32_t)(2 * kvh * a.s.block());      // of all heads: 2^29 at most
     const int r0 = lane / kChunks;                       // a load's rows begin with this lane's token
     const uint32_t l_ofs = r0 * (HD * 2) + ((lane % kChunks) ^ swizzle<HD>(r0)) * 16;
-    const uint32_t k_to = lds_addr(&k_lds[0][0]) + wave * (16 * HD * 2), v_to = lds_addr(&v_lds[0][0]) + wave * (16 * HD * 2);
+    const uint32_t k_to = lds_addr(&kv_lds[0][0][0]) + part * (8 * kHalf) + wave * (16 * HD * 2), v_to = k_to + 2 * kHalf;
     struct Place {                                       // of this wave's tokens of a tile
         uint64_t at;
         int tokens;
@@ -505,13 +548,17 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
         return p;
     };
     auto load = [&](uint64_t at, int tokens, uint32_t to) {
-        const u32x4 r = raw_rsrc(reinterpret_cast<const void*>(at), tokens * (HD * 2));
-        constexpr uint32_t kFlip = HD == 128 ? 16 : 32;  // the swizzle of the tokens of a load after
+        u32x4 r = raw_rsrc(reinterpret_cast<const void*>(at), tokens * (HD * 2));
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) buffer_load_lds_x4(r, (l_ofs ^ (kFlip * i)) + 1024 * i, 0, to + 1024 * i);
+        for (int i = 0; i < 3; ++i) r[i] = (uint32_t)__builtin_amdgcn_readfirstlane(r[i]);   // (the same for the wave)
+        constexpr uint32_t kFlip = HD == 128 ? 16 : 32;  // the swizzle of the tokens of a load after
+        if constexpr (kLoads == 4)
+            buffer_load_lds_4x4(r, l_ofs, l_ofs ^ kFlip, l_ofs ^ (2 * kFlip), l_ofs ^ (3 * kFlip), to);
+        else
+            buffer_load_lds_2x4(r, l_ofs, l_ofs ^ kFlip, to);
     };
-    auto load_k = [&](const Place& p, int stage) { load(p.at, p.tokens, k_to + stage * (2 * kHalf)); };
-    auto load_v = [&](const Place& p, int stage) { load(p.at + ((HD * 2) << log2), p.tokens, v_to + stage * (2 * kHalf)); };
+    auto load_k = [&](const Place& p, int stage) { load(p.at, p.tokens, k_to + stage * (4 * kHalf)); };
+    auto load_v = [&](const Place& p, int stage) { load(p.at + ((HD * 2) << log2), p.tokens, v_to + stage * (4 * kHalf)); };
     Place now = {}, next = {};                           // of this tile and the next
     if (tiles > 0) {
         now = locate(start);
@@ -519,7 +566,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
         load_v(now, 0);
     }
     if (tiles > 1) {
-        next = locate(start + kTileKeys);
+        next = locate(start + kStep);
         load_k(next, 1);
     }
 
@@ -553,9 +600,9 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
 
     // Operand addresses: token col (+ 32) and chunk 2 s + half of K; of V, lane 4 m + j of
     // 16 supplies four columns of token 4 half + m, and its group's other half of the 32 columns.
-    const uint32_t k_at = lds_addr(&k_lds[0][0]) + col * (HD * 2) + (half ^ swizzle<HD>(col)) * 16;
+    const uint32_t k_at = lds_addr(&kv_lds[0][0][0]) + part * (8 * kHalf) + col * (HD * 2) + (half ^ swizzle<HD>(col)) * 16;
     const int vm = 4 * half + (lane >> 2 & 3), vj = lane & 3;
-    const uint32_t v_at = lds_addr(&v_lds[0][0]) + vm * (HD * 2) + ((2 * (lane >> 4 & 1) + (vj >> 1)) ^ swizzle<HD>(vm)) * 16 + (vj & 1) * 8;
+    const uint32_t v_at = lds_addr(&kv_lds[0][0][0]) + part * (8 * kHalf) + 2 * kHalf + vm * (HD * 2) + ((2 * (lane >> 4 & 1) + (vj >> 1)) ^ swizzle<HD>(vm)) * 16 + (vj & 1) * 8;
 
     // A score s counts 2^(s unit + ref), scaled by kPScale: the sum is one fused step, rounded once.  Where ref is
     // large (`big`, for the whole wave) its own rounding would show; there it is (s - m) unit.
@@ -572,7 +619,7 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
     // Addresses of a stage are formed from one opaque register each tile: sixteen of them, hoisted, would be too many.
     typedef const __attribute__((address_space(3))) u32x4* lds16;
     auto in_stage = [&](uint32_t at, int stage) {
-        at += stage * (2 * kHalf);
+        at += stage * (4 * kHalf);
         asm volatile("" : "+v"(at));
         return at;
     };
@@ -597,11 +644,11 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_tile_kernel(Kv16AttnArgs
     };
     if (tiles > 0) all_scores(0);
     for (int tile = 0; tile < tiles; ++tile) {
-        const int key0 = start + tile * kTileKeys;
-        char* v_base = reinterpret_cast<char*>(&v_lds[tile & 1][0]);
+        const int key0 = start + tile * kStep;
+        char* v_base = reinterpret_cast<char*>(&kv_lds[part][tile & 1][kHalf]);
         Place after = {};
-        if (tile + 2 < tiles) after = locate(key0 + 2 * kTileKeys);
-asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (tile + 2 < tiles) after = locate(key0 + 2 * kStep);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what this wave has under way: the tile's V, the next one's K
         // Where some column does not see all of the tile's tokens, a value of V that is not finite must
         // not meet its probability of zero: each wave takes such values out of the tokens it
         // brought, and the rows that see them get NaN by their scores.
@@ -626,10 +673,9 @@ asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                         if (hit >> (kChunks * j) & ((1u << kChunks) - 1)) odd |= 1u << (kRows * i + j);
                 }
             }
-            if (lane == 0) odd_lds[tile & 1][wave] = (uint16_t)odd;
+            if (lane == 0) odd_lds[part][tile & 1][wave] = (uint16_t)odd;
         }
-        lds_barrier();
-                                           // the next tile's K and this one's V are there, the others read by all
+        lds_barrier();                                   // the next tile's K and this one's V are there, the others read by all
         const bool more = tile + 1 < tiles;
         const int stage = (tile + 1) & 1;
         if (tile + 2 < tiles) load_k(after, tile & 1);
@@ -643,7 +689,7 @@ asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         uint64_t bad = 0;                                // tokens that give NaN, a bit each
         if (edge) {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(&odd_lds[tile & 1][0]);
+            const u32x2 w = *reinterpret_cast<const u32x2*>(&odd_lds[part][tile & 1][0]);
             bad = (uint64_t)__builtin_amdgcn_readfirstlane(w.y) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane(w.x);
         }
         if (gone) {
@@ -695,17 +741,36 @@ asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 if (mine >> in & 1 && key >= sees.lo && key < sees.hi) s[i / 16][i % 16] = NAN;
             }
         }
-        if (__any(!some)) {
-            float mx = fmaxf(s[0][0], s[1][0]);
+        float mx = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+        if (__any(!some || big || fmaf(mx, unit, ref) > kMost)) {
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            if (!some && mx != -INFINITY) {
-                m = mx;
-                ref = kPScale<BF16> - mx * unit;
-                some = true;
+            float alpha = 1.0f;
+            if (!some) {
+                if (mx != -INFINITY) {
+                    m = mx;
+                    ref = kPScale<BF16> - mx * unit;
+                    some = true;
+                }
+            } else if (big) {
+                const float to = fmaxf(m, mx);
+                alpha = __builtin_amdgcn_exp2f((m - to) * unit);
+                m = to;
+            } else {
+                const float up = fmaf(mx, unit, ref) - kPScale<BF16>, to = ref - up;
+                m = up > 0.0f ? mx : (kPScale<BF16> - ref) / unit;
+                alpha = up > 0.0f ? __builtin_amdgcn_exp2f(to - ref) : 1.0f;
+                ref = up > 0.0f ? to : ref;
             }
             big = big || __any(fabsf(ref) > kBig);
+            l *= alpha;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < kDb; ++d) {
+                acc[d] *= alpha;
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         float y[32];
         if (!big) {
@@ -715,41 +780,10 @@ asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
             for (int i = 0; i < 32; ++i) y[i] = fmaf(s[i / 16][i % 16] - m, unit, kPScale<BF16>);
         }
-        // (here, where the scores' registers are free)
         const uint32_t k_now = in_stage(k_at, stage), v_now = in_stage(v_at, tile & 1);
         if (more) {
             read_k(k_now, 0);
             if (!SHAPED) read_k(k_now, 1);               // (shaped scores have more else in registers)
-        }
-        float top = fmaxf(y[0], y[1]);
-#pragma unroll
-        for (int i = 2; i < 32; i += 2) top = fmaxf(top, fmaxf(y[i], y[i + 1]));
-        if (__any(top > kMost)) {
-            top = fmaxf(top, __shfl_xor(top, 32));
-            float up = top > kPScale<BF16> ? top - kPScale<BF16> : 0.0f;
-            if (big) {
-                const float mn = m + up / unit;
-                up = (mn - m) * unit;
-                m = mn;
-            } else {
-                const float cn = ref - up;
-                up = ref - cn;
-                ref = cn;
-                if (__any(fabsf(ref) > kBig)) {
-                    m = (kPScale<BF16> - ref) / unit;
-                    big = true;
-                }
-            }
-            const float alpha = __builtin_amdgcn_exp2f(-up);
-            l *= alpha;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] -= up;
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int d = 0; d < kDb; ++d) {
-                acc[d] *= alpha;
-                __builtin_amdgcn_sched_barrier(0);
-            }
         }
         // V's operands: product j is of k-step j / kDb and column block j % kDb.
         constexpr int kProducts = 4 * kDb, kAhead = 4;
@@ -799,10 +833,49 @@ asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
     }
 
+    float most = !some ? -INFINITY : big ? m : (kPScale<BF16> - ref) / unit;
+    if constexpr (PARTS == 2) {
+        // The groups meet: the second's sums through LDS, each weighted by its reference.
+        floatx4* meet = reinterpret_cast<floatx4*>(&kv_lds[0][0][0]) + wave * (64 * (4 * kDb + 1)) + lane;
+        static_assert(sizeof(kv_lds) >= 4 * 64 * (4 * kDb + 1) * sizeof(floatx4), "room for a group's sums");
+        if (tiles < steps) lds_barrier();                // the other group has one more
+        if (steps > 0) {
+            lds_barrier();                               // the last tiles are read by all
+            if (part == 1) {
+#pragma unroll
+                for (int d = 0; d < kDb; ++d)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        meet[64 * (4 * d + j)] = floatx4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+                meet[64 * 4 * kDb] = floatx4{most, l, ref, big ? 1.0f : 0.0f};
+            }
+            lds_barrier();
+        }
+        if (part == 1) return;
+        if (steps > 0) {
+            const floatx4 other = meet[64 * 4 * kDb];
+            // Powers of two that bring each group's sums to the larger reference.  (One without a score has sums of
+            // 0, or of NaN.)
+            float up = 0.0f;
+            if (some && other[0] != -INFINITY) up = big || other[3] != 0.0f ? (other[0] - most) * unit : ref - other[2];
+            const float mine = __builtin_amdgcn_exp2f(-fmaxf(up, 0.0f)), add = __builtin_amdgcn_exp2f(fminf(up, 0.0f));
+            most = fmaxf(most, other[0]);
+            l = l * mine + other[1] * add;
+#pragma unroll
+            for (int d = 0; d < kDb; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const floatx4 o = meet[64 * (4 * d + j)];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[d][4 * j + r] = acc[d][4 * j + r] * mine + o[r] * add;
+                }
+        }
+    }
     l += __shfl_xor(l, 32);
     if (c >= all_cols) return;
     // This lane: columns 32 d + 8 j + 4 half + r of the head.
     if (it.splits == 1) {
+        const float inv = 1.0f / l;
         uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + ((int64_t)(it.r.row0 + row) * a.nh + head) * HD + 4 * half;
 #pragma unroll
         for (int d = 0; d < kDb; ++d)
@@ -810,7 +883,7 @@ asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             for (int j = 0; j < 4; ++j) {
                 float y[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = blind ? 0.0f : acc[d][4 * j + r] / l;
+                for (int r = 0; r < 4; ++r) y[r] = blind ? 0.0f : acc[d][4 * j + r] * inv;
                 *reinterpret_cast<u32x2*>(dst + 32 * d + 8 * j) = u32x2{pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3])};
             }
     } else {
@@ -821,7 +894,6 @@ asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             for (int j = 0; j < 4; ++j)
                 *reinterpret_cast<floatx4*>(dst + 32 * d + 8 * j + 4 * half) =
                     floatx4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
-        const float most = !some ? -INFINITY : big ? m : (kPScale<BF16> - ref) / unit;
         if (half == 0) *reinterpret_cast<floatx4*>(dst + HD) = floatx4{most, l, unit, 0.0f};
     }
 }
@@ -837,10 +909,11 @@ __global__ __launch_bounds__(kThreads) void awq_kv16_combine_kernel(Kv16AttnArgs
 
 template <int HD, bool BF16, bool SHAPED>
 hipError_t launch(Kv16AttnArgs a, hipStream_t stream) {
-    const AttentionPlan p = attention_plan<k16Cols>(a.requests, a.total, a.max_query, a.nh / a.s.kvh, a.s.kvh);
+    const AttentionPlan16 p = attention_plan16(a.requests, a.total, a.max_query, a.nh / a.s.kvh, a.s.kvh);
     a.limit = p.limit;
     a.decode_target = p.decode_target;
     a.tile_target = p.tile_target;
+    a.combine = p.combine;
     a.records = reinterpret_cast<i32x4*>(a.part);
     a.part += (size_t)a.total * (sizeof(i32x4) / sizeof(float));
     a.tile_part = a.part + p.decode_items * a.s.kvh * kCols * (HD + a.kExtra);
@@ -851,8 +924,8 @@ hipError_t launch(Kv16AttnArgs a, hipStream_t stream) {
         if (e != hipSuccess) return e;
     }
     if (p.tile) {
-        hipLaunchKernelGGL((awq_kv16_tile_kernel<HD, BF16, SHAPED>), dim3((unsigned)(p.tile_items * a.s.kvh)), dim3(kThreads), 0, stream,
-                           a);
+        auto kernel = p.tile_parts == 2 ? awq_kv16_tile_kernel<HD, BF16, SHAPED, 2> : awq_kv16_tile_kernel<HD, BF16, SHAPED, 1>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(p.tile_items * a.s.kvh)), dim3(256 * p.tile_parts), 0, stream, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -869,12 +942,12 @@ hipError_t launch(Kv16AttnArgs a, hipStream_t stream) {
 
 // A launch holds 2^32 threads.
 bool kv16_attn_fits(int requests, int total, int max_query, int nh, int kvh) {
-    const AttentionPlan p = attention_plan<k16Cols>(requests, total, max_query, nh / kvh, kvh);
-    return (p.decode_items > p.tile_items ? p.decode_items : p.tile_items) * kvh < ((int64_t)1 << 32) / kThreads;
+    const AttentionPlan16 p = attention_plan16(requests, total, max_query, nh / kvh, kvh);
+    return (p.decode_items > p.tile_items ? p.decode_items : p.tile_items) * kvh < ((int64_t)1 << 32) / 512;
 }
 
 size_t kv16_attn_workspace(int requests, int total, int max_query, int nh, int kvh, int hd) {
-    return part_bytes(attention_plan<k16Cols>(requests, total, max_query, nh / kvh, kvh), total, kvh, hd + Kv16AttnArgs::kExtra);
+    return part_bytes(attention_plan16(requests, total, max_query, nh / kvh, kvh), total, kvh, hd + Kv16AttnArgs::kExtra);
 }
 
 hipError_t launch_kv16_attention(const Kv16AttnArgs& a, bool bf16, hipStream_t stream) {

@@ -83,6 +83,8 @@ constexpr int item_steps(int target, int64_t work, int all_blocks, int requests)
                : work == 0 ? 1 : work < most ? (int)((work + target - 1) / target) : kMost;
 }
 constexpr int request_splits(int steps, int item) { return (int)((uint32_t)(steps + item - 1) / (uint32_t)item); }
+// Steps of an item of that request with its items made alike: as many items, none longer.
+constexpr int even_steps(int steps, int splits) { return splits > 1 ? (int)((uint32_t)(steps + splits - 1) / (uint32_t)splits) : steps; }
 // Where an item ends that begins at `start`, of a block that sees `limit` tokens.
 constexpr int item_end(int start, int chunk, int limit) {
     return limit - start < chunk ? limit : start + chunk;   // start + chunk may pass 32 bits where limit does not
@@ -116,6 +118,32 @@ AttentionPlan attention_plan(int requests, int total, int max_query, int group, 
         p.tile_items = blocks + p.tile_target + 1;
     }
     p.combine = p.decode || p.tile_target;
+    return p;
+}
+
+// The same for the 16-bit cache, whose tiles have 128 columns: workgroups of four waves, two on a CU, or of eight
+// that share 128 columns' tokens.  Blocks that are fewer than half the places are split into one round of workgroups
+// and their sums joined by another launch; those that fit into the round as they are get eight waves each, and none joins.
+// One request, rows behind a context of 32768 tokens, split for four waves / for eight: 300 rows 179 / 192 us, 512 287 / 311,
+// 768 394 / 527 (its 42 blocks have 128 places a head or 64); prompts of 1200, 1777 and 2300 rows split / with
+// eight waves: 42 / 31.5, 61 / 48, 76 / 63 us.
+constexpr int kTile16Cols = 128, kRound16 = 512;
+struct AttentionPlan16 : AttentionPlan {
+    int tile_parts;                    // 2: eight waves share the tokens of 128 columns
+};
+inline AttentionPlan16 attention_plan16(int requests, int total, int max_query, int group, int kvh) {
+    AttentionPlan16 p = {attention_plan<kTile16Cols>(requests, total, max_query, group, kvh), 1};
+    if (p.tile_target) {
+        // One round of workgroups.  The blocks of one request are known, and so are their items; of several each
+        // block may come out with an item more than its share (item_steps takes half of them off).
+        const int64_t blocks = p.tile_items - p.tile_target - 1, all = kvh < kRound16 ? kRound16 / kvh : 1;
+        const int64_t mine = ((int64_t)(max_query < total ? max_query : total) * group + kTile16Cols - 1) / kTile16Cols;
+        const int64_t target = requests > 1 ? all - blocks / 2 : mine > 0 ? all / mine * mine : 1;
+        p.tile_target = (int)(target > (all + 3) / 4 ? target : (all + 3) / 4);
+        p.tile_items = blocks + p.tile_target + 1;
+    } else if (p.tile && p.tile_items * kvh <= kRound16) {
+        p.tile_parts = 2;
+    }
     return p;
 }
 

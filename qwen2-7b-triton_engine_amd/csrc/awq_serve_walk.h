@@ -6,6 +6,9 @@
 //   kTileCols                       columns of a tile workgroup
 //   first_key(rows, len)            the first token that a row of a request may see
 //   sees_none(b, row0, rows, len, i)   whether the i-th row of request b sees no token
+//   least_steps(steps, prompts)     steps of a tile item, from those that the target gives; prompts: nothing lies before the rows
+//   kEven                           whether a request's tile items are made alike
+//   combine                         whether the joining launch follows, and needs records
 //   kExtra                          floats of a column in `part` past its sums: its maximum, the sum of its exponentials, ..
 //   factor(column)                  what one of that maximum's counts in powers of two
 #pragma once
@@ -103,6 +106,7 @@ __device__ __forceinline__ bool find_item(const Args& a, int want, int target, I
         }
         const int blocks_sum = a.requests == 1 ? 0 : __builtin_amdgcn_readlane(wave_scan32(all_blocks), 63);
         m = item_steps<KEYS>(target, all, blocks_sum, a.requests);
+        if (COLS != kCols) m = a.least_steps(m, __all(r.rows >= r.len));
         m = __builtin_amdgcn_readfirstlane(m);
     }
     int before = 0;
@@ -120,8 +124,8 @@ __device__ __forceinline__ bool find_item(const Args& a, int want, int target, I
             it.r = Request{pick(r.row0), pick(r.rows), pick(r.len)};
             it.b = b0 + at;
             it.first = a.first_key(it.r.rows, it.r.len) / KEYS * KEYS;
-            it.chunk = m * KEYS;
             it.splits = pick(splits);
+            it.chunk = (COLS != kCols && Args::kEven ? even_steps(pick(steps), it.splits) : m) * KEYS;
             it.blocks = pick(blocks);
             it.base = pick(upto - mine);
             it.rel = want - it.base;
@@ -140,7 +144,7 @@ struct RowRecord {
 // Written by the first item of a request.
 template <class Args>
 __device__ __forceinline__ void write_records(const Args& a, const Item& it, bool tile) {
-    if (it.rel != 0 || blockIdx.y != 0) return;
+    if (!a.combine || it.rel != 0 || blockIdx.y != 0) return;
     for (int i = threadIdx.x; i < it.r.rows; i += (int)blockDim.x) {
         const bool blind = a.sees_none(it.b, it.r.row0, it.r.rows, it.r.len, i);
         a.records[it.r.row0 + i] = i32x4{i, tile ? ~it.base : it.base, it.blocks,
@@ -156,6 +160,7 @@ __device__ __forceinline__ void fill_rows(const Args& a) {
     auto fill = [&](int lo, int hi, uint32_t w) {        // a word of two elements everywhere
         u32x4* out = reinterpret_cast<u32x4*>(a.out);
         for (int64_t i = (int64_t)lo * pieces + threadIdx.x; i < (int64_t)hi * pieces; i += blockDim.x) out[i] = u32x4{w, w, w, w};
+        if (!a.combine) return;
         for (int i = lo + (int)threadIdx.x; i < hi; i += (int)blockDim.x) a.records[i] = i32x4{0, 0, 0, 1};
     };
     int start = 0, first = 0, end = 0;                   // of all requests' rows

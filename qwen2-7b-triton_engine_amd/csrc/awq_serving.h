@@ -67,6 +67,8 @@ struct Kv4AttnArgs {
     int decode_target, tile_target;   // items of one kv head that the kernels aim at
     // what awq_serve_walk.h asks for
     static constexpr int kTileCols = 64, kExtra = 2;
+    static constexpr bool kEven = false, combine = true;
+    __device__ __forceinline__ int least_steps(int steps, bool) const { return steps; }
     __device__ __forceinline__ int first_key(int, int) const { return 0; }
     __device__ __forceinline__ bool sees_none(int, int, int rows, int len, int i) const { return (int64_t)len - rows + i < 0; }
     __device__ __forceinline__ float factor(const float*) const { return scale * 1.4426950408889634f; }
@@ -111,8 +113,16 @@ struct Kv16AttnArgs {
     float* tile_part;
     i32x4* records;             // [total]
     int limit, decode_target, tile_target;
+    bool combine;               // whether the joining launch follows
     // what awq_serve_walk.h asks for
-    static constexpr int kTileCols = 128, kExtra = 4;   // maximum, sum, unit, nothing
+    static constexpr int kTileCols = kTile16Cols, kExtra = 4;   // maximum, sum, unit, nothing
+    static constexpr bool kEven = true;
+    // Four tiles, sixteen of prompts, whose blocks see half of their items on average.  4 / 16: 300 rows behind
+    // 1748 tokens 34 / 40 us, three chunks of up to 389 rows 42 / 46; prompts of 700 tokens 34 / 28, 1024 44 / 36.
+    __device__ __forceinline__ int least_steps(int steps, bool prompts) const {
+        const int least = prompts ? 16 : 4;
+        return steps < least ? least : steps;
+    }
     __device__ __forceinline__ int first_key(int rows, int len) const {
         return first_token(window, rows, len, walked_tokens(width, s.page_log2, len));
     }

@@ -6,7 +6,6 @@ using namespace awq;
 
 namespace {
 
-constexpr int kTile16Cols = 128;
 struct Kernel {
     long long items, most_splits, wrong;
 };
@@ -57,7 +56,7 @@ Kernel walk(int requests, const int* starts, const int* lens, int total, int max
 // out: decode items, its grid, most splits, wrong; the same of the tile kernel; whether that has places for sums.
 extern "C" void attention16_items(int requests, const int* starts, const int* lens, int total, int max_query, int group,
                                   int kvh, int width, int page_log2, int window, long long* out) {
-    const AttentionPlan p = attention_plan<kTile16Cols>(requests, total, max_query, group, kvh);
+    const AttentionPlan16 p = attention_plan16(requests, total, max_query, group, kvh);
     const Kernel d = walk<kCols, kKeys>(requests, starts, lens, total, max_query, group, width, page_log2, window, p.limit,
                                         p.decode_target);
     const Kernel t = walk<kTile16Cols, kTileKeys>(requests, starts, lens, total, max_query, group, width, page_log2, window,
