@@ -72,6 +72,16 @@ def test_the_model_s_sizes(gpu, t):
     assert max((x.double() - y).abs().max().item() for x, y in zip(got, want)) <= 2 * math.sqrt(k) * 2.0**-24 * size
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("t", [130, 160, 161, 319, 320, 321, 384, 385, 640, 641, 799])
+def test_tiles_of_tokens(gpu, t, dtype):
+    """Widths of the tiles of many tokens and their neighbours, each token its own target."""
+    g = _gen(gpu, t)
+    hidden, weight = _whole(g, t, 777, 128, dtype)
+    targets = torch.arange(t, device=gpu) % 777
+    _check(token_logprobs(hidden, weight, targets), _reference(hidden, weight, targets))
+
+
 @pytest.mark.parametrize("t", [1, 50, 90, 300])
 def test_likely_tokens_and_large_logits(gpu, t):
     """Logits of thousands, a target that has nearly all of the probability: z - lse must not lose it."""
