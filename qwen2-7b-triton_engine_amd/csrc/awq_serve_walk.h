@@ -319,8 +319,8 @@ __device__ __forceinline__ void combine_items(const Args& a) {
     }
 }
 
-// Workgroups of the combining launch at most, one round of them: 5 long chunks with nothing to join, 5000 rows of 28 heads
-// (16-bit cache), 50.1 us with 2048 and 52.7 with 8192; three with all to join 42.0 and 42.5.
+// Workgroups of the combining launch at most, one round of them: 5 chunks of up to 700 rows, 32 heads, nothing to join
+// (16-bit cache) 50.1 us with 2048 and 52.7 with 8192; 3 of up to 389, all to join, 42.0 and 42.5.
 constexpr int kCombineGroups = 2048;
 constexpr int kFewUnits = 512;         // rows times heads that get four waves each there
 
