@@ -105,18 +105,28 @@ __global__ __launch_bounds__(L::kThreads, L::kPerCu * L::kWaves / 4) void awq_lo
         lds_barrier();                                   // the step is there, and the stage before it read by all
         if (step + S - 1 < steps) issue(step + S - 1);
         const unsigned char* st = smem + step % S * L::kStage;
+        u32x4 w[2][FV], x[2][FT];
+        auto read = [&](int h) {
+#pragma unroll
+            for (int v = 0; v < FV; ++v) w[h][v] = *reinterpret_cast<const u32x4*>(st + (wv * FV + v) * 2048 + (frag ^ (64 * h)));
+#pragma unroll
+            for (int t = 0; t < FT; ++t)
+                x[h][t] = *reinterpret_cast<const u32x4*>(st + L::BV * 128 + (wt * FT + t) * 2048 + (frag ^ (64 * h)));
+        };
+        // The second half's operands are read under the first's products, and a wave that has all of its operands goes
+        // before one that is reading: 2047 tokens 1951 us for 2019 without, 512 535 for 561.
+        read(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            u32x4 w[FV], x[FT];
-#pragma unroll
-            for (int v = 0; v < FV; ++v) w[v] = *reinterpret_cast<const u32x4*>(st + (wv * FV + v) * 2048 + (frag ^ (64 * h)));
-#pragma unroll
-            for (int t = 0; t < FT; ++t)
-                x[t] = *reinterpret_cast<const u32x4*>(st + L::BV * 128 + (wt * FT + t) * 2048 + (frag ^ (64 * h)));
+            if (h == 0) read(1);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int t = 0; t < FT; ++t)
 #pragma unroll
-                for (int v = 0; v < FV; ++v) acc[v][t] = mfma16<BF16>(w[v], x[t], acc[v][t]);
+                for (int v = 0; v < FV; ++v) acc[v][t] = mfma16<BF16>(w[h][v], x[h][t], acc[v][t]);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
