@@ -101,8 +101,11 @@ __device__ __forceinline__ u32x4 scaled_bf16(u32x4 w, float up) {
     for (int i = 0; i < 4; ++i) w[i] = pack2<true>(low16<true>(w[i]) * up, high16<true>(w[i]) * up);
     return w;
 }
-// What multiplies a product of the scaled query: kept finite (2^127 under a large scale passes fp32 here).
-__device__ __forceinline__ float unit_of(float factor, int exp) { return fminf(__builtin_ldexpf(factor, -exp), __FLT_MAX__); }
+// What multiplies a product of the scaled query: kept finite (2^127 under a large scale passes fp32 here) and above zero
+// (a masked score times it is -infinity; 2^-149 of any product is nothing beside 1).
+__device__ __forceinline__ float unit_of(float factor, int exp) {
+    return fminf(fmaxf(__builtin_ldexpf(factor, -exp), 0x1p-149f), __FLT_MAX__);
+}
 
 // c tanh(x / c) as c - 2 c / (1 + e^(2 x / c)): in absolute terms it errs by a few 2^-24 c, nothing beside the
 // probabilities' rounding while c is below 2^9; above, where small scores matter beside a large cap, the series
@@ -598,7 +601,7 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
     // Shaped scores are formed in powers of two, plain ones are products of the scaled query.
     const float unit = SHAPED ? 1.0f : unit_of(a.scale * kLog2e, exp);
     const float natural = unit_of(a.scale, exp), inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
-    const float cap2 = a.softcap * kLog2e, cap_in = unit_of(a.scale, exp) * inv_cap * 2.8853900817779268f;
+    const float cap2 = a.softcap * kLog2e, cap_in = fminf(unit_of(a.scale, exp) * inv_cap * 2.8853900817779268f, __FLT_MAX__);
     const float slope = SHAPED && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
     const int pos = it.r.len - it.r.rows + row;
     wait_vm_stores();                                    // the query, here: in the loop its wait would be one for the next tiles

@@ -232,6 +232,23 @@ def test_extremes(gpu, rows):
         assert (out.double().view(y.shape) - y).abs().max() <= 2.0**-8 * y.abs().max()
 
 
+@pytest.mark.parametrize("rows", [1, 200])
+def test_products_near_fp32_s_smallest_and_caps_far_below(gpu, rows):
+    """Scores that vanish beside 1, down to scales that no fp32 number but a subnormal holds, and a cap of 2^-100 over the
+    largest scores and over scores of 0: all tokens weigh alike, masked ones nothing.  One tile, several, split."""
+    g = _gen(gpu, 17)
+    for tokens in (300, 5000):
+        q, cache, tables, lens, starts = args = _batch(g, [(tokens, rows), (1, 1)], nh=2, kvh=1, hd=128, page=64)
+        for kw in ({"scale": 1e-44}, {"scale": 1e-37, "softcap": 2.0**-100}):
+            O.check(_call(*args, **kw), *O.attention(q, cache.data, tables, lens, starts, **kw), f"{tokens} {kw}")
+        half = Kv16Cache.of(cache.data.to(torch.bfloat16))
+        half.k[:, :, 5:9] = 0
+        for power, kw in ((-100, {"scale": 1e-30}), (-100, {"scale": 1e-30, "softcap": 5.0}), (125, {"softcap": 2.0**-100})):
+            far = (q.float() * 2.0**power).to(torch.bfloat16)
+            O.check(_call(far, half, tables, lens, starts, **kw), *O.attention(far, half.data, tables, lens, starts, **kw),
+                    f"{tokens} 2^{power} {kw}")
+
+
 def test_strides_and_streams(gpu):
     """Rows of a wider tensor, an unaligned view, another stream than the tensors' own."""
     g = _gen(gpu, 8)
