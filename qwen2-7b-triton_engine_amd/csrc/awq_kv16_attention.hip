@@ -83,9 +83,10 @@ __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
 // The probabilities' scale in powers of two, and how far above it a score may lie before the running maximum is
 // raised: of 32 columns one or another passes its maximum in many tiles, and each time the sums are rescaled.
 // fp16 holds values up to 2^16 and 11 bits down to 2^-14: 2^8 leaves both room for 2^7.5 above and
-// all bits down to 2^-22 of the maximum; bf16 has the range of fp32.
+// all bits down to 2^-22 of the maximum; bf16 has the range of fp32, and 2^-32, 2^-16 with what lies above, keeps the sums of
+// values near its largest inside fp32 for 2^16 tokens of one weight, and 2^94 of range below.
 template <bool BF16>
-constexpr float kPScale = BF16 ? 0.0f : 8.0f;
+constexpr float kPScale = BF16 ? -32.0f : 8.0f;
 template <bool BF16>
 constexpr float kSlack16 = BF16 ? 16.0f : 7.5f;
 
@@ -142,8 +143,11 @@ __device__ __forceinline__ float add2(uint32_t p, float sum) {
 // with few the chain of lengths, page, K, V, parts: one of 1100 tokens takes 7.2 us and the joining launch 3.9.
 // About 512, 768, 1024 and 1536 items took 65.8, 66.0, 67.1 and 66.0 us there, 26.6, 26.3, 27.9 and 29.5 for 4 requests of up
 // to 16384 tokens.
+//
+// Three waves a SIMD, 170 registers each, but for heads of 128 in fp16 with shaped scores, which would spill (175).  With
+// two, a window of 4096 over 8 requests, 32 heads over 8, took 30.7 us for 27.9.
 template <int HD, bool BF16, bool SHAPED>
-__global__ __launch_bounds__(kThreads, 2) void awq_kv16_decode_kernel(Kv16AttnArgs a) {
+__global__ __launch_bounds__(kThreads, HD == 128 && !BF16 && SHAPED ? 2 : 3) void awq_kv16_decode_kernel(Kv16AttnArgs a) {
     constexpr int kSteps = HD / 32;
     constexpr int VC = HD / 16;            // V columns per lane
     constexpr int VW = VC / 2;             // words of them
@@ -312,12 +316,14 @@ __global__ __launch_bounds__(kThreads, 2) void awq_kv16_decode_kernel(Kv16AttnAr
             m = mn;
         }
         const float ref = m == -INFINITY ? 0.0f : m;     // nothing yet: every exponential is 0
+        float p_scale = kPScale<BF16>;
+        asm("" : "+s"(p_scale));                         // in a scalar register: a vector one is one too many
         float p[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                p[4 * h + r] = __builtin_amdgcn_exp2f(fmaf(s[h][r] - ref, unit, kPScale<BF16>));
+                p[4 * h + r] = __builtin_amdgcn_exp2f(fmaf(s[h][r] - ref, unit, p_scale));
                 l += p[4 * h + r];
             }
         u32x4 phi, plo;

@@ -249,6 +249,22 @@ def test_products_near_fp32_s_smallest_and_caps_far_below(gpu, rows):
                     f"{tokens} 2^{power} {kw}")
 
 
+@pytest.mark.parametrize("rows", [1, 200])
+@pytest.mark.parametrize("tokens", [300, 5000])
+def test_values_near_bf16_s_largest_and_far_below(gpu, rows, tokens):
+    """Their weighted mean is no larger than they are: no sum on the way may pass fp32."""
+    g = _gen(gpu, 18)
+    q, cache, tables, lens, starts = _batch(g, [(tokens, rows), (1, 1)], nh=2, kvh=1, hd=128, page=64, dtype="bf16")
+    for size in (3.38e38, 1e-15):
+        cache.v.copy_(torch.where(cache.v > 0, size, -size * 0.75))
+        cache.v[..., 0] = size
+        out = _call(q, cache, tables, lens, starts)
+        O.check(out, *O.attention(q, cache.data, tables, lens, starts), f"{size}")
+        # (of the small ones the bound's absolute term says nothing)
+        y, _ = O.attention(q, cache.data, tables, lens, starts)
+        assert ((out.double().view(y.shape) - y).abs() <= 2.0**-6 * size).all()
+
+
 def test_strides_and_streams(gpu):
     """Rows of a wider tensor, an unaligned view, another stream than the tensors' own."""
     g = _gen(gpu, 8)
