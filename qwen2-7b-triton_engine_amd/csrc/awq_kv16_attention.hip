@@ -430,6 +430,35 @@ __device__ __forceinline__ constexpr int swizzle(int token) {
     return HD == 128 ? (token & 3) << 2 | (token >> 2 & 3) : (token >> 1 & 1) << 2 | (token >> 2 & 3);
 }
 
+// Over some columns: the first and the last of their first tokens, and of the ends of what they see.  (Columns that see none
+// count in lo_max and hi_max alone, as 0.)
+struct Span {
+    int lo_min, lo_max, hi_min, hi_max;
+};
+// Of rows r0 .. r1 of a request, where no row has a first token of its own: both ends go up with the rows, and rows before the
+// request's first token see none.  Scalar work; over the lanes it took a workgroup 1.5 us.
+__device__ __forceinline__ Span rising_span(const Kv16AttnArgs& a, const Item& it, int n, int r0, int r1) {
+    const int none = it.r.rows - it.r.len;
+    if (r0 < none) r0 = none;
+    if (r0 > r1) return Span{n, 0, n, 0};
+    const auto x = a.range(it.b, it.r.row0, it.r.rows, it.r.len, r0), y = a.range(it.b, it.r.row0, it.r.rows, it.r.len, r1);
+    return Span{x.lo, y.lo, x.hi, y.hi};
+}
+template <class Op>
+__device__ __forceinline__ int wave_int(int v, Op op) {
+    v = op(v, __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true));    // quad_perm [1,0,3,2]
+    v = op(v, __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true));    // quad_perm [2,3,0,1]
+    v = op(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true));   // row_half_mirror
+    v = op(v, __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true));   // row_mirror
+    auto row = [&](int lane) { return __builtin_amdgcn_readlane(v, lane); };
+    return op(op(row(0), row(16)), op(row(32), row(48)));
+}
+__device__ __forceinline__ Span wave_span(const Span& s) {
+    auto least = [](int x, int y) { return x < y ? x : y; };
+    auto most = [](int x, int y) { return x > y ? x : y; };
+    return Span{wave_int(s.lo_min, least), wave_int(s.lo_max, most), wave_int(s.hi_min, least), wave_int(s.hi_max, most)};
+}
+
 // One workgroup: 128 columns of one kv head, 32 a wave, over an item's tokens in tiles of
 // 64.  K and V go from memory to LDS without passing registers, the next tile's under
 // this one's products: two buffers and one barrier a tile.  V is transposed as it is
@@ -474,46 +503,43 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
     const int all_cols = columns(a, it.r.rows), c0 = block * k16Cols;
     const int n = walked(a, it.r.len);
 
-    // Every wave looks at all columns of the workgroup, two a lane: their first and last tokens.
-    int wg_lo = n, wg_lo_max = 0, wg_hi = 0, wg_hi_min = n;
-#pragma unroll
-    for (int i = 0; i < k16Cols; i += 64) {
-        const int c = c0 + i + lane;
-        if (c < all_cols) {
-            const auto r = a.range(it.b, it.r.row0, it.r.rows, it.r.len, c / group);
-            wg_lo = r.hi ? min(wg_lo, r.lo) : wg_lo;
-            wg_lo_max = max(wg_lo_max, r.lo);
-            wg_hi_min = r.hi ? min(wg_hi_min, r.hi) : wg_hi_min;
-            wg_hi = max(wg_hi, r.hi);
-        }
-    }
     const int local = 32 * wave + col, c = c0 + local, cc = c < all_cols ? c : all_cols - 1;
     const int row = cc / group, head = g * group + cc % group;
+    // This lane's query: columns 16 s + 8 half .. of the head.  Asked for first: loads come back in order.
+    u32x4 q[kKS];
+    {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + row) * a.ld + (int64_t)head * HD + 8 * half;
+#pragma unroll
+        for (int s = 0; s < kKS; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s);
+        __builtin_amdgcn_sched_barrier(0);
+    }
     const auto sees = a.range(it.b, it.r.row0, it.r.rows, it.r.len, row);
     const bool blind = sees.hi == 0;
-    int lo_min = blind ? n : sees.lo, lo_max = blind ? 0 : sees.lo, hi_min = blind ? n : sees.hi, hi_max = sees.hi;
+    // What the workgroup's columns see, and the wave's.
+    Span wg, mine;
+    if (a.first) {
+        wg = Span{n, 0, n, 0};
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        wg_lo = min(wg_lo, __shfl_xor(wg_lo, d));
-        wg_lo_max = max(wg_lo_max, __shfl_xor(wg_lo_max, d));
-        wg_hi_min = min(wg_hi_min, __shfl_xor(wg_hi_min, d));
-        wg_hi = max(wg_hi, __shfl_xor(wg_hi, d));
-        lo_min = min(lo_min, __shfl_xor(lo_min, d));
-        lo_max = max(lo_max, __shfl_xor(lo_max, d));
-        hi_min = min(hi_min, __shfl_xor(hi_min, d));
-        hi_max = max(hi_max, __shfl_xor(hi_max, d));
+        for (int i = 0; i < k16Cols; i += 64) {          // two columns a lane
+            const int ci = c0 + i + lane;
+            if (ci < all_cols) {
+                const auto r = a.range(it.b, it.r.row0, it.r.rows, it.r.len, ci / group);
+                wg = Span{r.hi ? min(wg.lo_min, r.lo) : wg.lo_min, max(wg.lo_max, r.lo), r.hi ? min(wg.hi_min, r.hi) : wg.hi_min,
+                          max(wg.hi_max, r.hi)};
+            }
+        }
+        wg = wave_span(wg);
+        mine = wave_span(Span{blind ? n : sees.lo, sees.lo, blind ? n : sees.hi, sees.hi});
+    } else {
+        const int last = all_cols - 1, w0 = c0 + 32 * wave;
+        wg = rising_span(a, it, n, c0 / group, min(c0 + k16Cols - 1, last) / group);
+        mine = rising_span(a, it, n, min(w0, last) / group, min(w0 + 31, last) / group);
     }
-    wg_lo = __builtin_amdgcn_readfirstlane(wg_lo);
-    wg_lo_max = __builtin_amdgcn_readfirstlane(wg_lo_max);
-    wg_hi_min = __builtin_amdgcn_readfirstlane(wg_hi_min);
-    wg_hi = __builtin_amdgcn_readfirstlane(wg_hi);
-    lo_min = __builtin_amdgcn_readfirstlane(lo_min);
-    lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-    hi_min = __builtin_amdgcn_readfirstlane(hi_min);
-    hi_max = __builtin_amdgcn_readfirstlane(hi_max);
+    const int wg_lo_max = wg.lo_max, wg_hi_min = wg.hi_min;
+    const int lo_min = mine.lo_min, lo_max = mine.lo_max, hi_min = mine.hi_min, hi_max = mine.hi_max;
     int start = it.first + split * it.chunk;
-    const int end = item_end(start, it.chunk, wg_hi);
-    if (start < wg_lo) start = wg_lo / kTileKeys * kTileKeys;
+    const int end = item_end(start, it.chunk, wg.hi_max);
+    if (start < wg.lo_min) start = wg.lo_min / kTileKeys * kTileKeys;
     const int all_tiles = end > start ? (end - start + kTileKeys - 1) / kTileKeys : 0;
     // Tile `tile` of this group is the (PARTS tile + part)-th.
     const int steps = (all_tiles + PARTS - 1) / PARTS, tiles = (all_tiles + PARTS - 1 - part) / PARTS;
@@ -574,6 +600,18 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
     };
     auto load_k = [&](const Place& p, int stage) { load(p.at, p.tokens, k_to + stage * (4 * kHalf)); };
     auto load_v = [&](const Place& p, int stage) { load(p.at + ((HD * 2) << log2), p.tokens, v_to + stage * (4 * kHalf)); };
+    int exp = 0;
+    if constexpr (BF16) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kKS; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(low16<true>(q[s][i])), fabsf(high16<true>(q[s][i]))));
+        exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)));
+        const float up = __builtin_ldexpf(1.0f, exp);
+#pragma unroll
+        for (int s = 0; s < kKS; ++s) q[s] = scaled_bf16(q[s], up);
+    }
     Place now = {}, next = {};                           // of this tile and the next
     if (tiles > 0) {
         now = locate(start);
@@ -585,32 +623,13 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
         load_k(next, 1);
     }
 
-    // This lane's query: columns 16 s + 8 half .. of the head.
-    u32x4 q[kKS];
-    int exp = 0;
-    {
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + row) * a.ld + (int64_t)head * HD + 8 * half;
-#pragma unroll
-        for (int s = 0; s < kKS; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s);
-        if constexpr (BF16) {
-            float mx = 0.0f;
-#pragma unroll
-            for (int s = 0; s < kKS; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(low16<true>(q[s][i])), fabsf(high16<true>(q[s][i]))));
-            exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)));
-            const float up = __builtin_ldexpf(1.0f, exp);
-#pragma unroll
-            for (int s = 0; s < kKS; ++s) q[s] = scaled_bf16(q[s], up);
-        }
-    }
     // Shaped scores are formed in powers of two, plain ones are products of the scaled query.
     const float unit = SHAPED ? 1.0f : unit_of(a.scale * kLog2e, exp);
     const float natural = unit_of(a.scale, exp), inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
     const float cap2 = a.softcap * kLog2e, cap_in = fminf(unit_of(a.scale, exp) * inv_cap * 2.8853900817779268f, __FLT_MAX__);
     const float slope = SHAPED && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
     const int pos = it.r.len - it.r.rows + row;
-    wait_vm_stores();                                    // the query, here: in the loop its wait would be one for the next tiles
+    wait_vm_stores();                                    // the first tiles
     lds_barrier();
 
     // Operand addresses: token col (+ 32) and chunk 2 s + half of K; of V, lane 4 m + j of
@@ -891,15 +910,21 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
     // This lane: columns 32 d + 8 j + 4 half + r of the head.
     if (it.splits == 1) {
         const float inv = 1.0f / l;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + ((int64_t)(it.r.row0 + row) * a.nh + head) * HD + 4 * half;
+        // Halves of a wave trade every other four columns: eight neighbouring ones a lane.
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + ((int64_t)(it.r.row0 + row) * a.nh + head) * HD + 8 * half;
 #pragma unroll
         for (int d = 0; d < kDb; ++d)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float y[4];
+            for (int j = 0; j < 4; j += 2) {
+                uint32_t w[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = blind ? 0.0f : acc[d][4 * j + r] * inv;
-                *reinterpret_cast<u32x2*>(dst + 32 * d + 8 * j) = u32x2{pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3])};
+                for (int i = 0; i < 4; ++i) {
+                    const int at = 4 * j + 2 * i;
+                    w[i] = blind ? 0u : pack2<BF16>(acc[d][at] * inv, acc[d][at + 1] * inv);
+                }
+                const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+                const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+                *reinterpret_cast<u32x4*>(dst + 32 * d + 8 * j) = u32x4{x[0], y[0], x[1], y[1]};
             }
     } else {
         float* dst = a.tile_part + (((int64_t)item * kvh + g) * k16Cols + local) * (HD + a.kExtra);
