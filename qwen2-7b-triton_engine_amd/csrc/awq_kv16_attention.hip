@@ -158,13 +158,14 @@ __global__ __launch_bounds__(kThreads, HD == 128 && !BF16 && SHAPED ? 2 : 3) voi
     __shared__ __align__(16) float o_lds[kWaves][kCols][kStride];
 
     Item it;
-    const int kvh = a.s.kvh, g = blockIdx.x % kvh, item = blockIdx.x / kvh;
+    uint32_t head_of;
+    const int kvh = a.s.kvh, item = (int)div_by(blockIdx.x, (uint32_t)kvh, a.kvh_inv, head_of), g = (int)head_of;
     if (!find_item<kCols, kKeys>(a, item, a.decode_target, it)) {
         if (blockIdx.x == gridDim.x - 1) fill_rows(a);   // the grid's last workgroup has no item
         return;
     }
     if (g == 0) write_records(a, it, false);
-    const int group = a.nh / kvh;
+    const int group = a.heads_each;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, t = lane >> 4;
@@ -437,11 +438,11 @@ struct Span {
 };
 // Of rows r0 .. r1 of a request, where no row has a first token of its own: both ends go up with the rows, and rows before the
 // request's first token see none.  Scalar work; over the lanes it took a workgroup 1.5 us.
-__device__ __forceinline__ Span rising_span(const Kv16AttnArgs& a, const Item& it, int n, int r0, int r1) {
+__device__ __forceinline__ Span rising_span(const Kv16AttnArgs& a, const Item& it, int n, int r0, int r1, int prefix) {
     const int none = it.r.rows - it.r.len;
     if (r0 < none) r0 = none;
     if (r0 > r1) return Span{n, 0, n, 0};
-    const auto x = a.range(it.b, it.r.row0, it.r.rows, it.r.len, r0), y = a.range(it.b, it.r.row0, it.r.rows, it.r.len, r1);
+    const auto x = a.seen(it.r.rows, it.r.len, r0, prefix, 0), y = a.seen(it.r.rows, it.r.len, r1, prefix, 0);
     return Span{x.lo, y.lo, x.hi, y.hi};
 }
 template <class Op>
@@ -488,24 +489,39 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
     __shared__ __align__(8) uint16_t odd_lds[PARTS][2][4];
 
     Item it;
-    const int kvh = a.s.kvh, g = blockIdx.x % kvh, item = blockIdx.x / kvh;
+    uint32_t head_of;
+    const int kvh = a.s.kvh, item = (int)div_by(blockIdx.x, (uint32_t)kvh, a.kvh_inv, head_of), g = (int)head_of;
     if (!find_item<k16Cols, kTileKeys>(a, item, a.tile_target, it)) {
         if (blockIdx.x == gridDim.x - 1 && a.limit == 0) fill_rows(a);
         return;
     }
     if (g == 0) write_records(a, it, true);
-    const int group = a.nh / kvh;
+    const int group = a.heads_each;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6 & 3), part = PARTS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int col = lane & 31, half = lane >> 5;
     // The last blocks, which see the most tokens, start first.
-    const int block = it.blocks - 1 - it.rel % it.blocks, split = it.rel / it.blocks;
+    const int split = it.rel / it.blocks, block = it.blocks - 1 - (it.rel - split * it.blocks);
     const int all_cols = columns(a, it.r.rows), c0 = block * k16Cols;
     const int n = walked(a, it.r.len);
 
-    const int local = 32 * wave + col, c = c0 + local, cc = c < all_cols ? c : all_cols - 1;
-    const int row = cc / group, head = g * group + cc % group;
-    // This lane's query: columns 16 s + 8 half .. of the head.  Asked for first: loads come back in order.
+    const int last = all_cols - 1, local = 32 * wave + col, c = c0 + local, cc = min(c, last);
+    auto over_group = [&](int column, uint32_t& rest) { return (int)div_by((uint32_t)column, (uint32_t)group, a.heads_inv, rest); };
+    auto row_of = [&](int column) {
+        uint32_t rest;
+        return over_group(column, rest);
+    };
+    uint32_t in_group;
+    const int row = over_group(cc, in_group), head = g * group + (int)in_group;
+    // Loads come back in order: what says which tokens are seen first, then this lane's query, columns 16 s + 8 half .. of the
+    // head, then the table and the tiles.
+    const int prefix = a.prefix ? a.prefix[it.b] : 0;
+    int first_of = 0, first_two[2] = {};                 // of this lane's column; of two of the workgroup's 128
+    if (a.first) {
+        first_of = a.first[it.r.row0 + row];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) first_two[i] = a.first[it.r.row0 + row_of(min(c0 + 64 * i + lane, last))];
+    }
     u32x4 q[kKS];
     {
         const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + row) * a.ld + (int64_t)head * HD + 8 * half;
@@ -513,27 +529,24 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
         for (int s = 0; s < kKS; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s);
         __builtin_amdgcn_sched_barrier(0);
     }
-    const auto sees = a.range(it.b, it.r.row0, it.r.rows, it.r.len, row);
+    const auto sees = a.seen(it.r.rows, it.r.len, row, prefix, first_of);
     const bool blind = sees.hi == 0;
     // What the workgroup's columns see, and the wave's.
     Span wg, mine;
     if (a.first) {
         wg = Span{n, 0, n, 0};
 #pragma unroll
-        for (int i = 0; i < k16Cols; i += 64) {          // two columns a lane
-            const int ci = c0 + i + lane;
-            if (ci < all_cols) {
-                const auto r = a.range(it.b, it.r.row0, it.r.rows, it.r.len, ci / group);
-                wg = Span{r.hi ? min(wg.lo_min, r.lo) : wg.lo_min, max(wg.lo_max, r.lo), r.hi ? min(wg.hi_min, r.hi) : wg.hi_min,
-                          max(wg.hi_max, r.hi)};
-            }
+        for (int i = 0; i < 2; ++i) {                    // (the last column again past it)
+            const auto r = a.seen(it.r.rows, it.r.len, row_of(min(c0 + 64 * i + lane, last)), prefix, first_two[i]);
+            wg = Span{r.hi ? min(wg.lo_min, r.lo) : wg.lo_min, max(wg.lo_max, r.lo), r.hi ? min(wg.hi_min, r.hi) : wg.hi_min,
+                      max(wg.hi_max, r.hi)};
         }
         wg = wave_span(wg);
         mine = wave_span(Span{blind ? n : sees.lo, sees.lo, blind ? n : sees.hi, sees.hi});
     } else {
-        const int last = all_cols - 1, w0 = c0 + 32 * wave;
-        wg = rising_span(a, it, n, c0 / group, min(c0 + k16Cols - 1, last) / group);
-        mine = rising_span(a, it, n, min(w0, last) / group, min(w0 + 31, last) / group);
+        const int w0 = c0 + 32 * wave;
+        wg = rising_span(a, it, n, row_of(c0), row_of(min(c0 + k16Cols - 1, last)), prefix);
+        mine = rising_span(a, it, n, row_of(min(w0, last)), row_of(min(w0 + 31, last)), prefix);
     }
     const int wg_lo_max = wg.lo_max, wg_hi_min = wg.hi_min;
     const int lo_min = mine.lo_min, lo_max = mine.lo_max, hi_min = mine.hi_min, hi_max = mine.hi_max;
@@ -954,6 +967,9 @@ hipError_t launch(Kv16AttnArgs a, hipStream_t stream) {
     a.decode_target = p.decode_target;
     a.tile_target = p.tile_target;
     a.combine = p.combine;
+    a.heads_each = a.nh / a.s.kvh;
+    a.heads_inv = div_inverse((uint32_t)a.heads_each);
+    a.kvh_inv = div_inverse((uint32_t)a.s.kvh);
     a.records = reinterpret_cast<i32x4*>(a.part);
     a.part += (size_t)a.total * (sizeof(i32x4) / sizeof(float));
     a.tile_part = a.part + p.decode_items * a.s.kvh * kCols * (HD + a.kExtra);

@@ -4,6 +4,7 @@
 //
 // Args, the kernels' argument block, has next to its fields
 //   kTileCols                       columns of a tile workgroup
+//   group()                         heads of a kv head
 //   first_key(rows, len)            the first token that a row of a request may see
 //   sees_none(b, row0, rows, len, i)   whether the i-th row of request b sees no token
 //   least_steps(steps, prompts)     steps of a tile item, from those that the target gives; prompts: nothing lies before the rows
@@ -58,7 +59,7 @@ template <class Args>
 __device__ __forceinline__ int walked(const Args& a, int len) { return walked_tokens(a.width, a.s.page_log2, len); }
 template <class Args>
 __device__ __forceinline__ int columns(const Args& a, int rows) {
-    return request_columns(rows, a.max_query, a.nh / a.s.kvh);
+    return request_columns(rows, a.max_query, a.group());
 }
 // Blocks of COLS columns that a request has in this kernel, and its tokens in steps of KEYS.
 template <int COLS, int KEYS, class Args>
@@ -216,7 +217,7 @@ template <int HD, int WAVES, bool BF16, class Args>
 __device__ __forceinline__ void combine_items(const Args& a) {
     constexpr int W = HD / 64;                           // columns a lane
     __shared__ float m_lds[kWaves], l_lds[kWaves], o_lds[kWaves][HD];
-    const int group = a.nh / a.s.kvh;
+    const int group = a.group();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int first = WAVES == 1 ? 0 : wave;
     const int64_t all = (int64_t)a.total * a.nh;

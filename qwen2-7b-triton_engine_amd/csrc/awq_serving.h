@@ -68,6 +68,7 @@ struct Kv4AttnArgs {
     // what awq_serve_walk.h asks for
     static constexpr int kTileCols = 64, kExtra = 2;
     static constexpr bool kEven = false, combine = true;
+    __device__ __forceinline__ int group() const { return nh / s.kvh; }
     __device__ __forceinline__ int least_steps(int steps, bool) const { return steps; }
     __device__ __forceinline__ int first_key(int, int) const { return 0; }
     __device__ __forceinline__ bool sees_none(int, int, int rows, int len, int i) const { return (int64_t)len - rows + i < 0; }
@@ -114,9 +115,12 @@ struct Kv16AttnArgs {
     i32x4* records;             // [total]
     int limit, decode_target, tile_target;
     bool combine;               // whether the joining launch follows
+    int heads_each;             // nh / kvh
+    uint32_t heads_inv, kvh_inv;   // div_inverse of it and of kvh
     // what awq_serve_walk.h asks for
     static constexpr int kTileCols = kTile16Cols, kExtra = 4;   // maximum, sum, unit, nothing
     static constexpr bool kEven = true;
+    __device__ __forceinline__ int group() const { return heads_each; }
     // Four tiles, sixteen of prompts, whose blocks see half of their items on average.  4 / 16: 300 rows behind
     // 1748 tokens 34 / 40 us, three chunks of up to 389 rows 42 / 46; prompts of 700 tokens 34 / 28, 1024 44 / 36.
     __device__ __forceinline__ int least_steps(int steps, bool prompts) const {
@@ -131,21 +135,19 @@ struct Kv16AttnArgs {
     struct Range {
         int lo, hi;
     };
-    __device__ __forceinline__ Range range(int b, int row0, int rows, int len, int i) const {
+    // of request b's prefix p and the row's first token f; 0: none
+    __device__ __forceinline__ Range seen(int rows, int len, int i, int p, int f) const {
         const int64_t pos = (int64_t)len - rows + i;
         int64_t lo = window ? pos - window + 1 : 0, hi = pos + 1;
-        if (prefix) {
-            const int p = prefix[b];
-            hi = hi > p ? hi : p < len ? p : len;
-        }
-        if (first) {
-            const int f = first[row0 + i];
-            lo = lo > f ? lo : f;
-        }
+        hi = hi > p ? hi : p < len ? p : len;
+        lo = lo > f ? lo : f;
         lo = lo > 0 ? lo : 0;
         if (pos < 0 || lo >= hi) return Range{0, 0};
         const int n = walked_tokens(width, s.page_log2, len);
         return Range{lo < n ? (int)lo : n - 1, hi < n ? (int)hi : n};
+    }
+    __device__ __forceinline__ Range range(int b, int row0, int rows, int len, int i) const {
+        return seen(rows, len, i, prefix ? prefix[b] : 0, first ? first[row0 + i] : 0);
     }
     __device__ __forceinline__ bool sees_none(int b, int row0, int rows, int len, int i) const {
         return range(b, row0, rows, len, i).hi == 0;
