@@ -437,7 +437,8 @@ struct Span {
     int lo_min, lo_max, hi_min, hi_max;
 };
 // Of rows r0 .. r1 of a request, where no row has a first token of its own: both ends go up with the rows, and rows before the
-// request's first token see none.  Scalar work; over the lanes it took a workgroup 1.5 us.
+// request's first token see none.  Scalar work: over the lanes, and with the query asked for
+// after it, a prompt of 256 rows took 16.4 us for 14.3.
 __device__ __forceinline__ Span rising_span(const Kv16AttnArgs& a, const Item& it, int n, int r0, int r1, int prefix) {
     const int none = it.r.rows - it.r.len;
     if (r0 < none) r0 = none;
@@ -470,13 +471,13 @@ __device__ __forceinline__ Span wave_span(const Span& s) {
 //
 // What bounds it: instructions.  The 64 x 32 exponentials and the steps around them take a wave as long as its
 // products, and two waves of a SIMD overlap the two only in part.  A prompt of 6001 rows, 28 heads of 128 over 4,
-// is 258 GFLOP in 306 us, 844 TFLOP/s, where a large product of a library reaches 1152; of zeros, at the clock that less power
-// allows, it took 252.  Behind them each workgroup costs 6 us of finding its item, pages, query and first tile,
-// so with few tiles the time is that: 256 rows take 16.5 us, 1024 36.
+// is 258 GFLOP in 305 us, 847 TFLOP/s, where a large product of a library reaches 1152; of zeros, at the clock that less power
+// allows, it took 252.  Before its first tile a workgroup spends 4 us on its item, the rows' ranges, the query and the table,
+// so with few tiles the time is that: 256 rows take 14.3 us, 1024 32.
 //
 // PARTS = 2: two groups of four waves take every other tile and meet through LDS, where whole workgroups of
-// four would be one round and leave CUs half empty (attention_plan16).  Prompts of 1200 / 1777 / 2300 rows: 31.5 / 48 / 63 us
-// against 36 / 55 / 69; with 6001, 349 against 311, for eight waves meet at each barrier.
+// four would be one round and leave CUs half empty (attention_plan16).  Prompts of 1200 / 1777 / 2300 rows: 29 / 41 / 62 us
+// against 35 / 50 / 67; with 6001, 325 against 305, for eight waves meet at each barrier.
 template <int HD, bool BF16, bool SHAPED, int PARTS>
 __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnArgs a) {
     constexpr int kKS = HD / 16;                         // k-steps of S

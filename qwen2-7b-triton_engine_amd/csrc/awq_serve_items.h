@@ -124,15 +124,23 @@ AttentionPlan attention_plan(int requests, int total, int max_query, int group, 
 // The same for the 16-bit cache, whose tiles have 128 columns: workgroups of four waves, two on a CU, or of eight
 // that share 128 columns' tokens.  Blocks that are fewer than half the places are split into one round of workgroups
 // and their sums joined by another launch; those that fit into the round as they are get eight waves each, and none joins.
-// One request, rows behind a context of 32768 tokens, split for four waves / for eight: 300 rows 179 / 192 us, 512 287 / 311,
-// 768 394 / 527 (its 42 blocks have 128 places a head or 64); prompts of 1200, 1777 and 2300 rows split / with
-// eight waves: 42 / 31.5, 61 / 48, 76 / 63 us.
+// One request, rows behind a context of 32768 tokens, split for four waves / for eight: 300 rows 174 / 195 us, 512 288 / 295,
+// 768 394 / 528 (its 42 blocks have 128 places a head or 64).  Prompts of 1200 / 1777 / 2300 rows: split 38 / 52 / 73 us,
+// whole with four waves 35 / 50 / 67, with eight 29 / 41 / 62.
 constexpr int kTile16Cols = 128, kRound16 = 512;
 struct AttentionPlan16 : AttentionPlan {
     int tile_parts;                    // 2: eight waves share the tokens of 128 columns
 };
 inline AttentionPlan16 attention_plan16(int requests, int total, int max_query, int group, int kvh) {
     AttentionPlan16 p = {attention_plan<kTile16Cols>(requests, total, max_query, group, kvh), 1};
+    if (p.decode && p.tile_target && 2 * (int64_t)total >= (int64_t)requests * max_query) {
+        // Requests are of max_query rows by half: as good as always none is the decode kernel's, and the tile kernel, which
+        // has all of them then, splits one that is.  Three chunks of up to 389 rows 41.0 us with its launch, 38.0
+        // without, sixteen of 64 rows behind 4032 tokens 60.3 and 57.0.
+        p.decode = false;
+        p.limit = p.decode_target = 0;
+        p.decode_items = 0;
+    }
     if (p.tile_target) {
         // One round of workgroups.  The blocks of one request are known, and so are their items; of several each
         // block may come out with an item more than its share (item_steps takes half of them off).

@@ -87,6 +87,14 @@ def test_attention(gpu, nh, kvh, hd, page, dtype, requests, features):
     O.check(_call(*args, **kw), *O.attention(args[0], args[1].data, *args[2:], **kw))
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("features", ["", "cap slopes window prefix first"])
+def test_a_chunk_beside_single_tokens(gpu, features, dtype):
+    """One request is the tile kernel's, the others the decode kernel's; then chunks of which one is a single token's."""
+    test_attention(gpu, 28, 4, 128, 64, dtype, [*DECODE[:5], (700, 300), *DECODE[5:]], features)
+    test_attention(gpu, 14, 2, 64, 32, dtype, [(900, 120), (1500, 1), (333, 150)], features)
+
+
 def test_split_along_the_tokens(gpu):
     """Few rows of long contexts are cut into items: decode and tiles, with a window that leaves out most of the context."""
     g = _gen(gpu, 2)
