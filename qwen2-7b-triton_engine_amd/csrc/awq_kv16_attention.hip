@@ -418,7 +418,7 @@ __device__ __forceinline__ void buffer_load_lds_4x4(u32x4 rsrc, uint32_t v0, uin
         "buffer_load_dwordx4 %0, %4, 0 offen lds\n\t"
         "buffer_load_dwordx4 %1, %4, 0 offen offset:1024 lds\n\t"
         "buffer_load_dwordx4 %2, %4, 0 offen offset:2048 lds\n\t"
-        "buffer_load_dwordx4 %3, %4, 0 offen offset:3072 lds"
+        "buffer_load_dwordx4 %3, %4, 0 offen offset:3*1024 lds"
         :
         : "v"(v0), "v"(v1), "v"(v2), "v"(v3), "s"(rsrc), "s"(lds_base)
         : "memory", "m0");

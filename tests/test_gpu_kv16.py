@@ -95,6 +95,14 @@ def test_a_chunk_beside_single_tokens(gpu, features, dtype):
     test_attention(gpu, 14, 2, 64, 32, dtype, [(900, 120), (1500, 1), (333, 150)], features)
 
 
+@pytest.mark.parametrize("features", ["", "cap slopes window prefix first"])
+def test_many_requests(gpu, features):
+    """More than a wave has lanes: single tokens, a few rows each with some that have none, and chunks alone."""
+    test_attention(gpu, 4, 2, 64, 16, "fp16", [(1 + 37 * i % 300, 1) for i in range(150)], features)
+    test_attention(gpu, 8, 2, 64, 32, "bf16", [(5 + 53 * i % 211, i % 4) for i in range(130)] + [(200, 90)], features)
+    test_attention(gpu, 4, 1, 128, 64, "fp16", [(41 + 17 * i % 400, 40) for i in range(70)], features)
+
+
 def test_split_along_the_tokens(gpu):
     """Few rows of long contexts are cut into items: decode and tiles, with a window that leaves out most of the context."""
     g = _gen(gpu, 2)
