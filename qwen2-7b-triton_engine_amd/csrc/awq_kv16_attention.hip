@@ -514,8 +514,8 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
     };
     uint32_t in_group;
     const int row = over_group(cc, in_group), head = g * group + (int)in_group;
-    // Loads come back in order: what says which tokens are seen first, then this lane's query, columns 16 s + 8 half .. of the
-    // head, then the table and the tiles.
+    // Loads come back in order: what says which tokens are seen first, then the table, then this lane's query, columns
+    // 16 s + 8 half .. of the head, then the tiles.
     const int prefix = a.prefix ? a.prefix[it.b] : 0;
     int first_of = 0, first_two[2] = {};                 // of this lane's column; of two of the workgroup's 128
     if (a.first) {
@@ -523,6 +523,26 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
 #pragma unroll
         for (int i = 0; i < 2; ++i) first_two[i] = a.first[it.r.row0 + row_of(min(c0 + 64 * i + lane, last))];
     }
+    // The table's entries from a tile's first page on are a lane's each, 64 of them; `lost` has a bit for
+    // those of the request's tokens that are no page of the cache.  First those from the item's begin on, which its
+    // first tile may lie behind.
+    int start = it.first + split * it.chunk;
+    const int32_t* table = a.tables + (int64_t)it.b * a.width;
+    const int log2 = a.s.page_log2;
+    const int held = (n + a.s.page() - 1) >> log2;       // pages of the request's tokens, one past the table's too
+    int first = 0, entry = 0;
+    uint64_t lost = 0;
+    auto ask = [&](int key0) {
+        first = __builtin_amdgcn_readfirstlane(key0 >> log2);
+        const int index = first + lane;
+        entry = index < min(a.width, held) ? table[index] : -1;
+    };
+    auto look = [&] {
+        const bool there = (uint32_t)entry < (uint32_t)a.s.num_pages;
+        lost = __ballot(!there && first + lane < held);
+        entry = there ? entry : 0;
+    };
+    ask(start);
     u32x4 q[kKS];
     {
         const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.r.row0 + row) * a.ld + (int64_t)head * HD + 8 * half;
@@ -551,7 +571,6 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
     }
     const int wg_lo_max = wg.lo_max, wg_hi_min = wg.hi_min;
     const int lo_min = mine.lo_min, lo_max = mine.lo_max, hi_min = mine.hi_min, hi_max = mine.hi_max;
-    int start = it.first + split * it.chunk;
     const int end = item_end(start, it.chunk, wg.hi_max);
     if (start < wg.lo_min) start = wg.lo_min / kTileKeys * kTileKeys;
     const int all_tiles = end > start ? (end - start + kTileKeys - 1) / kTileKeys : 0;
@@ -562,22 +581,7 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
 
     // Loads: wave w brings tokens 16 w .. of the tile.  A place past the
     // last token, or in a page outside the cache, lies past its resource's end and reads as zeros.
-    // The table's entries from a tile's first page on are a lane's each, 64 of them; `lost` has a bit for
-    // those of the request's tokens that are no page of the cache.
-    const int32_t* table = a.tables + (int64_t)it.b * a.width;
-    const int log2 = a.s.page_log2;
-    int first = 0, entry = 0;
-    uint64_t lost = 0;
-    auto fetch = [&](int key0) {
-        first = __builtin_amdgcn_readfirstlane(key0 >> log2);
-        const int index = first + lane;
-        const bool tokens = (int64_t)index << log2 < n;
-        entry = index < a.width && tokens ? table[index] : -1;
-        const bool there = entry >= 0 && entry < a.s.num_pages;
-        lost = __ballot(tokens && !there);
-        entry = there ? entry : 0;
-    };
-    fetch(start);
+    look();
     const uint64_t cache_g = reinterpret_cast<uint64_t>(a.cache) + 2 * g * a.s.block();
     const uint32_t page_bytes = (uint32_t)(2 * kvh * a.s.block());      // of all heads: 2^29 at most
     const int r0 = lane / kChunks;                       // a load's rows begin with this lane's token
@@ -589,7 +593,10 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
         uint32_t gone;                                   // the tile's blocks of 16 tokens in pages outside the cache, a bit each
     };
     auto locate = [&](int key0) {
-        if (((key0 + kTileKeys - 1) >> log2) - first >= 64) fetch(key0);
+        if (((key0 + kTileKeys - 1) >> log2) - first >= 64) {
+            ask(key0);
+            look();
+        }
         const int key = key0 + 16 * wave, left = n - key;
         Place p = {0, left < 16 ? (left > 0 ? left : 0) : 16, 0};
         if (lost) {
