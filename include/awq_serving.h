@@ -171,7 +171,8 @@ int awq_serve_kv16_append(const void* qkv, int64_t qkv_stride, void* cache, cons
  * A row that sees nothing (a negative position, first[i] past it) and a row of no request give zeros; rows past
  * max_query, and rows that see a token past the table or in a page outside the cache, NaN.  What a row does
  * not see may hold anything.  A row that sees a key of NaN, or a value that is not finite, is not finite: in the
- * columns that the arithmetic says, or in all of them.
+ * columns that the arithmetic says, or in all of them; likewise one whose scores, where softcap is 0 and slopes are given,
+ * pass 2^127.
  * Scores, softmax and sums are fp32; the probabilities enter the product with V in dtype where a request
  * has many rows (an error of half a step of dtype each, as the output's own), in two parts of dtype
  * otherwise.  bf16 queries are scaled by a power of two first.  scale positive and finite, softcap 0 or

@@ -91,10 +91,13 @@ template <bool BF16>
 constexpr float kSlack16 = BF16 ? 16.0f : 7.5f;
 
 // bf16 queries are brought to at most 2^8 by a power of two, so that a sum of products
-// stays inside fp32 for keys of ordinary size; fp16's are inside it as they are.  Returns the power's exponent.
+// stays inside fp32 for keys of ordinary size; fp16's are inside it as they are.  Under scales that would
+// bring what multiplies the products past 2^126 they stay larger instead, up to 2^108.  Returns the power's exponent.
 // mx: largest value of the row.
-__device__ __forceinline__ int query_exp(float mx) {
-    const int exp = 8 - __builtin_amdgcn_frexp_expf(mx);
+__device__ __forceinline__ int query_exp(float mx, float scale) {
+    int exp = 8 - __builtin_amdgcn_frexp_expf(mx);
+    const int over = __builtin_amdgcn_frexp_expf(scale) - exp - 126;
+    exp += over < 0 ? 0 : over < 100 ? over : 100;
     return exp < 100 ? exp : 100;
 }
 __device__ __forceinline__ u32x4 scaled_bf16(u32x4 w, float up) {
@@ -102,7 +105,7 @@ __device__ __forceinline__ u32x4 scaled_bf16(u32x4 w, float up) {
     for (int i = 0; i < 4; ++i) w[i] = pack2<true>(low16<true>(w[i]) * up, high16<true>(w[i]) * up);
     return w;
 }
-// What multiplies a product of the scaled query: kept finite (2^127 under a large scale passes fp32 here) and above zero
+// What multiplies a product of the scaled query: kept finite (an infinity times a product of 0 is NaN) and above zero
 // (a masked score times it is -infinity; 2^-149 of any product is nothing beside 1).
 __device__ __forceinline__ float unit_of(float factor, int exp) {
     return fminf(fmaxf(__builtin_ldexpf(factor, -exp), 0x1p-149f), __FLT_MAX__);
@@ -245,7 +248,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 && !BF16 && SHAPED ? 2 : 3) voi
 #pragma unroll
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(low16<true>(q[s][i])), fabsf(high16<true>(q[s][i]))));
         mx = fmaxf(mx, __shfl_xor(mx, 16));
-        exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)));
+        exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)), a.scale);
         const float up = __builtin_ldexpf(1.0f, exp);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) q[s] = scaled_bf16(q[s], up);
@@ -628,7 +631,7 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
         for (int s = 0; s < kKS; ++s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(low16<true>(q[s][i])), fabsf(high16<true>(q[s][i]))));
-        exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)));
+        exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)), a.scale);
         const float up = __builtin_ldexpf(1.0f, exp);
 #pragma unroll
         for (int s = 0; s < kKS; ++s) q[s] = scaled_bf16(q[s], up);
@@ -649,6 +652,7 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
     const float natural = unit_of(a.scale, exp), inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
     const float cap2 = a.softcap * kLog2e, cap_in = fminf(unit_of(a.scale, exp) * inv_cap * 2.8853900817779268f, __FLT_MAX__);
     const float slope = SHAPED && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    const float natural2 = fminf(natural * kLog2e, __FLT_MAX__);
     const int pos = it.r.len - it.r.rows + row;
     wait_vm_stores();                                    // the first tiles
     lds_barrier();
@@ -755,7 +759,7 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
         if constexpr (SHAPED) {
             if (a.softcap == 0.0f) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) s[i / 16][i % 16] *= natural * kLog2e;
+                for (int i = 0; i < 32; ++i) s[i / 16][i % 16] *= natural2;
             } else if (a.softcap <= kPlainCap) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {

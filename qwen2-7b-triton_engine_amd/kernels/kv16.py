@@ -99,6 +99,7 @@ def kv16_attention(q: torch.Tensor, cache: Kv16Cache, block_tables: torch.Tensor
 
     A row that sees no token, and a row of no request, gives zeros; one that sees a page outside the cache or a token
     past the table NaN; one that sees a key of NaN or a value that is not finite is not finite, in the columns that the
-    arithmetic says or in all.  What a row does not see may hold anything."""
+    arithmetic says or in all; so is one whose scores before the distance's part pass 2^127 (fp32 holds them) where ``slopes``
+    are given without a cap.  What a row does not see may hold anything."""
     return _native.binding().kv16_attention(q, cache.data, block_tables, seq_lens, query_start, max_query, scale, softcap, slopes,
                                             window, prefix, first)

@@ -1,0 +1,26 @@
+"""Scores of the 16-bit cache's attention (``kernels/kv16.py``) at the ends of fp32, against 64 bits."""
+import kv16_oracle as O
+import pytest
+import torch
+from test_gpu_kv16 import _batch, _call, _gen
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows", [1, 200])
+@pytest.mark.parametrize("tokens", [300, 3000])
+@pytest.mark.parametrize("scale", [768.0, 1e30, 3e38])
+def test_distances_under_large_scales(gpu, rows, tokens, scale):
+    """bf16 queries of 2^125, brought down by 2^118, under scales whose product with that is near fp32's largest number
+    or past it: keys of zero have a score of zero, and the distances alone weigh the tokens.  With keys of 2^-126 a
+    scale of 768 gives scores 384 apart, all of them inside fp32."""
+    g = _gen(gpu, 21)
+    q, cache, tables, lens, starts = _batch(g, [(tokens, rows), (64, 1)], nh=2, kvh=1, hd=128, page=64, dtype="bf16")
+    q = torch.where(q < 0, -(2.0**125), 2.0**125).to(torch.bfloat16)
+    cache.k.zero_()
+    slopes = torch.tensor([0.5, 0.03], device=gpu)
+    args = (q, cache, tables, lens, starts)
+    O.check(_call(*args, scale=scale, slopes=slopes), *O.attention(q, cache.data, *args[2:], scale=scale, slopes=slopes), "zeros")
+    if scale == 768.0:
+        cache.k.copy_(torch.randint(-1, 2, cache.k.shape, generator=g, device=gpu) * 2.0**-126)
+        O.check(_call(*args, scale=scale, slopes=slopes), *O.attention(q, cache.data, *args[2:], scale=scale, slopes=slopes), "small")
