@@ -1,7 +1,7 @@
-// How attention over the paged cache is cut into items (csrc/awq_serve_attention.hip):
-// the arithmetic that its kernels, their grids and the workspace have in common.
+// How attention over the paged caches is cut into items (csrc/awq_serve_attention.hip for 4 bits,
+// csrc/awq_kv16_attention.hip for 16): the arithmetic that the kernels, their grids and the workspace have in common.
 // Plain C++ without the HIP headers (constexpr functions are the device's too), so that
-// tests/test_attention_items.py runs it on the host: every item has to have a
+// tests/test_attention_items.py and tests/test_attention16_cuts.py run it on the host: every item has to have a
 // workgroup, and every item that is one of several a place for its sums.
 #pragma once
 
@@ -83,6 +83,10 @@ constexpr int item_steps(int target, int64_t work, int all_blocks, int requests)
                : work == 0 ? 1 : work < most ? (int)((work + target - 1) / target) : kMost;
 }
 constexpr int request_splits(int steps, int item) { return (int)((uint32_t)(steps + item - 1) / (uint32_t)item); }
+// The 16-bit cache's tiles: at least four steps an item, sixteen of prompts (nothing lies before the rows), whose blocks see half
+// of their items on average.  4 / 16: 300 rows behind 1748 tokens 34 / 40 us, three chunks of up to 389 rows 42 / 46; prompts of
+// 700 tokens 34 / 28, 1024 44 / 36.
+constexpr int least_tile_steps(int steps, bool prompts) { return steps < (prompts ? 16 : 4) ? (prompts ? 16 : 4) : steps; }
 // Steps of an item of that request with its items made alike: as many items, none longer.
 constexpr int even_steps(int steps, int splits) { return splits > 1 ? (int)((uint32_t)(steps + splits - 1) / (uint32_t)splits) : steps; }
 // Where an item ends that begins at `start`, of a block that sees `limit` tokens.

@@ -121,12 +121,7 @@ struct Kv16AttnArgs {
     static constexpr int kTileCols = kTile16Cols, kExtra = 4;   // maximum, sum, unit, nothing
     static constexpr bool kEven = true;
     __device__ __forceinline__ int group() const { return heads_each; }
-    // Four tiles, sixteen of prompts, whose blocks see half of their items on average.  4 / 16: 300 rows behind
-    // 1748 tokens 34 / 40 us, three chunks of up to 389 rows 42 / 46; prompts of 700 tokens 34 / 28, 1024 44 / 36.
-    __device__ __forceinline__ int least_steps(int steps, bool prompts) const {
-        const int least = prompts ? 16 : 4;
-        return steps < least ? least : steps;
-    }
+    __device__ __forceinline__ int least_steps(int steps, bool prompts) const { return least_tile_steps(steps, prompts); }
     __device__ __forceinline__ int first_key(int rows, int len) const {
         return first_token(window, rows, len, walked_tokens(width, s.page_log2, len));
     }
