@@ -137,25 +137,39 @@ struct AttentionPlan16 : AttentionPlan {
 };
 inline AttentionPlan16 attention_plan16(int requests, int total, int max_query, int group, int kvh) {
     AttentionPlan16 p = {attention_plan<kTile16Cols>(requests, total, max_query, group, kvh), 1};
-    if (p.decode && p.tile_target && 2 * (int64_t)total >= (int64_t)requests * max_query) {
+    if (!p.tile) return p;
+    // Blocks of columns at most, and those to count with: each request may have one more than its columns fill.  Beside the
+    // decode kernel only requests of more columns than that takes count, and all have a row as good as always: 64 single
+    // tokens beside a chunk are not 64 blocks more, which would leave the chunk's few unsplit.  Split / whole: 300 rows behind
+    // 32768 tokens beside 64 tokens behind 2000 each 256 / 587 us, 40 behind 4096 beside 128 behind 1000 each 65 / 140; a prompt
+    // of 300 rows beside 64 tokens behind 2000 each 63 / 61.
+    auto least = [](int64_t x, int64_t y) { return x < y ? x : y; };
+    const int64_t rows = least((int64_t)requests * max_query, total), full = rows * group / kTile16Cols;
+    const int64_t few = kDecodeColumns / group;          // rows that the decode kernel takes
+    int64_t most = full + (p.decode ? least(requests, rows / (few + 1)) : requests);
+    int64_t blocks = full + (p.decode ? least(requests, rows > requests ? (rows - requests) / few : 0) : requests);
+    if (p.decode && (full + requests) * kvh < kSplitBelow && 2 * (int64_t)total >= (int64_t)requests * max_query) {
         // Requests are of max_query rows by half: as good as always none is the decode kernel's, and the tile kernel, which
         // has all of them then, splits one that is.  Three chunks of up to 389 rows 41.0 us with its launch, 38.0
-        // without, sixteen of 64 rows behind 4032 tokens 60.3 and 57.0.
+        // without, sixteen of 64 rows behind 4032 tokens 60.3 and 57.0; a token behind 32768 beside a prompt of 700 rows
+        // 50 and 31, beside 300 rows behind 3796 tokens 65 and 51.
         p.decode = false;
         p.limit = p.decode_target = 0;
         p.decode_items = 0;
+        most = blocks = full + requests;
     }
-    if (p.tile_target) {
+    p.tile_target = 0;
+    if (blocks * kvh < kSplitBelow) {
         // One round of workgroups.  The blocks of one request are known, and so are their items; of several each
         // block may come out with an item more than its share (item_steps takes half of them off).
-        const int64_t blocks = p.tile_items - p.tile_target - 1, all = kvh < kRound16 ? kRound16 / kvh : 1;
+        const int64_t all = kvh < kRound16 ? kRound16 / kvh : 1;
         const int64_t mine = ((int64_t)(max_query < total ? max_query : total) * group + kTile16Cols - 1) / kTile16Cols;
         const int64_t target = requests > 1 ? all - blocks / 2 : mine > 0 ? all / mine * mine : 1;
         p.tile_target = (int)(target > (all + 3) / 4 ? target : (all + 3) / 4);
-        p.tile_items = blocks + p.tile_target + 1;
-    } else if (p.tile && p.tile_items * kvh <= kRound16) {
-        p.tile_parts = 2;
     }
+    p.tile_items = most + p.tile_target + 1;
+    p.combine = p.decode || p.tile_target;
+    if (!p.tile_target && p.tile_items * kvh <= kRound16) p.tile_parts = 2;
     return p;
 }
 

@@ -45,3 +45,14 @@ def test_one_request_of_every_row_count(cuts, steps):
             if rows <= n:
                 cuts([(n, rows)], 7, 4).check()
                 cuts([(n, n)], 7, 4).check()
+
+
+@pytest.mark.parametrize("decodes", [0, 1, 8, 32, 64, 200])
+def test_a_chunk_beside_single_tokens_keeps_its_split(cuts, decodes):
+    """300 rows behind 32768 tokens are 17 blocks of a kv head: whole, each would walk over all of the tokens by itself."""
+    for single in (1, 2000):
+        c = cuts([(single + 7 * i, 1) for i in range(decodes)] + [(32768, 300)], 7, 4).check()
+        assert c.tile_sums and c.parts == 1 and c.tile_splits >= 4 and c.tile_longest <= 128, c
+    # in front of the chunk, and several chunks
+    c = cuts([(32768, 300)] + [(500, 1)] * decodes + [(20000, 150)], 7, 4).check()
+    assert c.tile_sums and c.tile_splits >= 2, c
