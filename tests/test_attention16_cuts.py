@@ -2,6 +2,7 @@
 import random
 
 import kv16_cuts
+import kv16_plans
 import pytest
 
 
@@ -56,3 +57,13 @@ def test_a_chunk_beside_single_tokens_keeps_its_split(cuts, decodes):
     # in front of the chunk, and several chunks
     c = cuts([(32768, 300)] + [(500, 1)] * decodes + [(20000, 150)], 7, 4).check()
     assert c.tile_sums and c.tile_splits >= 2, c
+
+
+@pytest.mark.parametrize("name", kv16_plans.PLANS)
+def test_the_batches_of_the_long_plans(cuts, name):
+    """What ``kv16_plans`` says of each of its batches."""
+    nh, kvh, _, page, requests, want = kv16_plans.PLANS[name]
+    c = cuts(requests, nh // kvh, kvh, page=page).check()
+    assert {k: getattr(c, k) for k in want} == want, c
+    if name.startswith("split"):
+        assert c.tile_splits > 1 and c.tile_longest * 64 > 64 * page, c
