@@ -15,22 +15,13 @@ namespace awq {
 namespace {
 
 constexpr int k16Cols = Kv16AttnArgs::kTileCols;
-constexpr float kLog2e = 1.4426950408889634f;
 typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // ---- 16-bit operands of either type, eight in four words ---------------------------
 
-template <bool BF16>
-__device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c) {
-    if constexpr (BF16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else
-        return mfma16x16x32(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c);
-}
 template <bool BF16>
 __device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
     if constexpr (BF16)

@@ -17,18 +17,7 @@
 namespace awq {
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-
-template <bool BF16>
-__device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c) {
-    if constexpr (BF16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else
-        return mfma16x16x32(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c);
-}
-
 constexpr int kBK = 64;                // k of a step: rows of 128 bytes in LDS
-constexpr float kLog2e = 1.4426950408889634f;
 
 // WV x WT waves of FV x FT blocks of 16 vocabulary rows x 16 tokens, S stages of LDS.
 template <int WV, int WT, int FV, int FT, int S, int PER_CU>

@@ -222,6 +222,18 @@ __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
     *reinterpret_cast<u32x4*>(p) = w;
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A product of 16-bit operands of either type, eight in four words.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+template <bool BF16>
+__device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return mfma16x16x32(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c);
+}
+
 // A barrier for LDS alone: loads from memory stay in flight across it.
 __device__ __forceinline__ void lds_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
