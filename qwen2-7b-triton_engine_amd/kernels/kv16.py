@@ -7,7 +7,8 @@ RoPE of q and k (``kernels/rope.py:41-57``), k and v stored by a step's slots
 (``kernels.paged``).  ``kv16_attention`` is softmax(score) V for all rows of a batch, one token of
 each request or chunks of prompts (``model/qwen2.py:104-163``), and serves scores that the
 reference's model has no use for: capped by a tanh, with a bias for the distance; and rows that see a
-sliding window, a document of a packed text, or a prefix as a whole.
+sliding window, a document of a packed text, or a prefix as a whole.  Neither is differentiable: results
+carry no gradient.
 """
 from __future__ import annotations
 
@@ -100,6 +101,9 @@ def kv16_attention(q: torch.Tensor, cache: Kv16Cache, block_tables: torch.Tensor
     A row that sees no token, and a row of no request, gives zeros; one that sees a page outside the cache or a token
     past the table NaN; one that sees a key of NaN or a value that is not finite is not finite, in the columns that the
     arithmetic says or in all; so is one whose scores before the distance's part pass 2^127 (fp32 holds them) where ``slopes``
-    are given without a cap.  What a row does not see may hold anything."""
+    are given without a cap.  What a row does not see may hold anything.
+
+    Scores and sums are fp32; of requests with many rows each probability is rounded to the cache's type before its product
+    with V (half a step, as the result's own rounding), of the others it is held in two such parts."""
     return _native.binding().kv16_attention(q, cache.data, block_tables, seq_lens, query_start, max_query, scale, softcap, slopes,
                                             window, prefix, first)

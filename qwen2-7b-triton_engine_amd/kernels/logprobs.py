@@ -21,5 +21,6 @@ def token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
 
     ``hidden`` fp16 or bf16 ``[T, K]`` (any row stride), ``weight`` ``[V, K]`` of the same type (``nn.Linear.weight``), K a
     multiple of 64, ``targets`` int64 or int32 ``[T]``: a negative one (no target) gives 0, one of V or more NaN.
-    Products are exact and summed in fp32."""
+    Products are exact and summed in fp32.  Not differentiable: the results carry no gradient, whatever the inputs.  A
+    ``weight`` that is not contiguous, or does not begin on 16 bytes, is copied whole in each call."""
     return _native.binding().token_logprobs(hidden, weight, targets)
