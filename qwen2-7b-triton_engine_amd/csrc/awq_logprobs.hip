@@ -9,9 +9,9 @@
 // column, so that its maximum and sum are a lane's own up to two cross-lane steps.
 //
 // What bounds it: with up to 128 tokens the weight's bytes, read once.  152064 rows of 3584 are 1.09 GB: one token 182 us
-// (6.0 TB/s), 64 209, 128 245.  With many the product: 2047 tokens are 2.23 TFLOP in 1951 us, 1144 TFLOP/s, where a
-// library's product of the same sizes takes 1816 (1228) and leaves 622 MB of logits; power holds the clock at 1.8 GHz.  Between them,
-// at 256 tokens, both: 349 us.
+// (6.0 TB/s), 64 209, 128 245.  With many the product: 2047 tokens are 2.23 TFLOP in 1927 us, 1158 TFLOP/s (1881 to 1951 from
+// run to run), where a library's product of the same sizes takes 1799 (1240) and leaves 622 MB of logits; power holds the clock at
+// 1.8 GHz.  Between them, at 256 tokens, both: 349 us.
 #include "awq_serving.h"
 
 namespace awq {
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(L::kThreads, L::kPerCu * L::kWaves / 4) void awq_lo
                 x[h][t] = *reinterpret_cast<const u32x4*>(st + L::BV * 128 + (wt * FT + t) * 2048 + (frag ^ (64 * h)));
         };
         // The second half's operands are read under the first's products, and a wave that has all of its operands goes
-        // before one that is reading: 2047 tokens 1951 us for 2019 without, 512 535 for 561.
+        // before one that is reading: 2047 tokens 1951 us for 2019 without, 512 535 for 561 (in turn, in one run).
         read(0);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -220,8 +220,11 @@ using Narrow = LpTile<4, 1, 2, 4, 3, 2>;     // 128 x 64
 using Thin = LpTile<4, 1, 2, 1, 4, 2>;       // 128 x 16
 
 // Many tokens: the tiles that take least, by what one of them costs where there are several (Middle 126 us for 152064 rows
-// of 3584, Tall 150, Wide 218).  Wide / Tall / Middle there, us: 160 tokens 334 / 268 / 327,
+// of 3584, Tall 150, Wide 218).  Wide / Tall / Middle there, in one run, us: 160 tokens 334 / 268 / 327,
 // 256 345 / 389 / 350, 300 484 / 398 / 438, 384 505 / 520 / 462, 512 530 / 682 / 621, 2047 1906 / 2252 / 2185.
+// The vocabulary does not enter: from 50000 rows on the choice is within 4 % of the best; with fewer the tiles leave CUs
+// empty, and smaller ones would take less.  Wide / Middle / Narrow / Thin, 256 tokens: 1000 rows 85 / 54 / 32 / 21, 4000
+// 88 / 56 / 34 / 32, 16000 87 / 57 / 45 / 99, 50000 116 / 135 / 175 / 362.
 template <class F>
 auto with_tile(int tokens, F f) {
     if (tokens <= 16) return f(Thin{});

@@ -126,11 +126,14 @@ AttentionPlan attention_plan(int requests, int total, int max_query, int group, 
 }
 
 // The same for the 16-bit cache, whose tiles have 128 columns: workgroups of four waves, two on a CU, or of eight
-// that share 128 columns' tokens.  Blocks that are fewer than half the places are split into one round of workgroups
-// and their sums joined by another launch; those that fit into the round as they are get eight waves each, and none joins.
+// that share 128 columns' tokens.  Blocks that are fewer than half the places of four waves are split into one round of
+// workgroups and their sums joined by another launch; those that fit into that round as they are get eight waves each (of heads
+// of 128, with twice the LDS, one on a CU: a second round begins past 256), and none joins.
 // One request, rows behind a context of 32768 tokens, split for four waves / for eight: 300 rows 174 / 195 us, 512 288 / 295,
 // 768 394 / 528 (its 42 blocks have 128 places a head or 64).  Prompts of 1200 / 1777 / 2300 rows: split 38 / 52 / 73 us,
-// whole with four waves 35 / 50 / 67, with eight 29 / 41 / 62.
+// whole with four waves 35 / 50 / 67, with eight 29 / 41 / 62.  256 / 320 / 400 / 500 blocks of 16 kv heads, four waves and eight:
+// causal 55 45 / 69 54 / 86 68 / 108 95, nine documents 26 22 / 28 27 / 40 35 / 58 43; nine documents of 28 heads over 4
+// 16 15 / 19 23 / 31 29 / 30 32; heads of 64, causal 54 55 / 63 47 / 78 59 / 96 80.
 constexpr int kTile16Cols = 128, kRound16 = 512;
 struct AttentionPlan16 : AttentionPlan {
     int tile_parts;                    // 2: eight waves share the tokens of 128 columns
