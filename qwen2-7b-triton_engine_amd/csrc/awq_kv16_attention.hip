@@ -82,12 +82,13 @@ template <bool BF16>
 constexpr float kSlack16 = BF16 ? 16.0f : 7.5f;
 
 // bf16 queries are brought to at most 2^8 by a power of two, so that a sum of products
-// stays inside fp32 for keys of ordinary size; fp16's are inside it as they are.  Under scales that would
-// bring what multiplies the products past 2^126 they stay larger instead, up to 2^108.  Returns the power's exponent.
-// mx: largest value of the row.
+// stays inside fp32 for keys of ordinary size; fp16's are inside it as they are.  Returns the power's exponent.
+// mx: largest value of the row.  scale: of scores that meet the distance's part as they are, 0 of others (plain ones count by
+// their differences, capped ones end at the cap).  Such scores are formed, and under scales that would bring what multiplies
+// the products past 2^126 the query stays larger instead, up to 2^108.
 __device__ __forceinline__ int query_exp(float mx, float scale) {
     int exp = 8 - __builtin_amdgcn_frexp_expf(mx);
-    const int over = __builtin_amdgcn_frexp_expf(scale) - exp - 126;
+    const int over = scale > 0.0f ? __builtin_amdgcn_frexp_expf(scale) - exp - 126 : 0;
     exp += over < 0 ? 0 : over < 100 ? over : 100;
     return exp < 100 ? exp : 100;
 }
@@ -239,7 +240,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 && !BF16 && SHAPED ? 2 : 3) voi
 #pragma unroll
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(low16<true>(q[s][i])), fabsf(high16<true>(q[s][i]))));
         mx = fmaxf(mx, __shfl_xor(mx, 16));
-        exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)), a.scale);
+        exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)), SHAPED && a.softcap == 0.0f ? a.scale : 0.0f);
         const float up = __builtin_ldexpf(1.0f, exp);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) q[s] = scaled_bf16(q[s], up);
@@ -622,7 +623,7 @@ __global__ __launch_bounds__(256 * PARTS, 2) void awq_kv16_tile_kernel(Kv16AttnA
         for (int s = 0; s < kKS; ++s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(low16<true>(q[s][i])), fabsf(high16<true>(q[s][i]))));
-        exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)), a.scale);
+        exp = query_exp(fmaxf(mx, __shfl_xor(mx, 32)), SHAPED && a.softcap == 0.0f ? a.scale : 0.0f);
         const float up = __builtin_ldexpf(1.0f, exp);
 #pragma unroll
         for (int s = 0; s < kKS; ++s) q[s] = scaled_bf16(q[s], up);
